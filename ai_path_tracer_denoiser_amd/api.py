@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -30,6 +31,10 @@ DN_BN_BATCH, DN_BN_RUNNING, DN_HIDDEN_CARRY, DN_HIDDEN_RESET = 1, 0, 2, 0
 DN_IMPL_MFMA, DN_IMPL_VALU, DN_IMPL_MFMA_F16X3, DN_IMPL_MFMA_F16W = 0, 1, 2, 3
 DN_OPT_R_MINPIX, DN_OPT_F16_MINPIX, DN_OPT_SMALL_MINPIX, DN_OPT_FUSED_POOL, DN_OPT_KY_SPLIT = 1, 2, 3, 4, 5
 GEOM_SPHERE, GEOM_CUBE = 0, 1
+STREAM_DEFAULT = -1                                     # Context(stream=...): HIP's default stream, torch's own unless told otherwise
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+ACTIVATIONS = {"none": 0, "leaky": 1, "silu": 2, "gelu": 3}
+NORMS = {"rms": 0, "layer": 1}
 
 
 class Geom(C.Structure):
@@ -66,6 +71,7 @@ _P = C.c_void_p
 ABI = [
     ("aipt_create", C.c_int, [C.c_int, _P, C.POINTER(_P)]),
     ("aipt_destroy", None, [_P]),
+    ("aipt_stream", C.c_int, [_P, C.POINTER(_P)]),
     ("aipt_last_error", C.c_char_p, [_P]),
     ("aipt_abi_version", C.c_int, []),
     ("aipt_sync", C.c_int, [_P]),
@@ -117,6 +123,18 @@ ABI = [
     ("aipt_frame_set_timing", C.c_int, [_P, C.c_int]),
     ("aipt_frame_last_times", C.c_int, [_P, C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     ("aipt_frame_prefetch", C.c_int, [_P, _P, C.c_int, C.c_int, C.c_uint32]),
+    ("aipt_linear_workspace", C.c_int, [_P, C.c_char_p, C.POINTER(C.c_size_t)]),
+    ("aipt_linear", C.c_int, [_P, C.c_char_p, _P, C.c_size_t]),
+    ("aipt_linear_backward_workspace", C.c_int, [_P, C.c_char_p, C.POINTER(C.c_size_t)]),
+    ("aipt_linear_backward", C.c_int, [_P, C.c_char_p, _P, C.c_size_t]),
+    ("aipt_block_norm", C.c_int, [_P, C.c_char_p]),
+    ("aipt_block_norm_backward_workspace", C.c_int, [_P, C.c_char_p, C.POINTER(C.c_size_t)]),
+    ("aipt_block_norm_backward", C.c_int, [_P, C.c_char_p, _P, C.c_size_t]),
+    ("aipt_adamw_state_elements", C.c_longlong, [_P, C.c_int]),
+    ("aipt_adamw_workspace", C.c_longlong, [_P, C.c_int]),
+    ("aipt_adamw_create", C.c_int, [_P, _P, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, C.POINTER(_P)]),
+    ("aipt_adamw_step", C.c_int, [_P, _P] + [C.c_double] * 5 + [C.c_uint32]),
+    ("aipt_adamw_destroy", None, [_P]),
     ("aipt_comm_create", C.c_int, [C.POINTER(_P), C.c_int, C.c_int, C.POINTER(_P)]),
     ("aipt_comm_is_rccl", C.c_int, [_P]),
     ("aipt_comm_broadcast", C.c_int, [_P, C.POINTER(_P), C.c_size_t, C.c_int]),
@@ -138,6 +156,13 @@ ABI = [
     ("aipt_camera_orbit_params", None, [C.POINTER(Camera)] + [C.POINTER(C.c_float)] * 3),
     ("aipt_camera_orbit", None, [C.POINTER(Camera), C.c_float, C.c_float, C.c_float]),
 ]
+
+# the argument records of the layer operators (include/aiptd.h), packed by field: a ctypes structure costs a small call more than its kernel
+_LINEAR = struct.Struct("@iifi3q" + "Pqq" * 5 + "P")                 # aipt_linear_args
+_LINEAR_GRAD = struct.Struct("@iifi3q" + "Pqq" * 6 + "P")            # aipt_linear_grad_args
+_NORM = struct.Struct("@iifi2q4P4q6PP")                              # aipt_block_norm_args
+_NORM_GRAD = struct.Struct("@4i2q4PP5P2P6q6P")                       # aipt_block_norm_grad_args
+_ADAMW_TENSOR = struct.Struct("@3Pqfi")                              # aipt_adamw_tensor
 
 _LIB = None
 
@@ -256,7 +281,8 @@ class Scene:
 
 
 class Context:
-    """One context per GPU (aipt_create).  stream: a raw hipStream_t handle (int) or None."""
+    """One context per GPU (aipt_create).  stream: a raw hipStream_t handle (int), STREAM_DEFAULT (torch's default stream) or None (a stream of
+    the context's own)."""
 
     def __init__(self, device: int = 0, stream=None):
         L = lib()
@@ -267,6 +293,7 @@ class Context:
         self._h = h
         self.device = device
         self._keep = []
+        self._stream, self._ext = None, None             # of the layer operators: the context's stream (handle; torch object)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -481,3 +508,279 @@ class Context:
         a, b = C.c_float(), C.c_float()
         self._ck(lib().aipt_frame_last_times(self._h, C.byref(a), C.byref(b)))
         return a.value, b.value
+
+    # ------------------------------------------------------------------ layer operators
+    # Tensors are torch's; the work runs on the context's stream.  Where that is not torch's current stream, the call waits for what is
+    # queued there and what is queued there later waits for the call, so that tensors may be used, and freed, like in any torch program.
+    def _on_stream(self, entry, *args):
+        import torch
+        if self._stream is None:
+            p = _P()
+            self._ck(lib().aipt_stream(self._h, C.byref(p)))
+            self._stream = p.value or 0
+            # (ExternalStream takes 0 for "none given" and makes a new stream)
+            self._ext = torch.cuda.ExternalStream(self._stream, device=self.device) if self._stream else torch.cuda.default_stream(self.device)
+        if torch._C._cuda_getCurrentRawStream(self.device) == self._stream:
+            return self._ck(entry(self._h, *args))
+        now = torch.cuda.current_stream(self.device)
+        if not self._stream and torch.cuda.is_current_stream_capturing():
+            raise AiptError("a context on the default stream cannot take part in a capture: make one with stream=<the capturing stream's handle>")
+        self._ext.wait_stream(now)
+        rc = entry(self._h, *args)
+        now.wait_stream(self._ext)
+        self._ck(rc)
+
+    def _scratch(self, entry, record):
+        """(memory or None, its address, bytes) of an operator's workspace: torch's, so that a captured graph keeps its own"""
+        n = C.c_size_t()
+        self._ck(entry(self._h, record, C.byref(n)))
+        if not n.value:
+            return None, None, 0
+        import torch
+        t = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", self.device))
+        return t, t.data_ptr(), n.value
+
+    def _type(self, t):
+        kind = _types().get(t.dtype)
+        if kind is None or not t.is_cuda or t.get_device() != self.device:
+            raise AiptError(f"a {t.dtype} tensor on {t.device}: float32, bfloat16 or float16 on cuda:{self.device} is wanted")
+        return kind
+
+    def _want(self, name, t, dtype, *shape):
+        if t.dtype != dtype or not t.is_cuda or t.get_device() != self.device or tuple(t.shape) != shape:
+            raise AiptError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; {dtype} {shape} on cuda:{self.device} is wanted")
+
+    def _matrix(self, name, t, dtype, rows, cols):
+        """(address, row stride, column stride) of an optional matrix"""
+        if t is None:
+            return 0, 0, 0
+        self._want(name, t, dtype, rows, cols)
+        return (t.data_ptr(), *t.stride())
+
+    def _vector(self, name, t, dtype, n):
+        if t is None:
+            return 0
+        self._want(name, t, dtype, n)
+        if n > 1 and t.stride(0) != 1:
+            raise AiptError(f"{name}: stride {t.stride(0)}")
+        return t.data_ptr()
+
+    def linear(self, x, w, y, bias=None, residual=None, preact=None, act: str = "none", slope: float = 0.1):
+        """aipt_linear: y = act(x w^T + bias) + residual.  x [m, k], w [n, k], y [m, n] -- each with unit stride along either axis, so a planar
+        feature map [channels, pixels] comes as its .t() -- bias [n], residual [m, n] (may be y); preact [m, n] receives x w^T + bias, which
+        linear_backward of an activation wants.  All float32, bfloat16 or float16.  act: none, leaky (slope), silu, gelu."""
+        kind, d = self._type(x), x.dtype
+        if x.dim() != 2 or w.dim() != 2:
+            raise AiptError(f"linear: x {tuple(x.shape)}, w {tuple(w.shape)}")
+        (m, k), n = x.shape, w.shape[0]
+        record = _LINEAR.pack(kind, _choice("act", act, ACTIVATIONS), slope, 0, m, n, k, *self._matrix("x", x, d, m, k), *self._matrix("w", w, d, n, k),
+                              *self._matrix("y", y, d, m, n), *self._matrix("residual", residual, d, m, n),
+                              *self._matrix("preact", preact, d, m, n), self._vector("bias", bias, d, n))
+        hold, ptr, size = self._scratch(lib().aipt_linear_workspace, record)
+        self._on_stream(lib().aipt_linear, record, ptr, size)
+        return y
+
+    def linear_backward(self, dy, x, w, preact=None, act: str = "none", slope: float = 0.1, dx=None, dw=None, dbias=None):
+        """aipt_linear_backward: gradients of linear() into dx [m, k], dw [n, k], dbias [n], each or None (the residual's is dy).  preact: what
+        linear() kept; not needed with act "none".  x is looked at for dw alone, w for dx alone: either may be None without."""
+        kind, d = self._type(dy), dy.dtype
+        if dy.dim() != 2:
+            raise AiptError(f"linear_backward: dy {tuple(dy.shape)}")
+        if (dw is not None and x is None) or (dx is not None and w is None):
+            raise AiptError("linear_backward: dw wants x, dx wants w")
+        (m, n), like = dy.shape, x if x is not None else w if w is not None else None
+        if like is not None and like.dim() != 2:
+            raise AiptError(f"linear_backward: x or w {tuple(like.shape)}")
+        k = like.shape[1] if like is not None else 0
+        act = _choice("act", act, ACTIVATIONS)
+        if act and preact is None:
+            raise AiptError("linear_backward: an activation wants preact")
+        record = _LINEAR_GRAD.pack(kind, act, slope, 0, m, n, k, *self._matrix("dy", dy, d, m, n), *self._matrix("x", x, d, m, k),
+                                   *self._matrix("w", w, d, n, k), *self._matrix("preact", preact, d, m, n), *self._matrix("dx", dx, d, m, k),
+                                   *self._matrix("dw", dw, d, n, k), self._vector("dbias", dbias, d, n))
+        hold, ptr, size = self._scratch(lib().aipt_linear_backward_workspace, record)
+        self._on_stream(lib().aipt_linear_backward, record, ptr, size)
+
+    def _rows(self, name, t, dtype, rows, c):
+        """(address, row stride) of an optional [rows, c] with contiguous rows"""
+        if t is None:
+            return 0, 0
+        self._want(name, t, dtype, rows, c)
+        if c > 1 and t.stride(1) != 1:
+            raise AiptError(f"{name}: stride {t.stride(1)} between the channels of a row")
+        return t.data_ptr(), t.stride(0)
+
+    def _gates(self, name, t, dtype, c, groups):
+        if t is None:
+            return 0
+        if t.dim() != 2 or not t.is_contiguous():
+            raise AiptError(f"{name}: {tuple(t.shape)} contiguous [groups, channels] is wanted")
+        self._want(name, t, dtype, groups, c)
+        return t.data_ptr()
+
+    def _stats(self, stats, rows):
+        if stats is None:
+            return 0
+        import torch
+        self._want("stats", stats, torch.float32, rows, 4)
+        if not stats.is_contiguous():
+            raise AiptError("stats is not contiguous")
+        return stats.data_ptr()
+
+    def block_norm(self, y, x, h, z=None, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, kind: str = "rms",
+                   eps: float = 1e-5, stats=None):
+        """aipt_block_norm: the norm behind a residual block, its gate and residual scale, and the norm before the next block:
+        h = x + scale * gate * (norm(y) * post_weight + post_bias), z = norm(h) * pre_weight + pre_bias.  y (None: no block yet, h = x), x, h (may
+        be x), z (None: no norm) [rows, channels]; gate [groups, channels], one for each rows / groups rows; the rest [channels]; stats
+        float32 [rows, 4] receives what block_norm_backward wants.  kind: rms, or layer (which alone has biases)."""
+        t, d = self._type(x), x.dtype
+        if x.dim() != 2:
+            raise AiptError(f"block_norm: x {tuple(x.shape)}")
+        rows, c = x.shape
+        groups = gate.shape[0] if gate is not None and gate.dim() == 2 else 1
+        (xp, xs), (yp, ys), (hp, hs), (zp, zs) = self._rows("x", x, d, rows, c), self._rows("y", y, d, rows, c), self._rows("h", h, d, rows, c), self._rows("z", z, d, rows, c)
+        record = _NORM.pack(t, _choice("kind", kind, NORMS), eps, c, rows, groups, xp, yp, hp, zp, xs, ys, hs, zs, self._gates("gate", gate, d, c, groups),
+                            self._vector("scale", scale, d, c), self._vector("post_weight", post_weight, d, c), self._vector("post_bias", post_bias, d, c),
+                            self._vector("pre_weight", pre_weight, d, c), self._vector("pre_bias", pre_bias, d, c), self._stats(stats, rows))
+        self._on_stream(lib().aipt_block_norm, record)
+        return h, z
+
+    def block_norm_backward(self, dh, dz, y, h, stats, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None, kind: str = "rms",
+                            dx=None, dy=None, dgate=None, dscale=None, dpost_weight=None, dpost_bias=None, dpre_weight=None, dpre_bias=None):
+        """aipt_block_norm_backward: gradients of block_norm() from dh (None: zero) and dz (None: there was no z), with y, h and stats as it left
+        them, into dx (may be dh), dy and the parameters' gradients, each or None."""
+        like = dh if dh is not None else dz
+        if like is None or like.dim() != 2:
+            raise AiptError("block_norm_backward: dh or dz [rows, channels] is wanted")
+        t, d = self._type(like), like.dtype
+        rows, c = like.shape
+        g = gate if gate is not None else dgate
+        groups = g.shape[0] if g is not None and g.dim() == 2 else 1
+        r = [self._rows(n, v, d, rows, c) for n, v in (("dh", dh), ("dz", dz), ("y", y), ("h", h), ("dx", dx), ("dy", dy))]
+        vec = [self._vector(n, v, d, c) for n, v in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("dscale", dscale),
+                                                     ("dpost_weight", dpost_weight), ("dpost_bias", dpost_bias), ("dpre_weight", dpre_weight), ("dpre_bias", dpre_bias))]
+        record = _NORM_GRAD.pack(t, _choice("kind", kind, NORMS), c, 0, rows, groups, r[0][0], r[1][0], r[2][0], r[3][0], self._stats(stats, rows),
+                                 self._gates("gate", gate, d, c, groups), *vec[:4], r[4][0], r[5][0], r[0][1], r[1][1], r[2][1], r[3][1], r[4][1], r[5][1],
+                                 self._gates("dgate", dgate, d, c, groups), *vec[4:])
+        hold, ptr, size = self._scratch(lib().aipt_block_norm_backward_workspace, record)
+        self._on_stream(lib().aipt_block_norm_backward, record, ptr, size)
+
+    def adamw(self, params, grads, copies=None, weight_decay=0.01, state_bits: int = 32, state=None) -> "AdamW":
+        """A plan for AdamW steps over these tensors (class AdamW)."""
+        return AdamW(self, params, grads, copies, weight_decay, state_bits, state)
+
+
+def _types():
+    global _TYPES
+    if _TYPES is None:
+        import torch
+        _TYPES = {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
+    return _TYPES
+
+
+_TYPES = None
+
+
+def _choice(name, value, choices):
+    if value not in choices:
+        raise AiptError(f"{name} {value!r}: one of {', '.join(choices)} is wanted")
+    return choices[value]
+
+
+class AdamW:
+    """AdamW over many tensors at once (aipt_adamw_*; the reference trains with torch's Adam, training/train.py:54-112).
+
+    params: contiguous float32 tensors; grads: as many, of the same sizes, all float32, bfloat16 or float16; copies: None, or bfloat16 or
+    float16 tensors that receive the rounded parameters (an entry may be None); weight_decay: a number, or one for each tensor.  The plan is
+    bound to these tensors' memory: a gradient that is replaced by another tensor, or storage that moves, is bound anew with bind().
+    state: None (zeros, step 0) or the dict that state() of an earlier plan of the same sizes returned, which goes on being updated in place:
+    step int32 [1]; m and v float32 (state_bits 32), or m, v float8_e4m3fn with m_scale, v_scale float32 for each 256 elements (state_bits
+    8; v holds the second moment's root); tensor i begins at element 256 * (number of 256-blocks of the tensors before it).
+    norm: float32 [1], the gradients' norm at the last update that clipped."""
+
+    def __init__(self, ctx, params, grads, copies=None, weight_decay=0.01, state_bits=32, state=None):
+        import torch
+        self.ctx, self._h = ctx, None
+        params = list(params)
+        copies = list(copies) if copies is not None else [None] * len(params)
+        decay = [float(weight_decay)] * len(params) if isinstance(weight_decay, (int, float)) else [float(v) for v in weight_decay]
+        if not (len(params) == len(copies) == len(decay)):
+            raise AiptError(f"adamw: {len(params)} params, {len(copies)} copies, {len(decay)} weight_decay")
+        if state_bits not in (8, 32):
+            raise AiptError(f"adamw: state_bits {state_bits}: 32 or 8 is wanted")
+        self._params, self._copies, self._decay, self.state_bits = params, copies, decay, state_bits
+        dev = torch.device("cuda", ctx.device)
+        n = len(params)
+        counts = (C.c_longlong * max(1, n))(*[p.numel() for p in params])
+        total, need = lib().aipt_adamw_state_elements(counts, n), lib().aipt_adamw_workspace(counts, n)
+        if total < 0 or need < 0:
+            raise AiptError("adamw: a tensor has too many elements")
+        kind, blocks = torch.float32 if state_bits == 32 else torch.float8_e4m3fn, total // 256
+        want = {"m": (kind, total), "v": (kind, total), "step": (torch.int32, 1)}
+        if state_bits == 8:
+            want.update(m_scale=(torch.float32, blocks), v_scale=(torch.float32, blocks))
+        if state is None:
+            state = {k: torch.zeros(size, device=dev, dtype=torch.uint8 if t.itemsize == 1 else t).view(t) for k, (t, size) in want.items()}
+        if set(state) != set(want):
+            raise AiptError(f"adamw: state has {sorted(state)}, {sorted(want)} are wanted")
+        for k, (t, size) in want.items():
+            ctx._want("state " + k, state[k], t, size)
+            if not state[k].is_contiguous():
+                raise AiptError(f"adamw: state {k} is not contiguous")
+        self._state = dict(state)
+        self.norm = torch.zeros(1, device=dev)
+        self._scratch = torch.zeros(need, device=dev, dtype=torch.uint8)
+        self.bind(grads)
+
+    def bind(self, grads):
+        """Bind the plan to these gradients, and to where the parameters and copies lie now."""
+        import torch
+        grads, ctx = list(grads), self.ctx
+        if len(grads) != len(self._params):
+            raise AiptError(f"adamw: {len(self._params)} params, {len(grads)} grads")
+        kinds = {g.dtype for g in grads} or {torch.float32}
+        copies = {c.dtype for c in self._copies if c is not None} or {torch.bfloat16}
+        if len(kinds) != 1 or not kinds <= set(_types()) or len(copies) != 1 or not copies <= {torch.bfloat16, torch.float16}:
+            raise AiptError("adamw: gradients of one type (float32, bfloat16, float16) and copies of one (bfloat16, float16) are wanted")
+        records = []
+        for i, (p, g, c, d) in enumerate(zip(self._params, grads, self._copies, self._decay)):
+            for name, t, kind in (("param", p, torch.float32), ("grad", g, g.dtype), ("copy", c, None if c is None else c.dtype)):
+                if t is not None:
+                    ctx._want(f"{name} {i}", t, kind, *p.shape)
+                    if not t.is_contiguous():
+                        raise AiptError(f"adamw: {name} {i} is not contiguous")
+            records.append(_ADAMW_TENSOR.pack(p.data_ptr(), g.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), d, 0))
+        s, h = self._state, _P()
+        ptr = {k: s[k].data_ptr() if k in s else None for k in ("m", "v", "m_scale", "v_scale", "step")}
+        ctx._ck(lib().aipt_adamw_create(ctx._h, b"".join(records), len(records), _types()[kinds.pop()], _types()[copies.pop()], self.state_bits, ptr["m"], ptr["v"],
+                                        ptr["m_scale"], ptr["v_scale"], ptr["step"], self.norm.data_ptr(), self._scratch.data_ptr(), self._scratch.numel(), C.byref(h)))
+        self.close()
+        self._h, self._grads = h, grads
+        self._held = [t for t in (*self._params, *grads, *self._copies, *s.values()) if t is not None]
+        self._at = [t.data_ptr() for t in self._held]
+
+    def state(self) -> dict:
+        """The state tensors themselves, to be saved, or to go on from in another plan."""
+        return dict(self._state)
+
+    def update(self, lr: float, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8, max_norm: float = None, seed: int = 0):
+        """One step.  max_norm: clip the gradients' norm to this (None: no clipping); a step whose norm is not finite then changes nothing.  seed: key of
+        the chances by which 8-bit state is rounded.  A captured step replays its lr; the step number goes on with every replay."""
+        if not self._h:
+            raise AiptError("adamw: the plan is closed")
+        if [t.data_ptr() for t in self._held] != self._at:
+            raise AiptError("adamw: a tensor's storage has moved: bind() the plan anew")
+        if max_norm is not None and not max_norm > 0:
+            raise AiptError(f"adamw: max_norm {max_norm}")
+        self.ctx._on_stream(lib().aipt_adamw_step, self._h, lr, beta1, beta2, eps, 0.0 if max_norm is None else max_norm, seed & 0xffffffff)
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().aipt_adamw_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

@@ -57,7 +57,9 @@ int aipt_create(int device, void* stream, aipt_ctx** out) {
     aipt_ctx* ctx = new (std::nothrow) aipt_ctx();
     if (!ctx) return fail(nullptr, AIPT_E_NOMEM, "aipt_create: out of host memory");
     ctx->device = device;
-    if (stream) {
+    if (stream == AIPT_STREAM_DEFAULT) {
+        ctx->stream = nullptr;
+    } else if (stream) {
         ctx->stream = (hipStream_t)stream;
     } else {
         e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking);
@@ -101,6 +103,13 @@ void aipt_destroy(aipt_ctx* ctx) {
     for (auto& ev : ctx->fev) if (ev) hipEventDestroy(ev);
     if (ctx->own_stream) hipStreamDestroy(ctx->stream);
     delete ctx;
+}
+
+int aipt_stream(const aipt_ctx* ctx, void** stream_out) {
+    AIPT_CHECK_CTX(ctx);
+    if (!stream_out) return AIPT_E_INVALID;
+    *stream_out = (void*)ctx->stream;
+    return AIPT_OK;
 }
 
 const char* aipt_last_error(const aipt_ctx* ctx) {

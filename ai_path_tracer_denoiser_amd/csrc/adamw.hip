@@ -1,0 +1,463 @@
+// adamw.hip -- one AdamW step over many tensors (aipt_adamw_*).
+//
+// What it cannot do without: p in and out, the gradient, the state in and out -- 28 bytes a parameter with fp32 state and gradients,
+// 14 with 8-bit state and bf16 gradients -- and some 40 operations on them: memory bounds it, and for small sets the launch.  So: ONE
+// launch over all tensors (their pointers travel in the kernel arguments, up to TENSORS of them, which a captured graph keeps by
+// itself), a wave per 256-element block (16-byte accesses, and the block's scale is a wave's own maximum), and the step number on the
+// device, advanced by the last workgroup, so that neither the host nor a second launch has a part in it.
+#include "layer_ops.h"
+
+#include <cmath>
+#include <new>
+
+namespace aipt {
+
+constexpr int BLOCK = 256;           // elements that share a scale; what one wave handles at a time
+constexpr int TENSORS = 112;         // of one launch: 112 x 33 bytes + the scalars stay below 4 KB of kernel arguments
+constexpr int GRID = 2048;           // most workgroups of a launch: 8 a CU; the blocks beyond 4 a workgroup go round
+constexpr size_t SCRATCH = 256;      // bytes of the workspace before the partial sums
+constexpr float TOP = 448.f;         // largest e4m3
+constexpr float LIVE = 0x1p-100f;    // blocks below this are kept as zeros (448 / top stays finite)
+
+struct AdamTensor {
+    float* p;
+    const void* g;
+    void* copy;
+    unsigned first;                  // its first block in the launch's numbering
+    float decay;
+};
+
+struct AdamTable {
+    AdamTensor t[TENSORS];
+    unsigned char tail[TENSORS];     // elements of its last block, less one
+    int n;
+    unsigned blocks;                 // of this launch
+};
+
+struct AdamArgs {
+    AdamTable tab;
+    unsigned long long state0;       // the first block's place among the state's blocks
+    void *m, *v;
+    float *ms, *vs;
+    int* step;
+    const float* clip;               // {norm, factor}, or NULL
+    unsigned* ticket;                // workgroups done; non-NULL on the step's last launch: advances `step`
+    double b1, b2;                   // the powers are taken of the betas as given ...
+    float lr, beta1, beta2, eps;
+    float omb1, omb2;                // ... and 1 - beta is rounded once: 1 - 0.999f is 5e-5 off 0.001
+    unsigned seed;
+    int pad;
+};
+static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
+
+template <typename G> __device__ inline void load4(const G* g, float* o);
+template <> __device__ inline void load4<float>(const float* g, float* o) {
+    const float4 q = *(const float4*)g;
+    o[0] = q.x; o[1] = q.y; o[2] = q.z; o[3] = q.w;
+}
+template <> __device__ inline void load4<bf16>(const bf16* g, float* o) {
+    struct alignas(8) Q { bf16 v[4]; } q = *(const Q*)g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = (float)q.v[i];
+}
+template <> __device__ inline void load4<f16>(const f16* g, float* o) {
+    struct alignas(8) Q { f16 v[4]; } q = *(const Q*)g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = (float)q.v[i];
+}
+
+// e4m3 <-> float: the chip's own conversions (OCP e4m3 on gfx950; to nearest even, and these values are at most 448)
+__device__ inline void from_e4m3(unsigned q, float* o) {
+    o[0] = __builtin_amdgcn_cvt_f32_fp8(q, 0);
+    o[1] = __builtin_amdgcn_cvt_f32_fp8(q, 1);
+    o[2] = __builtin_amdgcn_cvt_f32_fp8(q, 2);
+    o[3] = __builtin_amdgcn_cvt_f32_fp8(q, 3);
+}
+__device__ inline unsigned to_e4m3(const float* o) {
+    int q = __builtin_amdgcn_cvt_pk_fp8_f32(o[0], o[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(o[2], o[3], q, true);
+}
+
+// 24 random bits as a number in [0, 1) from a place and a key: multiplications by odd constants (fractions of the golden ratio and of
+// the roots of 3 and 5) carry low bits up, the shifts bring high ones down
+__device__ inline float uniform(unsigned long long place, unsigned key) {
+    unsigned x = (unsigned)(place ^ (place >> 32)) ^ key;
+    x *= 0x9E3779B1u; x ^= x >> 15;
+    x *= 0xBB67AE85u; x ^= x >> 13;
+    x *= 0x3C6EF373u; x ^= x >> 16;
+    return (float)(x >> 8) * 0x1p-24f;
+}
+
+// x >= 0 to one of the two e4m3 values around it, up with the probability of its distance from the lower one: the mean is x
+__device__ inline float chance_e4m3(float x, float u) {
+    const int e = max((int)(__float_as_uint(x) >> 23) - 127, -6);          // below 2^-6 the steps stay 2^-9
+    const float unit = __uint_as_float((unsigned)(e - 3 + 127) << 23), inv = __uint_as_float((unsigned)(3 - e + 127) << 23);
+    return fminf(floorf(x * inv + u) * unit, TOP);
+}
+
+// Where block b lies: `ti` its tensor (blocks only grow, so a wave's search goes on from its last one's), `at` the lane's first element,
+// the return value how many of the lane's four exist (<= 0: none).
+__device__ inline int locate(const AdamTable& tab, unsigned b, int lane, int& ti, long long& at) {
+    int hi = tab.n;
+    while (hi - ti > 1) {
+        const int mid = (ti + hi) >> 1;
+        if (tab.t[mid].first <= b) ti = mid; else hi = mid;
+    }
+    const unsigned next = ti + 1 < tab.n ? tab.t[ti + 1].first : tab.blocks;
+    at = (long long)(b - tab.t[ti].first) * BLOCK + lane * 4;
+    return (b + 1 == next ? (int)tab.tail[ti] + 1 : BLOCK) - lane * 4;
+}
+
+template <typename G, typename C, int BITS>
+__global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
+    __shared__ float bias[2];
+    float factor = 1.f;
+    bool skip = false;
+    if (a.clip) {
+        factor = a.clip[1];
+        skip = !(a.clip[0] <= 3.4028235e38f);                              // inf and NaN
+    }
+    const int step = *a.step + 1;
+    if (threadIdx.x < 2) {                                                 // 1 - beta^t without the cancellation, in fp64
+        const double b = threadIdx.x ? a.b2 : a.b1;
+        bias[threadIdx.x] = (float)-expm1((double)step * log(b));
+    }
+    __syncthreads();
+    const float rate = a.lr / bias[0], root2 = 1.f / sqrtf(bias[1]);
+    const unsigned key = a.seed + (unsigned)step * 0x9E3779B1u;
+    const int lane = threadIdx.x & 63;
+    const unsigned waves = gridDim.x * 4;
+    int ti = 0;
+    if (!skip)
+        for (unsigned b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b < a.tab.blocks; b += waves) {
+            long long at;
+            const int left = locate(a.tab, b, lane, ti, at);
+            const AdamTensor& t = a.tab.t[ti];
+            const unsigned long long sb = a.state0 + b, place = sb * BLOCK + lane * 4;
+            const G* gp = (const G*)t.g + at;
+            float* pp = t.p + at;
+            C* cp = t.copy ? (C*)t.copy + at : nullptr;
+            const bool wide = left >= 4 && !(((uintptr_t)t.p & 15) | ((uintptr_t)t.g & (4 * sizeof(G) - 1)) | ((uintptr_t)t.copy & (4 * sizeof(C) - 1)));
+            float p[4] = {}, g[4] = {}, m[4], v[4];
+            if (wide) {
+                load4<float>(pp, p);
+                load4<G>(gp, g);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (i < left) { p[i] = pp[i]; g[i] = (float)gp[i]; }
+            }
+            if constexpr (BITS == 32) {
+                load4<float>((const float*)a.m + place, m);
+                load4<float>((const float*)a.v + place, v);
+            } else {
+                from_e4m3(((const unsigned*)a.m)[place >> 2], m);
+                from_e4m3(((const unsigned*)a.v)[place >> 2], v);
+                const float ms = a.ms[sb], vs = a.vs[sb];
+#pragma unroll
+                for (int i = 0; i < 4; i++) { m[i] *= ms; v[i] *= vs; v[i] *= v[i]; }
+            }
+            const float keep = 1.f - a.lr * t.decay;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float gi = g[i] * factor;
+                m[i] = m[i] * a.beta1 + gi * a.omb1;
+                v[i] = v[i] * a.beta2 + gi * gi * a.omb2;
+                p[i] = p[i] * keep - rate * m[i] / (sqrtf(v[i]) * root2 + a.eps);
+            }
+            if (wide) {
+                *(float4*)pp = make_float4(p[0], p[1], p[2], p[3]);
+                if (cp) {
+                    struct alignas(4 * sizeof(C)) Q { C v[4]; } q;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) q.v[i] = (C)p[i];
+                    *(Q*)cp = q;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (i < left) { pp[i] = p[i]; if (cp) cp[i] = (C)p[i]; }
+            }
+            if constexpr (BITS == 32) {
+                *(float4*)((float*)a.m + place) = make_float4(m[0], m[1], m[2], m[3]);
+                *(float4*)((float*)a.v + place) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                float mt = 0, vt = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (i >= left) { m[i] = 0; v[i] = 0; }                 // the padding stays zero whatever was in it
+                    v[i] = sqrtf(v[i]);
+                    mt = fmaxf(mt, fabsf(m[i])); vt = fmaxf(vt, v[i]);
+                }
+                mt = wave_max(mt); vt = wave_max(vt);
+                const float mi = mt >= LIVE ? TOP / mt : 0.f, vi = vt >= LIVE ? TOP / vt : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    m[i] = fminf(fmaxf(m[i] * mi, -TOP), TOP);
+                    const float c = chance_e4m3(v[i] * vi, uniform(place + i, key));
+                    v[i] = c == 0.f && v[i] > 0.f && vi > 0.f ? 0x1p-9f : c;
+                }
+                ((unsigned*)a.m)[place >> 2] = to_e4m3(m);
+                ((unsigned*)a.v)[place >> 2] = to_e4m3(v);
+                if (lane == 0) {
+                    a.ms[sb] = mt >= LIVE ? mt / TOP : 0.f;
+                    a.vs[sb] = vt >= LIVE ? vt / TOP : 0.f;
+                }
+            }
+        }
+    // the last workgroup of the step's last launch advances the step number: every workgroup has read it before it takes its ticket
+    if (a.ticket && threadIdx.x == 0) {
+        __threadfence();
+        if (atomicAdd(a.ticket, 1u) == gridDim.x - 1) {
+            *a.ticket = 0;
+            if (!skip) *a.step = step;
+        }
+    }
+}
+
+// ---- the norm of all gradients: partial sums of squares in fixed places, then one workgroup.  It reads the gradients once more than the
+// step itself would, and there is no way round it: no parameter may change before the last gradient has been seen.
+struct NormArgs {
+    AdamTable tab;
+    float* partial;                  // one for each workgroup
+};
+template <typename G>
+__global__ __launch_bounds__(256) void grad_square(const NormArgs a) {
+    const int lane = threadIdx.x & 63;
+    const unsigned waves = gridDim.x * 4;
+    int ti = 0;
+    float s = 0;
+    for (unsigned b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b < a.tab.blocks; b += waves) {
+        long long at;
+        const int left = locate(a.tab, b, lane, ti, at);
+        const AdamTensor& t = a.tab.t[ti];
+        const G* gp = (const G*)t.g + at;
+        float g[4] = {};
+        if (left >= 4 && !((uintptr_t)t.g & (4 * sizeof(G) - 1))) load4<G>(gp, g);
+        else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) if (i < left) g[i] = (float)gp[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s += g[i] * g[i];
+    }
+    __shared__ float part[4];
+    s = wave_sum(s);
+    if (lane == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+}
+struct NormEndArgs {
+    const float* partial;
+    int n;
+    float max_norm;
+    float* clip;
+    float* norm;
+};
+__global__ __launch_bounds__(256) void grad_norm_end(const NormEndArgs a) {
+    double s = 0;
+    for (int i = threadIdx.x; i < a.n; i += 256) s += (double)a.partial[i];
+    __shared__ double part[256];
+    part[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const float norm = (float)sqrt(part[0]);
+        a.clip[0] = norm;
+        a.clip[1] = fminf(1.f, a.max_norm / (norm + 1e-6f));
+        *a.norm = norm;
+    }
+}
+
+}  // namespace aipt
+
+static_assert(sizeof(aipt_adamw_tensor) == 40, "argument record (api.py packs it by field)");
+
+struct aipt_adamw {
+    aipt_ctx* ctx = nullptr;
+    int grad_type = 0, copy_type = 0, bits = 0;
+    std::vector<aipt::AdamArgs> launches;
+    std::vector<unsigned> grids, norm_grids;
+    long long blocks = 0;
+    unsigned* ticket = nullptr;      // the caller's workspace: ticket, clip[2] at 64, partial sums at SCRATCH
+    float* clip = nullptr;
+    float* partial = nullptr;
+    int npartial = 0;
+    float* norm = nullptr;
+};
+
+namespace aipt {
+
+typedef void (*AdamKernel)(AdamArgs);
+typedef void (*NormKernel)(NormArgs);
+template <typename G> static AdamKernel adam_of(int copy_type, int bits) {
+    if (copy_type == AIPT_TYPE_BF16) return bits == 32 ? adamw_step<G, bf16, 32> : adamw_step<G, bf16, 8>;
+    return bits == 32 ? adamw_step<G, f16, 32> : adamw_step<G, f16, 8>;
+}
+
+}  // namespace aipt
+
+using aipt::fail;
+
+extern "C" {
+
+long long aipt_adamw_state_elements(const long long* counts, int n) {
+    if (n < 0 || (n > 0 && !counts)) return AIPT_E_INVALID;
+    long long blocks = 0;
+    for (int i = 0; i < n; i++) {
+        if (counts[i] < 0 || counts[i] > (1ll << 40)) return AIPT_E_INVALID;
+        blocks += (counts[i] + aipt::BLOCK - 1) / aipt::BLOCK;
+    }
+    return blocks * aipt::BLOCK;
+}
+
+long long aipt_adamw_workspace(const long long* counts, int n) {
+    if (aipt_adamw_state_elements(counts, n) < 0) return AIPT_E_INVALID;
+    // a partial sum for each workgroup of each launch; a launch ends with TENSORS tensors or where the next would not fit its block count
+    const size_t blocks = (size_t)aipt_adamw_state_elements(counts, n) / aipt::BLOCK;
+    const size_t launches = 1 + (size_t)n / aipt::TENSORS + 2 * (blocks / 0xf0000000ull);
+    return (long long)(aipt::SCRATCH + launches * aipt::GRID * sizeof(float));
+}
+
+int aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, int grad_type, int copy_type, int state_bits,
+                      void* m, void* v, float* m_scale, float* v_scale, int* step, float* norm, void* d_workspace,
+                      size_t workspace_bytes, aipt_adamw** out) {
+    if (!out) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: out is NULL");
+    *out = nullptr;
+    if (n < 0 || (n > 0 && !tensors)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: %d tensors", n);
+    if (!aipt::type_ok(grad_type)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: grad_type %d", grad_type);
+    if (copy_type != AIPT_TYPE_BF16 && copy_type != AIPT_TYPE_F16) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: copy_type %d (bf16 or f16)", copy_type);
+    if (state_bits != 32 && state_bits != 8) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: state_bits %d (32 or 8)", state_bits);
+    if (!step || !norm || !d_workspace) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: step, norm or d_workspace is NULL");
+    long long blocks = 0;
+    for (int i = 0; i < n; i++) {
+        const aipt_adamw_tensor& t = tensors[i];
+        if (t.count < 0 || t.count > (1ll << 40)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: tensor %d has %lld elements", i, t.count);
+        if (t.count && (!t.param || !t.grad)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: tensor %d: NULL param or grad", i);
+        const size_t ga = aipt::type_bytes(grad_type) - 1;
+        if (((uintptr_t)t.param & 3) || ((uintptr_t)t.grad & ga) || ((uintptr_t)t.copy & 1)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: tensor %d: misaligned pointer", i);
+        if (!std::isfinite(t.weight_decay)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: tensor %d: weight_decay is not finite", i);
+        blocks += (t.count + aipt::BLOCK - 1) / aipt::BLOCK;
+    }
+    if (blocks && (!m || !v)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: m or v is NULL");
+    if (blocks && state_bits == 8 && (!m_scale || !v_scale)) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: 8-bit state wants m_scale and v_scale");
+    const size_t sa = state_bits == 32 ? 15 : 3;
+    if (((uintptr_t)m & sa) || ((uintptr_t)v & sa) || ((uintptr_t)m_scale & 3) || ((uintptr_t)v_scale & 3) || ((uintptr_t)step & 3) || ((uintptr_t)norm & 3) || ((uintptr_t)d_workspace & 15))
+        return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: m and v are aligned to four elements, scales, step and norm to one, d_workspace to 16 bytes");
+    // what a step writes may not be what it reads elsewhere: sorted by address, neighbours are apart
+    {
+        std::vector<aipt::Extent> mem;
+        std::vector<int> rank;
+        try {
+            auto add = [&](const void* q, long long bytes, bool written) { if (q && bytes) { mem.push_back({(const char*)q, 1, bytes, bytes}); rank.push_back(written); } };
+            for (int i = 0; i < n; i++) {
+                add(tensors[i].param, tensors[i].count * 4, true);
+                add(tensors[i].copy, tensors[i].count * 2, true);
+                add(tensors[i].grad, tensors[i].count * aipt::type_bytes(grad_type), false);
+            }
+            const long long el = blocks * aipt::BLOCK, sb = state_bits == 32 ? 4 : 1;
+            add(m, el * sb, true); add(v, el * sb, true);
+            if (state_bits == 8) { add(m_scale, blocks * 4, true); add(v_scale, blocks * 4, true); }
+            add(step, 4, true); add(norm, 4, true); add(d_workspace, (long long)workspace_bytes, true);
+            std::vector<size_t> order(mem.size());
+            for (size_t i = 0; i < order.size(); i++) order[i] = i;
+            std::sort(order.begin(), order.end(), [&](size_t x, size_t y) { return mem[x].data < mem[y].data; });
+            const char *end_any = nullptr, *end_written = nullptr;       // furthest end so far, of all and of what is written
+            for (size_t i : order) {
+                if (mem[i].data < end_written || (rank[i] && mem[i].data < end_any))
+                    return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: memory that a step writes overlaps another tensor's, the state's, step or norm");
+                const char* e = mem[i].data + mem[i].len;
+                end_any = std::max(end_any, e);
+                if (rank[i]) end_written = std::max(end_written, e);
+            }
+        } catch (const std::bad_alloc&) {
+            return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
+        }
+    }
+    AIPT_NEED_CTX(ctx);
+    aipt_adamw* a = new (std::nothrow) aipt_adamw();
+    if (!a) return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
+    a->ctx = ctx; a->grad_type = grad_type; a->copy_type = copy_type; a->bits = state_bits; a->blocks = blocks; a->norm = norm;
+    try {
+        unsigned long long state0 = 0;
+        for (int i = 0; i < n;) {
+            aipt::AdamArgs l = {};
+            l.state0 = state0; l.m = m; l.v = v; l.ms = m_scale; l.vs = v_scale; l.step = step;
+            unsigned long long nb = 0;
+            for (; i < n && l.tab.n < aipt::TENSORS; i++) {
+                const aipt_adamw_tensor& t = tensors[i];
+                const unsigned long long tb = (unsigned long long)((t.count + aipt::BLOCK - 1) / aipt::BLOCK);
+                if (!tb) continue;
+                if (nb + tb > 0xf0000000ull) {
+                    if (l.tab.n) break;                                        // its own launch
+                    delete a;
+                    return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: tensor %d has %lld elements", i, t.count);
+                }
+                l.tab.tail[l.tab.n] = (unsigned char)((t.count - 1) % aipt::BLOCK);
+                l.tab.t[l.tab.n++] = {t.param, t.grad, t.copy, (unsigned)nb, t.weight_decay};
+                nb += tb;
+            }
+            if (!l.tab.n) break;
+            l.tab.blocks = (unsigned)nb;
+            state0 += nb;
+            a->launches.push_back(l);
+            a->grids.push_back((unsigned)std::min<unsigned long long>((nb + 3) / 4, aipt::GRID));
+        }
+        for (unsigned g : a->grids) a->npartial += (int)g;
+    } catch (const std::bad_alloc&) {
+        delete a;
+        return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
+    }
+    const size_t need = aipt::SCRATCH + sizeof(float) * (size_t)a->npartial;
+    if (workspace_bytes < need) {
+        delete a;
+        return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: workspace of %zu bytes, %zu are wanted", workspace_bytes, need);
+    }
+    a->ticket = (unsigned*)d_workspace;
+    a->clip = (float*)d_workspace + 16;
+    a->partial = (float*)((char*)d_workspace + aipt::SCRATCH);
+    *out = a;
+    return AIPT_OK;
+}
+
+int aipt_adamw_step(aipt_ctx* ctx, aipt_adamw* a, double lr, double beta1, double beta2, double eps, double max_norm, uint32_t seed) {
+    if (!a || a->ctx != ctx) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_step: no plan of this context");
+    if (!std::isfinite(lr) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !std::isfinite(eps) || std::isnan(max_norm))
+        return fail(ctx, AIPT_E_INVALID, "aipt_adamw_step: lr %g, beta1 %g, beta2 %g, eps %g, max_norm %g", lr, beta1, beta2, eps, max_norm);
+    if (a->launches.empty()) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_step: the plan holds no elements");
+    AIPT_NEED_CTX(ctx);
+    aipt::DeviceScope dev(ctx->device);
+    AIPT_HIP(ctx, dev.err);
+    const bool clip = max_norm > 0;
+    const size_t nl = a->launches.size();
+    if (clip) {
+        aipt::NormKernel k = a->grad_type == AIPT_TYPE_F32 ? aipt::grad_square<float> : a->grad_type == AIPT_TYPE_BF16 ? aipt::grad_square<aipt::bf16> : aipt::grad_square<aipt::f16>;
+        float* partial = a->partial;
+        for (size_t i = 0; i < nl; i++) {
+            aipt::NormArgs na;
+            na.tab = a->launches[i].tab; na.partial = partial;
+            AIPT_HIP(ctx, aipt::launch(k, a->grids[i], 256, 0, ctx->stream, na));
+            partial += a->grids[i];
+        }
+        AIPT_HIP(ctx, aipt::launch(aipt::grad_norm_end, 1, 256, 0, ctx->stream, aipt::NormEndArgs{a->partial, a->npartial, (float)max_norm, a->clip, a->norm}));
+    }
+    aipt::AdamKernel k = a->grad_type == AIPT_TYPE_F32 ? aipt::adam_of<float>(a->copy_type, a->bits) : a->grad_type == AIPT_TYPE_BF16 ? aipt::adam_of<aipt::bf16>(a->copy_type, a->bits)
+                                                                                                   : aipt::adam_of<aipt::f16>(a->copy_type, a->bits);
+    for (size_t i = 0; i < nl; i++) {
+        aipt::AdamArgs l = a->launches[i];
+        l.clip = clip ? a->clip : nullptr;
+        l.ticket = i + 1 == nl ? a->ticket : nullptr;
+        l.b1 = beta1; l.b2 = beta2; l.lr = (float)lr; l.beta1 = (float)beta1; l.beta2 = (float)beta2; l.eps = (float)eps;
+        l.omb1 = (float)(1.0 - beta1); l.omb2 = (float)(1.0 - beta2);
+        l.seed = seed;
+        AIPT_HIP(ctx, aipt::launch(k, a->grids[i], 256, 0, ctx->stream, l));
+    }
+    return AIPT_OK;
+}
+
+void aipt_adamw_destroy(aipt_adamw* a) {
+    delete a;
+}
+
+}  // extern "C"

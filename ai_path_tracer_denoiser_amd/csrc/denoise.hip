@@ -2427,7 +2427,7 @@ int aipt::denoise_run(aipt_ctx* ctx, const float* d_in10, float* d_out3, uint32_
     hipStream_t st = on ? on : pipelined ? stream_of(a) : ctx->stream;     // on: the CU-masked denoiser stream of aipt_frame
     // the pass reads the G-buffer the last trace wrote: unless it runs on the CU-masked denoiser stream of aipt_frame_prefetch
     // (which orders itself behind ITS trace), it starts after the last trace, whichever stream that ran on
-    if (ctx->last_trace_stream && ctx->last_trace_stream != st && st != ctx->st_dn)
+    if (ctx->traced && ctx->last_trace_stream != st && !(ctx->st_dn && st == ctx->st_dn))
         AIPT_HIP(ctx, hipStreamWaitEvent(st, ctx->ev_traced, 0));
     s->cur = st;
     s->aset = a;

@@ -56,7 +56,8 @@ struct aipt_ctx {
     hipEvent_t ev_prefetched = nullptr;               // the prefetched trace has finished
     hipEvent_t ev_traced = nullptr;                   // last trace (any stream) has finished: traces share one path state
     hipEvent_t ev_entry = nullptr;                    // aipt_frame: what the host had queued on `stream` before the call
-    hipStream_t last_trace_stream = nullptr;
+    hipStream_t last_trace_stream = nullptr;            // ... which stream that was on (valid once `traced`; nullptr is HIP's default stream)
+    bool traced = false;
     bool denoised_valid[2] = {false, false};
     bool denoised_masked[2] = {false, false};         // that denoise ran on the CU-masked stream st_dn (a prefetched frame)
     struct { bool valid = false; aipt_camera cam; int iter = 0, depth = 0; uint32_t flags = 0; int buf = 0; } pf;

@@ -1680,7 +1680,7 @@ int trace_on_stream(aipt_ctx* ctx, hipStream_t st, const aipt_camera* cam, int n
         AIPT_HIP(ctx, hipMalloc((void**)&t->d_stack_ovf, sizeof(int) * (size_t)ovf_need * t->P * t->batch));
         t->ovf_entries = ovf_need;
     }
-    if (!lane && ctx->last_trace_stream && ctx->last_trace_stream != st) AIPT_HIP(ctx, hipStreamWaitEvent(st, ctx->ev_traced, 0));
+    if (!lane && ctx->traced && ctx->last_trace_stream != st) AIPT_HIP(ctx, hipStreamWaitEvent(st, ctx->ev_traced, 0));
     if (blur && !(iter % 4) && iter < 3000) {                   // moveGeom, pathtrace.cu:442-446 (dt = 0.10)
         bool moved = false;
         for (aipt_geom& g : s->h_geoms) {
@@ -1763,6 +1763,7 @@ int trace_on_stream(aipt_ctx* ctx, hipStream_t st, const aipt_camera* cam, int n
     if (!lane) {
         AIPT_HIP(ctx, hipEventRecord(ctx->ev_traced, st));
         ctx->last_trace_stream = st;
+        ctx->traced = true;
     }
     if (lane) tstate(ctx)->side_used = true; else s->side_used = false;
     s->last_depth = depth;
@@ -1861,7 +1862,7 @@ int aipt_trace_live_counts(aipt_ctx* ctx, int* h_n_live, int n) {
     if (!s->d_nlive || !s->last_depth) return fail(ctx, AIPT_E_STATE, "aipt_trace_live_counts: no trace has run");
     if (!h_n_live || n < 1) return fail(ctx, AIPT_E_INVALID, "aipt_trace_live_counts: bad arguments");
     std::vector<int> tmp(MAX_DEPTH + 1);
-    if (ctx->last_trace_stream) AIPT_HIP(ctx, hipStreamWaitEvent(ctx->stream, ctx->ev_traced, 0));
+    if (ctx->traced) AIPT_HIP(ctx, hipStreamWaitEvent(ctx->stream, ctx->ev_traced, 0));
     AIPT_HIP(ctx, hipMemcpyAsync(tmp.data(), s->d_nlive, sizeof(int) * (MAX_DEPTH + 1), hipMemcpyDeviceToHost, ctx->stream));
     AIPT_HIP(ctx, aipt::sync_streams(ctx));
     tmp[0] = s->P * s->last_frames;
@@ -1892,7 +1893,7 @@ int aipt_trace_live_counts_frame(aipt_ctx* ctx, int frame, int* h_n_live, int n)
         return AIPT_OK;
     }
     std::vector<int> tmp((MAX_DEPTH + 1) * BMAX);
-    if (ctx->last_trace_stream) AIPT_HIP(ctx, hipStreamWaitEvent(ctx->stream, ctx->ev_traced, 0));
+    if (ctx->traced) AIPT_HIP(ctx, hipStreamWaitEvent(ctx->stream, ctx->ev_traced, 0));
     AIPT_HIP(ctx, hipMemcpyAsync(tmp.data(), s->d_nlive_f, sizeof(int) * tmp.size(), hipMemcpyDeviceToHost, ctx->stream));
     AIPT_HIP(ctx, aipt::sync_streams(ctx));
     for (int i = 0; i < n; i++) h_n_live[i] = i == 0 ? s->P : (i <= s->last_depth ? tmp[i * BMAX + frame] : 0);
@@ -1908,7 +1909,7 @@ int aipt_trace_first_hit_materials(aipt_ctx* ctx, int* h_mat, int n) {
     const TraceState* const side = s->side_used && s->side && s->side->mat0_valid && s->side->d_mat0 ? s->side : nullptr;
     const int n_main = s->P * s->last_frames, n_side = side ? side->P * side->last_frames : 0;
     if (!h_mat || n != n_main + n_side) return fail(ctx, AIPT_E_INVALID, "aipt_trace_first_hit_materials: n=%d, expected %d", n, n_main + n_side);
-    if (ctx->last_trace_stream) AIPT_HIP(ctx, hipStreamWaitEvent(ctx->stream, ctx->ev_traced, 0));
+    if (ctx->traced) AIPT_HIP(ctx, hipStreamWaitEvent(ctx->stream, ctx->ev_traced, 0));
     AIPT_HIP(ctx, hipMemcpyAsync(h_mat, s->d_mat0, sizeof(int) * (size_t)n_main, hipMemcpyDeviceToHost, ctx->stream));
     AIPT_HIP(ctx, aipt::sync_streams(ctx));
     if (side) AIPT_HIP(ctx, hipMemcpy(h_mat + n_main, side->d_mat0, sizeof(int) * (size_t)n_side, hipMemcpyDeviceToHost));

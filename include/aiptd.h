@@ -106,9 +106,12 @@ typedef struct aipt_aabb {            /* MeshBoundingBox, sceneStructs.h:84-87, 
 } aipt_aabb;
 
 /* ---- context ---------------------------------------------------------------------------------------------- */
-/* stream: an existing hipStream_t to enqueue on (e.g. the caller's torch stream), or NULL to create one. */
+/* stream: an existing hipStream_t to enqueue on (e.g. the caller's torch stream), AIPT_STREAM_DEFAULT for HIP's default stream (the one
+ * torch uses unless told otherwise), or NULL to create one. */
+#define AIPT_STREAM_DEFAULT ((void*)(intptr_t)-1)
 int  aipt_create(int device, void* stream, aipt_ctx** out);
 void aipt_destroy(aipt_ctx* ctx);
+int  aipt_stream(const aipt_ctx* ctx, void** stream_out);   /* the hipStream_t the context enqueues on (NULL = HIP's default stream) */
 const char* aipt_last_error(const aipt_ctx* ctx);      /* ctx may be NULL: error of the last failed aipt_create */
 int  aipt_abi_version(void);
 int  aipt_sync(aipt_ctx* ctx);                          /* hipStreamSynchronize on the context stream */
@@ -320,6 +323,134 @@ int aipt_gbuffer(aipt_ctx* ctx, float** d_gbuf, int* rows, int* stride);
 /* per-stage GPU time of the last aipt_frame with timing enabled (ms; synchronous) */
 int aipt_frame_set_timing(aipt_ctx* ctx, int enabled);
 int aipt_frame_last_times(aipt_ctx* ctx, float* trace_ms, float* denoise_ms);
+
+/* ---- layer operators ----------------------------------------------------------------------------------------
+ * Layers beside the denoiser -- a residual block over its feature maps, its gradients, and the step that trains its weights (the
+ * reference trains with Adam, training/train.py:54-112; it has these through torch).  Same manner as the rest: enqueued on the
+ * context's stream, asynchronous, no allocation, no synchronisation, no state kept between calls (but for the aipt_adamw plan): a
+ * call may be captured into a hipGraph and replayed.  Scratch memory is the caller's: where an operator wants some, its _workspace
+ * entry says how much, and two calls that may run at the same time (two streams, two graphs) are given different memory.  Every
+ * sum is in fp32 and in an order that depends on the sizes alone: the same inputs give the same bits.  Outputs may not overlap inputs
+ * (AIPT_E_INVALID) but where an entry says so.  All tensors of a call have one element type; sums, statistics and the activation are
+ * fp32, and a result is rounded once, to nearest even.  Arguments are checked before the context is looked at: with ctx NULL, which no call
+ * accepts but the _workspace entries, aipt_last_error(NULL) says what else is wrong. */
+#define AIPT_TYPE_F32  0
+#define AIPT_TYPE_BF16 1
+#define AIPT_TYPE_F16  2
+
+#define AIPT_ACT_NONE  0
+#define AIPT_ACT_LEAKY 1    /* z > 0 ? z : slope * z (the denoiser's, slope 0.1; slope 0 is ReLU) */
+#define AIPT_ACT_SILU  2    /* z / (1 + e^-z) */
+#define AIPT_ACT_GELU  3    /* z * Phi(z), Phi the normal distribution (erf, not the tanh approximation) */
+
+/* Element (i, j) is data[i * row_stride + j * col_stride] (strides in elements).  One of the strides is 1, or its extent is at most
+ * 1: rows [pixels][channels], or the planar layout [channels][pixels] of the G-buffer and the hidden states (row_stride 1).  The
+ * strides of an input may be 0 (a broadcast row); elements of an output may not coincide. */
+typedef struct aipt_matrix {
+    void* data;
+    long long row_stride, col_stride;
+} aipt_matrix;
+
+/* y = act(x w^T + bias) + residual;  x [m][k], w [n][k], bias [n] or NULL, residual [m][n] or data NULL, y [m][n];
+ * preact [m][n] (or data NULL) receives z = x w^T + bias, which the backward pass of an activation wants.
+ * residual may be y itself (same data and strides).  Sizes may be 0 (k = 0: z = bias); each below 2^31 - 4096. */
+typedef struct aipt_linear_args {
+    int type, act;
+    float slope;
+    int reserved;                     /* 0 */
+    long long m, n, k;
+    aipt_matrix x, w, y, residual, preact;
+    const void* bias;
+} aipt_linear_args;
+int aipt_linear_workspace(aipt_ctx* ctx, const aipt_linear_args* args, size_t* bytes);      /* pointers are not looked at */
+int aipt_linear(aipt_ctx* ctx, const aipt_linear_args* args, void* d_workspace, size_t workspace_bytes);
+
+/* Gradients: dz = dy * act'(z);  dx = dz w  [m][k];  dw = dz^T x  [n][k];  dbias = sum over rows of dz  [n].  Outputs whose data is
+ * NULL are not computed (the gradient of the residual is dy).  preact: the z that aipt_linear kept (not looked at with AIPT_ACT_NONE).  dz
+ * is rounded to the element type before the two products (bf16 / fp16: an error of half a step of each factor, as of an input). */
+typedef struct aipt_linear_grad_args {
+    int type, act;
+    float slope;
+    int reserved;                     /* 0 */
+    long long m, n, k;
+    aipt_matrix dy, x, w, preact, dx, dw;
+    void* dbias;
+} aipt_linear_grad_args;
+int aipt_linear_backward_workspace(aipt_ctx* ctx, const aipt_linear_grad_args* args, size_t* bytes);   /* looks at which outputs are wanted, not where */
+int aipt_linear_backward(aipt_ctx* ctx, const aipt_linear_grad_args* args, void* d_workspace, size_t workspace_bytes);
+
+/* The norms around a residual block, with its gate and residual scale.  For every row of c channels:
+ *     u = norm(y) * post_weight + post_bias        the norm behind the block (y NULL: no block, h = x)
+ *     h = x + scale * gate * u                     the residual stream
+ *     z = norm(h) * pre_weight + pre_bias          the norm before the next block (z NULL: none)
+ * norm(v) = v * rstd (AIPT_NORM_RMS, rstd = 1 / sqrt(mean(v^2) + eps)) or (v - mean) * rstd (AIPT_NORM_LAYER, rstd from the variance).
+ * x, y, h, z: rows of c contiguous elements, a row stride each.  scale and the weights [c] (NULL: 1), biases [c] (NULL: 0; AIPT_NORM_LAYER
+ * only), gate [groups][c] (NULL: 1), row r taking the gate r / (rows / groups): groups = rows is a gate for each element; rows must be
+ * a multiple of groups.  stats (or NULL): float [rows][4] = mean and rstd of y, mean and rstd of h, for the backward pass.
+ * 1 <= c <= 16384, any number of rows.  h may be x. */
+#define AIPT_NORM_RMS   0
+#define AIPT_NORM_LAYER 1
+typedef struct aipt_block_norm_args {
+    int type, kind;
+    float eps;
+    int c;
+    long long rows, groups;
+    const void *x, *y;
+    void *h, *z;
+    long long x_stride, y_stride, h_stride, z_stride;
+    const void *gate, *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;
+    float* stats;
+} aipt_block_norm_args;
+int aipt_block_norm(aipt_ctx* ctx, const aipt_block_norm_args* args);
+
+/* Gradients from dh (of the residual stream; NULL: zero) and dz (NULL: there was no norm before the next block), with y, h and stats as
+ * the forward pass left them:  dx (also the gradient that passes the block by; may be dh), dy, dgate [groups][c], dscale, the weights' and
+ * biases' [c] (each NULL if not wanted). */
+typedef struct aipt_block_norm_grad_args {
+    int type, kind;
+    int c, reserved;                  /* reserved: 0 */
+    long long rows, groups;
+    const void *dh, *dz, *y, *h;
+    const float* stats;
+    const void *gate, *scale, *post_weight, *post_bias, *pre_weight;
+    void *dx, *dy;
+    long long dh_stride, dz_stride, y_stride, h_stride, dx_stride, dy_stride;
+    void *dgate, *dscale, *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+} aipt_block_norm_grad_args;
+int aipt_block_norm_backward_workspace(aipt_ctx* ctx, const aipt_block_norm_grad_args* args, size_t* bytes);
+int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* args, void* d_workspace, size_t workspace_bytes);
+
+/* AdamW (decoupled weight decay) over many tensors at once.  A plan is bound to its tensors' memory when it is made; a step reads the
+ * gradients and updates parameters, state and the step number in place:
+ *     t = step + 1;  g = gradient * clip;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *     p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps);   copy = p rounded;   step = t
+ * clip = min(1, max_norm / (norm + 1e-6)), norm the 2-norm of all gradients together; with max_norm <= 0 there is no clipping and the
+ * norm is not computed.  If the norm is not finite the step changes nothing, not the step number either.
+ * State: elements of tensor i begin at 256 * (number of 256-blocks of the tensors before it), each tensor's last block padded with
+ * zeros; aipt_adamw_state_elements(counts, n) elements in all.  state_bits 32: m and v are float.  state_bits 8: m and sqrt(v) as OCP
+ * e4m3 multiples of one float scale for each 256-block (its largest magnitude / 448): m rounded to nearest, the root up or down by
+ * chance -- a change of 0.1 % of v must not be lost to rounding for ever -- with 24 bits of a hash of (seed, t, place), a positive
+ * root never to zero.  A block whose largest magnitude is below 2^-100 is kept as zeros.  An infinite or NaN gradient spoils its
+ * element's state (8 bits: its block's): clip, and such steps are skipped. */
+typedef struct aipt_adamw aipt_adamw;
+typedef struct aipt_adamw_tensor {
+    float* param;
+    const void* grad;                 /* of the plan's grad_type */
+    void* copy;                       /* NULL, or the rounded parameters (of the plan's copy_type) for the next forward pass */
+    long long count;                  /* elements, >= 0 */
+    float weight_decay;
+    int reserved;                     /* 0 */
+} aipt_adamw_tensor;
+long long aipt_adamw_state_elements(const long long* counts, int n);
+long long aipt_adamw_workspace(const long long* counts, int n);      /* bytes; both: AIPT_E_INVALID for counts that are none */
+/* m, v: float (32 bits) or e4m3 bytes; m_scale, v_scale: float per 256-block (8 bits) or NULL; step: int, device, steps taken so far; norm: float,
+ * device, receives the norm of a step that clips.  d_workspace: aipt_adamw_workspace bytes, ZEROED by the caller, the plan's own as long as
+ * it (or a graph that captured a step of it) lives.  What a step writes must be apart from everything else the plan names. */
+int  aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, int grad_type, int copy_type, int state_bits,
+                       void* m, void* v, float* m_scale, float* v_scale, int* step, float* norm, void* d_workspace,
+                       size_t workspace_bytes, aipt_adamw** out);
+int  aipt_adamw_step(aipt_ctx* ctx, aipt_adamw* plan, double lr, double beta1, double beta2, double eps, double max_norm, uint32_t seed);
+void aipt_adamw_destroy(aipt_adamw* plan);      /* host memory alone: all device memory is the caller's */
 
 /* ---- multi-GPU hosts: the one-time broadcast (no reference equivalent: single GPU) ------------------------------ */
 /* The path shards by frames (one context per GPU, contiguous frame chunks, no per-frame exchange); the only collective is
