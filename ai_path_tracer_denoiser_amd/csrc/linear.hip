@@ -30,6 +30,7 @@ struct GemmArgs {
     long long ri, rj;
     void* pre;
     long long pi, pj;
+    int c16;                         // rows of c, res and pre lie on 16 bytes, j contiguous
 };
 
 __device__ inline float act_of(float z, int act, float slope) {
@@ -166,6 +167,233 @@ __global__ __launch_bounds__(256) void gemm_any(const GemmArgs g) {
             }
 }
 
+// ---- 16-bit types, lines on 16 bytes: tiles of TI x TJ, fed without a pause.
+// A step is 32 of k (64 bytes).  ST steps of both operands lie in LDS, loaded there directly (buffer loads to LDS, 16 bytes a lane), ST - 1
+// steps ahead of their use; the fragments of a step are read into registers while the matrix instructions of the step before run.  One
+// barrier a step: behind it every wave has its fragments of step t, so that t's LDS is free for t + ST, and step t + 1 is visible.
+//   k contiguous:    rows of 64 bytes, 16-byte chunk c of row r at c ^ (r / 4 % 4): the 16 rows a read takes together lie on all banks
+//   rows contiguous: 32 lines (k) of the tile's rows, 32-byte chunk c of line k at c ^ (k % 4 + k / 8 % 2 * 4), read by the transposing
+//                    LDS load (16 lanes x 4 elements: lines 4q .. 4q + 3, 16 rows -> each lane its row's four)
+// Lines beyond the operand are clamped to its last one (their results are not stored), steps beyond k read as zero (beyond num_records).
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+#define AIPT_LDS __attribute__((address_space(3)))
+
+template <typename T> struct Frag;
+template <> struct Frag<bf16> {
+    using V = bf16x8;
+    static __device__ inline f32x4 mac(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Frag<f16> {
+    using V = f16x8;
+    static __device__ inline f32x4 mac(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// loads of one operand's part of a step: R rows x 32 k = R * 64 bytes, split over NT threads
+template <bool KC, int R, int NT> struct TileLoad {
+    static constexpr int L = R * 4 / NT;
+    unsigned off[L];
+    int kof[L];                      // the k of this lane's chunk, for the last steps
+    const char* base;
+    long long step;                  // bytes to the next step
+    int k1;
+    __device__ inline void init(const void* p, long long stride, int r0, int rows, int k0, int k1_, int tid) {
+        k1 = k1_;
+        // (a line's contiguous rows come in eights: rows is a multiple of 8, or its lines are padded to one)
+        base = (const char*)p + (KC ? ((long long)r0 * stride + k0) * 2 : ((long long)k0 * stride + r0) * 2);
+        step = KC ? 64 : 64 * stride;
+        const int last = KC ? rows - 1 - r0 : ((rows + 7) & ~7) - 8 - r0;
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            const int q = i * NT + tid;
+            if (KC) {
+                const int r = q >> 2, c = (q & 3) ^ ((r >> 2) & 3);
+                off[i] = (unsigned)min(r, last) * (unsigned)(stride * 2) + c * 16;
+                kof[i] = k0 + c * 8;
+            } else {
+                const int k = q / (R / 8), c = q % (R / 8);
+                const int mn = (((c >> 1) ^ ((k & 3) | ((k >> 1) & 4))) * 2 + (c & 1)) * 8;
+                off[i] = (unsigned)k * (unsigned)(stride * 2) + (unsigned)min(mn, last) * 2;
+                kof[i] = k0 + k;
+            }
+        }
+    }
+    __device__ inline void go(int t, AIPT_LDS char* lds, int wave) const {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + t * step), 0, 0x7fffffff, 0x00027000);
+        const bool all = __builtin_amdgcn_readfirstlane(kof[0] & ~31) + (t + 1) * 32 <= k1;      // (k0 is a multiple of 32)
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            const unsigned o = all || kof[i] + t * 32 < k1 ? off[i] : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AIPT_LDS void*)(lds + (i * NT + wave * 64) * 16), 16, o, 0, 0, 0);
+        }
+    }
+};
+
+// fragments of N x 16 rows from r0 on, 32 k
+template <typename T, bool KC, int R, int N> struct TileRead {
+    int at[KC ? 1 : N][2];
+    __device__ inline void init(int r0, int lane) {
+        if constexpr (KC) {
+            const int r = r0 + (lane & 15);
+            at[0][0] = r * 64 + (((lane >> 4) ^ ((r >> 2) & 3)) * 16);
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int k = (lane >> 4) * 8 + h * 4 + ((lane & 15) >> 2);
+                    at[n][h] = k * R * 2 + (((r0 / 16 + n) ^ ((k & 3) | ((k >> 1) & 4))) * 32) + (lane & 3) * 8;
+                }
+        }
+    }
+    __device__ inline void go(AIPT_LDS char* lds, typename Frag<T>::V* f) const {
+        using V = typename Frag<T>::V;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            if constexpr (KC) f[n] = *(AIPT_LDS V*)(lds + at[0][0] + n * 1024);
+            else {
+                union { i16x4 h[2]; V v; } u;
+                u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][0]));
+                u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][1]));
+                f[n] = u.v;
+            }
+        }
+    }
+};
+
+// eight neighbours of a row: bias, activation, residual, 16-byte stores
+template <typename T, int ACT> __device__ inline void epilogue8(const GemmArgs& g, int i, int j, float* z, const float* bias_j) {
+    float b[8];
+    if (g.bias_i) {
+        const float v = g.bias ? (float)((const T*)g.bias)[i] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) b[e] = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) b[e] = bias_j[e];
+    }
+    Chunk<T> q;
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] += b[e];
+    if (g.pre) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) q.v[e] = (T)z[e];
+        *(Chunk<T>*)((T*)g.pre + i * g.pi + j) = q;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] = act_of(z[e], ACT, g.slope);
+    if (g.res) {
+        const Chunk<T> r = *(const Chunk<T>*)((const T*)g.res + i * g.ri + j);
+#pragma unroll
+        for (int e = 0; e < 8; e++) z[e] += (float)r.v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) q.v[e] = (T)z[e];
+    *(Chunk<T>*)((T*)g.c + i * g.cs + j) = q;
+}
+
+template <typename T, bool AK, bool BK, int TI, int TJ, int WI, int WJ, int ST>
+__global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
+    constexpr int NT = WI * WJ * 64, WTI = TI / WI, WTJ = TJ / WJ, FI = WTI / 16, FJ = WTJ / 16, SB = (TI + TJ) * 64;
+    constexpr int SLAB = WTI < 64 ? WTI : 64;                // rows of a wave's results that go through LDS at a time
+    constexpr int BYTES = ST * SB > WI * WJ * SLAB * WTJ * 4 ? ST * SB : WI * WJ * SLAB * WTJ * 4;
+    __shared__ __attribute__((aligned(1024))) char lds_[BYTES];
+    AIPT_LDS char* lds = (AIPT_LDS char*)lds_;
+    using V = typename Frag<T>::V;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // workgroups go round the eight XCDs: each XCD takes a run of neighbouring tiles, which share operands in its L2 ...
+    const int total = gridDim.x, per = total >> 3, extra = total & 7, x = blockIdx.x & 7;
+    int job = (x < extra ? x * (per + 1) : extra * (per + 1) + (x - extra) * per) + (blockIdx.x >> 3);
+    const int tiles = g.tiles_i * g.tiles_j, split = job / tiles;
+    job -= split * tiles;
+    // ... in columns of 8 tiles
+    const int band = 8 * g.tiles_j, b0 = job / band * 8, bh = min(8, g.tiles_i - b0);
+    const int i0 = (b0 + (job % band) % bh) * TI, j0 = (job % band) / bh * TJ;
+    const int k0 = split * g.k_split, k1 = min(g.K, k0 + g.k_split), n = (k1 - k0 + 31) >> 5;
+
+    TileLoad<AK, TI, NT> la;
+    TileLoad<BK, TJ, NT> lb;
+    la.init(g.a, g.as, i0, g.I, k0, k1, tid);
+    lb.init(g.b, g.bs, j0, g.J, k0, k1, tid);
+    const int wi = wave / WJ * WTI, wj = wave % WJ * WTJ;
+    TileRead<T, AK, TI, FI> ra;
+    TileRead<T, BK, TJ, FJ> rb;
+    ra.init(wi, lane);
+    rb.init(wj, lane);
+    constexpr int L = decltype(la)::L + decltype(lb)::L;
+    auto issue = [&](int t, int slot) {
+        la.go(t, lds + slot * SB, wave);
+        lb.go(t, lds + slot * SB + TI * 64, wave);
+    };
+    f32x4 acc[FI][FJ] = {};
+    V a0[FI], b0f[FJ], a1[FI], b1f[FJ];
+#pragma unroll
+    for (int t = 0; t < ST; t++) issue(t, t);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((ST - 1) * L) : "memory");
+    ra.go(lds, a0);
+    rb.go(lds + TI * 64, b0f);
+    int slot = 0;
+    auto step = [&](int t, V* a, V* b, V* an, V* bn) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * L) : "memory");
+        issue(t + ST, slot);
+        slot = slot == ST - 1 ? 0 : slot + 1;
+        ra.go(lds + slot * SB, an);
+        rb.go(lds + slot * SB + TI * 64, bn);
+#pragma unroll
+        for (int p = 0; p < FI; p++)
+#pragma unroll
+            for (int q = 0; q < FJ; q++) acc[p][q] = Frag<T>::mac(b[q], a[p], acc[p][q]);
+    };
+    for (int t = 0; t < n; t += 2) {                         // (an odd last step adds zeros)
+        step(t, a0, b0f, a1, b1f);
+        step(t + 1, a1, b1f, a0, b0f);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+    // results: through a slab of LDS of the wave's own (chunk c of row r at c ^ (r % 16)), so that rows are stored in 16-byte pieces
+    AIPT_LDS char* slab = lds + wave * (SLAB * WTJ * 4);
+    constexpr int LR = WTJ / 8, RPI = 64 / LR;               // lanes of a row, rows of an instruction
+    const int j = j0 + wj + lane % LR * 8;
+    const bool whole = j + 8 <= g.J && g.c16;
+    float bias_j[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) bias_j[e] = g.bias && !g.bias_i && g.splits == 1 && j + e < g.J ? (float)((const T*)g.bias)[j + e] : 0.f;
+#pragma unroll
+    for (int s = 0; s < WTI / SLAB; s++) {
+#pragma unroll
+        for (int p = 0; p < SLAB / 16; p++)
+#pragma unroll
+            for (int q = 0; q < FJ; q++) {
+                const int r = p * 16 + (lane & 15), c = q * 4 + (lane >> 4);
+                *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & 15)) * 16)) = acc[s * (SLAB / 16) + p][q];
+            }
+        auto rows = [&](auto done) {
+            for (int r = lane / LR; r < SLAB; r += RPI) {
+                const int i = i0 + wi + s * SLAB + r;
+                if (i >= g.I || j >= g.J) continue;
+                float z[8];
+                const int c = lane % LR * 2;
+                *(f32x4*)z = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & 15)) * 16));
+                *(f32x4*)(z + 4) = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + (((c + 1) ^ (r & 15)) * 16));
+                done(i, z);
+            }
+        };
+        if (g.splits > 1) rows([&](int i, float* z) {
+            float* o = g.partial + ((long long)split * g.I + i) * g.J + j;
+#pragma unroll
+            for (int e = 0; e < 8; e++) if (j + e < g.J) o[e] = z[e];
+        });
+        else if (!whole) rows([&](int i, float* z) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) if (j + e < g.J) epilogue<T>(g, i, j + e, z[e]);
+        });
+        else if (g.act == AIPT_ACT_NONE) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_NONE>(g, i, j, z, bias_j); });
+        else if (g.act == AIPT_ACT_LEAKY) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_LEAKY>(g, i, j, z, bias_j); });
+        else if (g.act == AIPT_ACT_SILU) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_SILU>(g, i, j, z, bias_j); });
+        else rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_GELU>(g, i, j, z, bias_j); });
+    }
+}
+
 // the splits of a long contraction, added in order, and the epilogue
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join(const GemmArgs g) {
@@ -184,6 +412,7 @@ struct DzArgs {
     float* part;                     // [row tiles][N] sums over 64 rows, or NULL
     long long dyi, dyj, zi, zj, dzi, dzj;
     int M, N, tiles_n, turned;       // turned: rows are the contiguous axis
+    int line;                        // dz's lines, with their padding (of zeros)
     int act;
     float slope;
 };
@@ -198,8 +427,8 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g) {
         if (m < g.M && n < g.N) {
             d = (float)((const T*)g.dy)[m * g.dyi + n * g.dyj];
             if (g.act != AIPT_ACT_NONE) d *= act_slope_of((float)((const T*)g.z)[m * g.zi + n * g.zj], g.act, g.slope);
-            if (g.dz) ((T*)g.dz)[m * g.dzi + n * g.dzj] = (T)d;
         }
+        if (g.dz && (g.turned ? n < g.N && m < g.line : m < g.M && n < g.line)) ((T*)g.dz)[m * g.dzi + n * g.dzj] = (T)d;
         lds[g.turned ? x : y][g.turned ? y : x] = d;
     }
     if (!g.part) return;
@@ -248,6 +477,7 @@ struct View {
     long long ri, rj;                // strides of the first and the second axis
     bool second;                     // the second axis is the contiguous one
     long long other;                 // the stride of the other
+    bool padded = false;             // lines are padded with zeros to a multiple of 16 bytes
 };
 static View view_of(const aipt_matrix& m, long long n0, long long n1) {
     View v{(char*)m.data, m.row_stride, m.col_stride, false, 0};
@@ -282,6 +512,8 @@ static Extent extent_of(const aipt_matrix& m, long long n0, long long n1, int es
 struct Plan {                        // a product as it will be launched, and the workspace it wants
     GemmArgs g = {};
     bool ak = true, bk = true;
+    int tile = 0;                    // 0: gemm_any; else gemm_tile of this size
+    unsigned threads = 256;
     size_t partial_bytes = 0, blocks = 0;
     bool fits = true;
 };
@@ -296,11 +528,16 @@ static Plan plan_gemm(int type, const View& a, const View& b, long long I, long 
     p.g.I = (int)I; p.g.J = (int)J; p.g.K = (int)K;
     p.g.avec = !((uintptr_t)a.p & 15) && (a.other % E == 0);
     p.g.bvec = !((uintptr_t)b.p & 15) && (b.other % E == 0);
-    p.g.tiles_i = (int)((I + GT - 1) / GT); p.g.tiles_j = (int)((J + GT - 1) / GT);
+    // gemm_tile wants 16-bit elements, lines on 16 bytes that hold whole 16-byte chunks, and a tile's lines within 31 bits of its first
+    auto lines_ok = [&](const View& v, bool vec, long long len) { return vec && (v.padded || len % E == 0) && v.other * 2 * 256 < (1ll << 31); };
+    if (es == 2 && K >= 32 && lines_ok(a, p.g.avec, a.second ? K : I) && lines_ok(b, p.g.bvec, b.second ? K : J)) p.tile = 256;
+    const int ts = p.tile ? p.tile : GT;
+    p.g.tiles_i = (int)((I + ts - 1) / ts); p.g.tiles_j = (int)((J + ts - 1) / ts);
     const long long tiles = (long long)p.g.tiles_i * p.g.tiles_j, steps = (K + ks - 1) / ks;
     // few tiles and a long contraction: split it until some 512 workgroups (two a CU) run, none with fewer than 4 steps
     long long splits = 1;
-    if (tiles > 0 && tiles < 512) splits = std::max(1ll, std::min((512 + tiles - 1) / tiles, steps / 4));
+    const long long want = p.tile ? 256 : 512;
+    if (tiles > 0 && tiles < want) splits = std::max(1ll, std::min(want / tiles, steps / 4));
     const long long per = splits > 1 ? (steps + splits - 1) / splits : std::max(1ll, steps);
     splits = std::max(1ll, (steps + per - 1) / per);
     p.g.splits = (int)splits;
@@ -312,11 +549,22 @@ static Plan plan_gemm(int type, const View& a, const View& b, long long I, long 
 }
 
 template <typename T> static void (*gemm_of(const Plan& p))(GemmArgs) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.tile) return p.ak ? (p.bk ? gemm_tile<T, true, true, 256, 256, 2, 2, 4> : gemm_tile<T, true, false, 256, 256, 2, 2, 4>)
+                                : (p.bk ? gemm_tile<T, false, true, 256, 256, 2, 2, 4> : gemm_tile<T, false, false, 256, 256, 2, 2, 4>);
+    }
     return p.ak ? (p.bk ? gemm_any<T, true, true> : gemm_any<T, true, false>) : (p.bk ? gemm_any<T, false, true> : gemm_any<T, false, false>);
 }
+// whether the epilogue may move 16 bytes at a time
+static int rows16(int es, const GemmArgs& g) {
+    const long long e = 16 / es;
+    return !(((uintptr_t)g.c | (uintptr_t)g.res | (uintptr_t)g.pre) & 15) && g.cs % e == 0 && (!g.res || (g.rj == 1 && g.ri % e == 0)) && (!g.pre || (g.pj == 1 && g.pi % e == 0));
+}
+
 template <typename T> static hipError_t run_gemm_t(hipStream_t st, Plan& p, void* ws) {
     if (!p.blocks) return hipSuccess;
     p.g.partial = (float*)ws;
+    p.g.c16 = rows16(sizeof(T), p.g);
     hipError_t e = launch(gemm_of<T>(p), p.blocks, 256, 0, st, p.g);
     if (e == hipSuccess && p.g.splits > 1)
         e = launch(gemm_join<T>, std::min<size_t>(((size_t)p.g.I * p.g.J + 255) / 256, 4096), 256, 0, st, p.g);
@@ -360,7 +608,8 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
     if (p.make_dz) {                 // laid out like dy, with lines a multiple of 16 bytes apart
         const long long line = dy.second ? a->n : a->m, lines = dy.second ? a->m : a->n, ld = (line + E - 1) / E * E;
         p.dz_bytes = up256((size_t)(lines * ld) * es);
-        d = {ws, dy.second ? ld : 1, dy.second ? 1 : ld, dy.second, ld};
+        p.dz.line = (int)ld;
+        d = {ws, dy.second ? ld : 1, dy.second ? 1 : ld, dy.second, ld, true};
     }
     const long long tm = (a->m + 63) / 64, tn = (a->n + 63) / 64;
     if (p.want_db) p.part_bytes = up256((size_t)tm * a->n * sizeof(float));
