@@ -179,26 +179,34 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 #define AIPT_LDS __attribute__((address_space(3)))
 
+// The accumulators are pinned to accumulation registers in place: with the builtin the compiler keeps a part of 64 of them in vector
+// registers and moves it to and fro each step (0.84 of 1.3 PFLOP/s).  settle() stands between these instructions and everything else that
+// touches an accumulator: the compiler does not know that they are matrix instructions, whose results and sources want wait states.
 template <typename T> struct Frag;
 template <> struct Frag<bf16> {
     using V = bf16x8;
-    static __device__ inline f32x4 mac(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ inline void mac(V a, V b, f32x4& c) { asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 };
 template <> struct Frag<f16> {
     using V = f16x8;
-    static __device__ inline f32x4 mac(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ inline void mac(V a, V b, f32x4& c) { asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 };
+template <int N> __device__ inline void settle(f32x4* acc) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (i == 0) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i]));
+        else asm volatile("" : "+a"(acc[i]));
+    }
+}
 
 // loads of one operand's part of a step: R rows x 32 k = R * 64 bytes, split over NT threads
 template <bool KC, int R, int NT> struct TileLoad {
     static constexpr int L = R * 4 / NT;
     unsigned off[L];
-    int kof[L];                      // the k of this lane's chunk, for the last steps
+    int kof[L];                      // the k of this lane's chunk within a step
     const char* base;
     long long step;                  // bytes to the next step
-    int k1;
-    __device__ inline void init(const void* p, long long stride, int r0, int rows, int k0, int k1_, int tid) {
-        k1 = k1_;
+    __device__ inline void init(const void* p, long long stride, int r0, int rows, int k0, int tid) {
         // (a line's contiguous rows come in eights: rows is a multiple of 8, or its lines are padded to one)
         base = (const char*)p + (KC ? ((long long)r0 * stride + k0) * 2 : ((long long)k0 * stride + r0) * 2);
         step = KC ? 64 : 64 * stride;
@@ -209,23 +217,20 @@ template <bool KC, int R, int NT> struct TileLoad {
             if (KC) {
                 const int r = q >> 2, c = (q & 3) ^ ((r >> 2) & 3);
                 off[i] = (unsigned)min(r, last) * (unsigned)(stride * 2) + c * 16;
-                kof[i] = k0 + c * 8;
+                kof[i] = c * 8;
             } else {
                 const int k = q / (R / 8), c = q % (R / 8);
                 const int mn = (((c >> 1) ^ ((k & 3) | ((k >> 1) & 4))) * 2 + (c & 1)) * 8;
                 off[i] = (unsigned)k * (unsigned)(stride * 2) + (unsigned)min(mn, last) * 2;
-                kof[i] = k0 + k;
+                kof[i] = k;
             }
         }
     }
-    __device__ inline void go(int t, AIPT_LDS char* lds, int wave) const {
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + t * step), 0, 0x7fffffff, 0x00027000);
-        const bool all = __builtin_amdgcn_readfirstlane(kof[0] & ~31) + (t + 1) * 32 <= k1;      // (k0 is a multiple of 32)
-#pragma unroll
-        for (int i = 0; i < L; i++) {
-            const unsigned o = all || kof[i] + t * 32 < k1 ? off[i] : 0x80000000u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AIPT_LDS void*)(lds + (i * NT + wave * 64) * 16), 16, o, 0, 0, 0);
-        }
+    // where step t lies; load i of it, `left` of k being left
+    __device__ inline __amdgpu_buffer_rsrc_t at(int t) const { return __builtin_amdgcn_make_buffer_rsrc((void*)(base + t * step), 0, 0x7fffffff, 0x00027000); }
+    __device__ inline void one(int i, __amdgpu_buffer_rsrc_t rs, int left, AIPT_LDS char* lds, int wave) const {
+        const unsigned o = kof[i] < left ? off[i] : 0x80000000u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AIPT_LDS void*)(lds + (i * NT + wave * 64) * 16), 16, o, 0, 0, 0);
     }
 };
 
@@ -246,17 +251,14 @@ template <typename T, bool KC, int R, int N> struct TileRead {
                 }
         }
     }
-    __device__ inline void go(AIPT_LDS char* lds, typename Frag<T>::V* f) const {
+    __device__ inline typename Frag<T>::V one(int n, AIPT_LDS char* lds) const {
         using V = typename Frag<T>::V;
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            if constexpr (KC) f[n] = *(AIPT_LDS V*)(lds + at[0][0] + n * 1024);
-            else {
-                union { i16x4 h[2]; V v; } u;
-                u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][0]));
-                u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][1]));
-                f[n] = u.v;
-            }
+        if constexpr (KC) return *(AIPT_LDS V*)(lds + at[0][0] + n * 1024);
+        else {
+            union { i16x4 h[2]; V v; } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][0]));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][1]));
+            return u.v;
         }
     }
 };
@@ -313,42 +315,68 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
 
     TileLoad<AK, TI, NT> la;
     TileLoad<BK, TJ, NT> lb;
-    la.init(g.a, g.as, i0, g.I, k0, k1, tid);
-    lb.init(g.b, g.bs, j0, g.J, k0, k1, tid);
+    la.init(g.a, g.as, i0, g.I, k0, tid);
+    lb.init(g.b, g.bs, j0, g.J, k0, tid);
     const int wi = wave / WJ * WTI, wj = wave % WJ * WTJ;
     TileRead<T, AK, TI, FI> ra;
     TileRead<T, BK, TJ, FJ> rb;
     ra.init(wi, lane);
     rb.init(wj, lane);
-    constexpr int L = decltype(la)::L + decltype(lb)::L;
-    auto issue = [&](int t, int slot) {
-        la.go(t, lds + slot * SB, wave);
-        lb.go(t, lds + slot * SB + TI * 64, wave);
-    };
+    constexpr int LA = decltype(la)::L, LB = decltype(lb)::L, L = LA + LB;
     f32x4 acc[FI][FJ] = {};
+    settle<FI * FJ>(&acc[0][0]);
     V a0[FI], b0f[FJ], a1[FI], b1f[FJ];
 #pragma unroll
-    for (int t = 0; t < ST; t++) issue(t, t);
+    for (int t = 0; t < ST; t++) {
+        const auto sa = la.at(t), sb = lb.at(t);
+#pragma unroll
+        for (int i = 0; i < L; i++)
+            if (i < LA) la.one(i, sa, k1 - k0 - t * 32, lds + t * SB, wave);
+            else lb.one(i - LA, sb, k1 - k0 - t * 32, lds + t * SB + TI * 64, wave);
+    }
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((ST - 1) * L) : "memory");
-    ra.go(lds, a0);
-    rb.go(lds + TI * 64, b0f);
+#pragma unroll
+    for (int p = 0; p < FI; p++) a0[p] = ra.one(p, lds);
+#pragma unroll
+    for (int q = 0; q < FJ; q++) b0f[q] = rb.one(q, lds + TI * 64);
     int slot = 0;
+    // The order is the program's, not the scheduler's (which would read the next fragments behind the last product, into the registers
+    // that these leave, and so wait for them): rows of FJ products, the reads of the next fragments between the first half of the rows, the
+    // loads of a later step between the second half.
     auto step = [&](int t, V* a, V* b, V* an, V* bn) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * L) : "memory");
-        issue(t + ST, slot);
+        AIPT_LDS char* into = lds + slot * SB;
         slot = slot == ST - 1 ? 0 : slot + 1;
-        ra.go(lds + slot * SB, an);
-        rb.go(lds + slot * SB + TI * 64, bn);
+        AIPT_LDS char* from = lds + slot * SB;
+        const auto sa = la.at(t + ST), sb = lb.at(t + ST);
+        const int left = k1 - k0 - (t + ST) * 32;
+        constexpr int H = FI / 2, R = (FI + FJ + H - 1) / H, G = (L + H - 1) / H;
 #pragma unroll
-        for (int p = 0; p < FI; p++)
+        for (int p = 0; p < FI; p++) {
+            if (p < H) {
 #pragma unroll
-            for (int q = 0; q < FJ; q++) acc[p][q] = Frag<T>::mac(b[q], a[p], acc[p][q]);
+                for (int r = p * R; r < (p + 1) * R && r < FI + FJ; r++) {
+                    if (r < FI) an[r] = ra.one(r, from);
+                    else bn[r - FI] = rb.one(r - FI, from + TI * 64);
+                }
+            } else {
+#pragma unroll
+                for (int i = (p - H) * G; i < (p - H + 1) * G && i < L; i++)
+                    if (i < LA) la.one(i, sa, left, into, wave);
+                    else lb.one(i - LA, sb, left, into + TI * 64, wave);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int q = 0; q < FJ; q++) Frag<T>::mac(b[q], a[p], acc[p][q]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     for (int t = 0; t < n; t += 2) {                         // (an odd last step adds zeros)
         step(t, a0, b0f, a1, b1f);
         step(t + 1, a1, b1f, a0, b0f);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    settle<FI * FJ>(&acc[0][0]);
 
     // results: through a slab of LDS of the wave's own (chunk c of row r at c ^ (r % 16)), so that rows are stored in 16-byte pieces
     AIPT_LDS char* slab = lds + wave * (SLAB * WTJ * 4);
