@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 namespace aipt {
 

@@ -167,14 +167,18 @@ __global__ __launch_bounds__(256) void gemm_any(const GemmArgs g) {
             }
 }
 
-// ---- 16-bit types, lines on 16 bytes: tiles of TI x TJ, fed without a pause.
-// A step is 32 of k (64 bytes).  ST steps of both operands lie in LDS, loaded there directly (buffer loads to LDS, 16 bytes a lane), ST - 1
-// steps ahead of their use; the fragments of a step are read into registers while the matrix instructions of the step before run.  One
-// barrier a step: behind it every wave has its fragments of step t, so that t's LDS is free for t + ST, and step t + 1 is visible.
-//   k contiguous:    rows of 64 bytes, 16-byte chunk c of row r at c ^ (r / 4 % 4): the 16 rows a read takes together lie on all banks
-//   rows contiguous: 32 lines (k) of the tile's rows, 32-byte chunk c of line k at c ^ (k % 4 + k / 8 % 2 * 4), read by the transposing
-//                    LDS load (16 lanes x 4 elements: lines 4q .. 4q + 3, 16 rows -> each lane its row's four)
-// Lines beyond the operand are clamped to its last one (their results are not stored), steps beyond k read as zero (beyond num_records).
+// ---- Lines on 16 bytes: tiles of TI x TJ, fed without a pause.
+// A pair of steps is 128 bytes of k (64, or 32 floats): whole 128-byte lines of an operand with k contiguous (half lines cost the L2 as much as whole ones: 32 of k
+// at a time ran at 1.15 PFLOP/s).  LDS is a ring of S slots, each one operand's part of a pair, loaded there directly (buffer loads to LDS, 16
+// bytes a lane) in the order A(0) B(0) A(1) B(1) ...; the fragments of a step are read into registers while the matrix instructions of
+// the step before run.  One barrier a pair, before its second step: behind it every wave has read all of pair P, whose slots are
+// free for the loads S ahead of them, and pair P + 1 is visible.
+//   k contiguous:    rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 % 8): the 16 rows a read takes together lie on all banks
+//   rows contiguous: 64 lines (k) of the tile's rows, 32-byte group c of line k at c ^ (k % 4 + k / 8 % 2 * 4), read by the transposing
+//                    LDS load (16 lanes x 4 elements: lines 4q .. 4q + 3, 16 rows -> each lane its row's four); floats: 32 lines, 64-byte
+//                    group c at c ^ (k / 4 % 4), read one by one
+// Lines beyond the operand are clamped to its last one (their results are not stored), what lies beyond k reads as zero (an offset beyond
+// num_records).
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 #define AIPT_LDS __attribute__((address_space(3)))
@@ -182,14 +186,23 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 // The accumulators are pinned to accumulation registers in place: with the builtin the compiler keeps a part of 64 of them in vector
 // registers and moves it to and fro each step (0.84 of 1.3 PFLOP/s).  settle() stands between these instructions and everything else that
 // touches an accumulator: the compiler does not know that they are matrix instructions, whose results and sources want wait states.
+// float: 16 bytes are four k, one for each of four instructions (any order is a sum).
 template <typename T> struct Frag;
 template <> struct Frag<bf16> {
     using V = bf16x8;
-    static __device__ inline void mac(V a, V b, f32x4& c) { asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
+    static constexpr int Q = 1;
+    template <int> static __device__ inline void mac(V a, V b, f32x4& c) { asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 };
 template <> struct Frag<f16> {
     using V = f16x8;
-    static __device__ inline void mac(V a, V b, f32x4& c) { asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
+    static constexpr int Q = 1;
+    template <int> static __device__ inline void mac(V a, V b, f32x4& c) { asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
+};
+template <> struct Frag<float> {
+    using V = f32x4;
+    static constexpr int Q = 4;
+    // (the next of the four adds to what the last but FJ wrote: with FJ = 2, one instruction of 8 passes lies between, and wait states make it sure)
+    template <int q> static __device__ inline void mac(V a, V b, f32x4& c) { asm("s_nop 3\n\tv_mfma_f32_16x16x4_f32 %0, %1, %2, %0" : "+a"(c) : "v"(a[q]), "v"(b[q])); }
 };
 template <int N> __device__ inline void settle(f32x4* acc) {
 #pragma unroll
@@ -199,65 +212,79 @@ template <int N> __device__ inline void settle(f32x4* acc) {
     }
 }
 
-// loads of one operand's part of a step: R rows x 32 k = R * 64 bytes, split over NT threads
-template <bool KC, int R, int NT> struct TileLoad {
-    static constexpr int L = R * 4 / NT;
+// loads of one operand's part of a pair: R rows x 128 bytes of k, split over NT threads, W bytes (16, or 4 for lines on 4) a lane
+template <int ES, bool KC, int R, int NT, int W> struct TileLoad {
+    static constexpr int E = 16 / ES, U = W / ES, KP = 128 / ES, L = R * 128 / (NT * W), GC = ES == 2 ? 2 : 4;   // GC: chunks of a group that stay together
     unsigned off[L];
-    int kof[L];                      // the k of this lane's chunk within a step
+    int kof[L];                      // the k of this lane's elements within a pair
     const char* base;
-    long long step;                  // bytes to the next step
+    long long step;                  // bytes to the next pair
     __device__ inline void init(const void* p, long long stride, int r0, int rows, int k0, int tid) {
-        // (a line's contiguous rows come in eights: rows is a multiple of 8, or its lines are padded to one)
-        base = (const char*)p + (KC ? ((long long)r0 * stride + k0) * 2 : ((long long)k0 * stride + r0) * 2);
-        step = KC ? 64 : 64 * stride;
-        const int last = KC ? rows - 1 - r0 : ((rows + 7) & ~7) - 8 - r0;
+        // (a line's contiguous rows come in whole loads: rows is a multiple of U, or its lines are padded to one)
+        base = (const char*)p + (KC ? ((long long)r0 * stride + k0) * ES : ((long long)k0 * stride + r0) * ES);
+        step = KC ? 128 : 128 * stride;
+        const int last = KC ? rows - 1 - r0 : (rows + U - 1) / U * U - U - r0;
 #pragma unroll
         for (int i = 0; i < L; i++) {
-            const int q = i * NT + tid;
+            const int at = (i * NT + tid) * W, q = at >> 4, in = (at & 15) / ES;      // chunk, and the element of it
             if (KC) {
-                const int r = q >> 2, c = (q & 3) ^ ((r >> 2) & 3);
-                off[i] = (unsigned)min(r, last) * (unsigned)(stride * 2) + c * 16;
-                kof[i] = c * 8;
+                const int r = q >> 3, c = (q & 7) ^ ((r >> 1) & 7);
+                off[i] = (unsigned)min(r, last) * (unsigned)(stride * ES) + (c * E + in) * ES;
+                kof[i] = c * E + in;
             } else {
-                const int k = q / (R / 8), c = q % (R / 8);
-                const int mn = (((c >> 1) ^ ((k & 3) | ((k >> 1) & 4))) * 2 + (c & 1)) * 8;
-                off[i] = (unsigned)k * (unsigned)(stride * 2) + (unsigned)min(mn, last) * 2;
+                const int k = q / (R / E), c = q % (R / E);
+                const int mn = ((c / GC ^ swap(k)) * GC + c % GC) * E + in;
+                off[i] = (unsigned)k * (unsigned)(stride * ES) + (unsigned)min(mn, last) * ES;
                 kof[i] = k;
             }
         }
     }
-    // where step t lies; load i of it, `left` of k being left
+    // which group of line k lies where: as many values as a line has groups, 8 (4) at most
+    static __device__ inline int swap(int k) {
+        constexpr int G = R / 16;
+        return ES == 2 ? ((k & 3) | ((k >> 1) & 4)) & (G < 8 ? G - 1 : 7) : (k >> 2) & (G < 4 ? G - 1 : 3);
+    }
+    // where pair t lies; load i of it, `left` of k being left
     __device__ inline __amdgpu_buffer_rsrc_t at(int t) const { return __builtin_amdgcn_make_buffer_rsrc((void*)(base + t * step), 0, 0x7fffffff, 0x00027000); }
     __device__ inline void one(int i, __amdgpu_buffer_rsrc_t rs, int left, AIPT_LDS char* lds, int wave) const {
         const unsigned o = kof[i] < left ? off[i] : 0x80000000u;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (AIPT_LDS void*)(lds + (i * NT + wave * 64) * 16), 16, o, 0, 0, 0);
+        AIPT_LDS void* to = (AIPT_LDS void*)(lds + (i * NT + wave * 64) * W);
+        if constexpr (W == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, to, 16, o, 0, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, to, 4, o, 0, 0, 0);
     }
 };
 
-// fragments of N x 16 rows from r0 on, 32 k
+// fragments of N x 16 rows from r0 on: the first or the second half of a pair
 template <typename T, bool KC, int R, int N> struct TileRead {
-    int at[KC ? 1 : N][2];
+    static constexpr int ES = sizeof(T);
+    int at[KC ? 1 : N][2];           // k contiguous: of the two halves; else (16 bits) of the two groups of four k
     __device__ inline void init(int r0, int lane) {
         if constexpr (KC) {
             const int r = r0 + (lane & 15);
-            at[0][0] = r * 64 + (((lane >> 4) ^ ((r >> 2) & 3)) * 16);
+#pragma unroll
+            for (int h = 0; h < 2; h++) at[0][h] = r * 128 + (((h * 4 + (lane >> 4)) ^ ((r >> 1) & 7)) * 16);
         } else {
 #pragma unroll
             for (int n = 0; n < N; n++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int k = (lane >> 4) * 8 + h * 4 + ((lane & 15) >> 2);
-                    at[n][h] = k * R * 2 + (((r0 / 16 + n) ^ ((k & 3) | ((k >> 1) & 4))) * 32) + (lane & 3) * 8;
+                    const int k = ES == 2 ? (lane >> 4) * 8 + h * 4 + ((lane & 15) >> 2) : (lane >> 4) * 4;
+                    at[n][h] = k * R * ES + (((r0 / 16 + n) ^ TileLoad<ES, false, R, 64, 16>::swap(k)) * 16 * ES) + (ES == 2 ? (lane & 3) * 8 : (lane & 15) * 4);
                 }
         }
     }
-    __device__ inline typename Frag<T>::V one(int n, AIPT_LDS char* lds) const {
+    template <int H> __device__ inline typename Frag<T>::V one(int n, AIPT_LDS char* lds) const {
         using V = typename Frag<T>::V;
-        if constexpr (KC) return *(AIPT_LDS V*)(lds + at[0][0] + n * 1024);
-        else {
+        if constexpr (KC) return *(AIPT_LDS V*)(lds + at[0][H] + n * 2048);
+        else if constexpr (ES == 4) {
+            V v;
+#pragma unroll
+            for (int q = 0; q < 4; q++) v[q] = *(AIPT_LDS float*)(lds + at[n][0] + (H * 16 + q) * R * 4);
+            return v;
+        } else {
             union { i16x4 h[2]; V v; } u;
-            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][0]));
-            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][1]));
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][0] + H * 32 * R * 2));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((AIPT_LDS i16x4*)(lds + at[n][1] + H * 32 * R * 2));
             return u.v;
         }
     }
@@ -274,31 +301,34 @@ template <typename T, int ACT> __device__ inline void epilogue8(const GemmArgs& 
 #pragma unroll
         for (int e = 0; e < 8; e++) b[e] = bias_j[e];
     }
-    Chunk<T> q;
+    struct alignas(16) Oct { T v[8]; } q;
 #pragma unroll
     for (int e = 0; e < 8; e++) z[e] += b[e];
     if (g.pre) {
 #pragma unroll
         for (int e = 0; e < 8; e++) q.v[e] = (T)z[e];
-        *(Chunk<T>*)((T*)g.pre + i * g.pi + j) = q;
+        *(Oct*)((T*)g.pre + i * g.pi + j) = q;
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) z[e] = act_of(z[e], ACT, g.slope);
     if (g.res) {
-        const Chunk<T> r = *(const Chunk<T>*)((const T*)g.res + i * g.ri + j);
+        const Oct r = *(const Oct*)((const T*)g.res + i * g.ri + j);
 #pragma unroll
         for (int e = 0; e < 8; e++) z[e] += (float)r.v[e];
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) q.v[e] = (T)z[e];
-    *(Chunk<T>*)((T*)g.c + i * g.cs + j) = q;
+    *(Oct*)((T*)g.c + i * g.cs + j) = q;
 }
 
-template <typename T, bool AK, bool BK, int TI, int TJ, int WI, int WJ, int ST>
+template <typename T, bool AK, bool BK, int TI, int TJ, int WI, int WJ, int S, int W>
 __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
-    constexpr int NT = WI * WJ * 64, WTI = TI / WI, WTJ = TJ / WJ, FI = WTI / 16, FJ = WTJ / 16, SB = (TI + TJ) * 64;
+    constexpr int NT = WI * WJ * 64, WTI = TI / WI, WTJ = TJ / WJ, FI = WTI / 16, FJ = WTJ / 16;
+    static_assert(TI == TJ || S % 2 == 0, "an odd ring's slots hold A and B in turn");
+    constexpr int SA = TI * 128, SB = TJ * 128;              // bytes of a slot
     constexpr int SLAB = WTI < 64 ? WTI : 64;                // rows of a wave's results that go through LDS at a time
-    constexpr int BYTES = ST * SB > WI * WJ * SLAB * WTJ * 4 ? ST * SB : WI * WJ * SLAB * WTJ * 4;
+    constexpr int RING = S % 2 ? S * SA : S / 2 * (SA + SB);
+    constexpr int BYTES = RING > WI * WJ * SLAB * WTJ * 4 ? RING : WI * WJ * SLAB * WTJ * 4;
     __shared__ __attribute__((aligned(1024))) char lds_[BYTES];
     AIPT_LDS char* lds = (AIPT_LDS char*)lds_;
     using V = typename Frag<T>::V;
@@ -311,10 +341,10 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
     // ... in columns of 8 tiles
     const int band = 8 * g.tiles_j, b0 = job / band * 8, bh = min(8, g.tiles_i - b0);
     const int i0 = (b0 + (job % band) % bh) * TI, j0 = (job % band) / bh * TJ;
-    const int k0 = split * g.k_split, k1 = min(g.K, k0 + g.k_split), n = (k1 - k0 + 31) >> 5;
+    const int k0 = split * g.k_split, k1 = min(g.K, k0 + g.k_split), KP = 128 / (int)sizeof(T), n = (k1 - k0 + KP - 1) / KP;
 
-    TileLoad<AK, TI, NT> la;
-    TileLoad<BK, TJ, NT> lb;
+    TileLoad<sizeof(T), AK, TI, NT, W> la;
+    TileLoad<sizeof(T), BK, TJ, NT, W> lb;
     la.init(g.a, g.as, i0, g.I, k0, tid);
     lb.init(g.b, g.bs, j0, g.J, k0, tid);
     const int wi = wave / WJ * WTI, wj = wave % WJ * WTJ;
@@ -322,63 +352,89 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
     TileRead<T, BK, TJ, FJ> rb;
     ra.init(wi, lane);
     rb.init(wj, lane);
-    constexpr int LA = decltype(la)::L, LB = decltype(lb)::L, L = LA + LB;
+    constexpr int LA = decltype(la)::L, LB = decltype(lb)::L;
+    // bytes from the ring's start to the slot of load u (2 P: A, 2 P + 1: B of pair P); `slot`: u % S
+    auto place = [&](int slot) { return lds + (S % 2 ? slot * SA : (slot >> 1) * (SA + SB) + (slot & 1) * SA); };
+    auto next = [](int slot, int by) { slot += by; return slot >= S ? slot - S : slot; };
     f32x4 acc[FI][FJ] = {};
     settle<FI * FJ>(&acc[0][0]);
     V a0[FI], b0f[FJ], a1[FI], b1f[FJ];
 #pragma unroll
-    for (int t = 0; t < ST; t++) {
-        const auto sa = la.at(t), sb = lb.at(t);
+    for (int u = 0; u < S - 1; u++) {
+        const int t = u / 2, left = k1 - k0 - t * KP;
+        if (u % 2 == 0) {
+            const auto rs = la.at(t);
 #pragma unroll
-        for (int i = 0; i < L; i++)
-            if (i < LA) la.one(i, sa, k1 - k0 - t * 32, lds + t * SB, wave);
-            else lb.one(i - LA, sb, k1 - k0 - t * 32, lds + t * SB + TI * 64, wave);
+            for (int i = 0; i < LA; i++) la.one(i, rs, left, place(u), wave);
+        } else {
+            const auto rs = lb.at(t);
+#pragma unroll
+            for (int i = 0; i < LB; i++) lb.one(i, rs, left, place(u), wave);
+        }
     }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((ST - 1) * L) : "memory");
+    // loads behind A(0) B(0), and, at a barrier, behind the pair that it makes visible: they may still be under way
+    constexpr int W0 = (S - 3) / 2 * (LA + LB) + (S % 2 ? 0 : LA), W1 = (S - 4) / 2 * (LA + LB) + (S % 2 ? LA : 0);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(W0) : "memory");
 #pragma unroll
-    for (int p = 0; p < FI; p++) a0[p] = ra.one(p, lds);
+    for (int p = 0; p < FI; p++) a0[p] = ra.template one<0>(p, place(0));
 #pragma unroll
-    for (int q = 0; q < FJ; q++) b0f[q] = rb.one(q, lds + TI * 64);
-    int slot = 0;
+    for (int q = 0; q < FJ; q++) b0f[q] = rb.template one<0>(q, place(1));
+    // A step: the products of one half of a pair, from registers, and between them the reads of the next half and the loads of a slot.
     // The order is the program's, not the scheduler's (which would read the next fragments behind the last product, into the registers
-    // that these leave, and so wait for them): rows of FJ products, the reads of the next fragments between the first half of the rows, the
-    // loads of a later step between the second half.
-    auto step = [&](int t, V* a, V* b, V* an, V* bn) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((ST - 2) * L) : "memory");
-        AIPT_LDS char* into = lds + slot * SB;
-        slot = slot == ST - 1 ? 0 : slot + 1;
-        AIPT_LDS char* from = lds + slot * SB;
-        const auto sa = la.at(t + ST), sb = lb.at(t + ST);
-        const int left = k1 - k0 - (t + ST) * 32;
-        constexpr int H = FI / 2, R = (FI + FJ + H - 1) / H, G = (L + H - 1) / H;
+    // that these leave, and so wait for them): rows of FJ products, the reads between the first half of the rows, the loads between the
+    // second.
+    auto step = [&](auto half, auto is_a, int t, AIPT_LDS char* into, AIPT_LDS char* from_a, AIPT_LDS char* from_b, V* a, V* b, V* an, V* bn) {
+        constexpr int HALF = decltype(half)::value, LN = decltype(is_a)::value ? LA : LB;
+        constexpr int H = FI / 2, R = (FI + FJ + H - 1) / H, G = (LN + H - 1) / H;
+        const auto rs = decltype(is_a)::value ? la.at(t) : lb.at(t);
+        const int left = k1 - k0 - t * KP;
 #pragma unroll
         for (int p = 0; p < FI; p++) {
             if (p < H) {
 #pragma unroll
                 for (int r = p * R; r < (p + 1) * R && r < FI + FJ; r++) {
-                    if (r < FI) an[r] = ra.one(r, from);
-                    else bn[r - FI] = rb.one(r - FI, from + TI * 64);
+                    if (r < FI) an[r] = ra.template one<HALF>(r, from_a);
+                    else bn[r - FI] = rb.template one<HALF>(r - FI, from_b);
                 }
             } else {
 #pragma unroll
-                for (int i = (p - H) * G; i < (p - H + 1) * G && i < L; i++)
-                    if (i < LA) la.one(i, sa, left, into, wave);
-                    else lb.one(i - LA, sb, left, into + TI * 64, wave);
+                for (int i = (p - H) * G; i < (p - H + 1) * G && i < LN; i++)
+                    if constexpr (decltype(is_a)::value) la.one(i, rs, left, into, wave);
+                    else lb.one(i, rs, left, into, wave);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int q = 0; q < FJ; q++) Frag<T>::mac(b[q], a[p], acc[p][q]);
+            for (int q = 0; q < FJ; q++) Frag<T>::template mac<0>(b[q], a[p], acc[p][q]);
+            if constexpr (Frag<T>::Q == 4) {
+#pragma unroll
+                for (int q = 0; q < FJ; q++) Frag<T>::template mac<1>(b[q], a[p], acc[p][q]);
+#pragma unroll
+                for (int q = 0; q < FJ; q++) Frag<T>::template mac<2>(b[q], a[p], acc[p][q]);
+#pragma unroll
+                for (int q = 0; q < FJ; q++) Frag<T>::template mac<3>(b[q], a[p], acc[p][q]);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    for (int t = 0; t < n; t += 2) {                         // (an odd last step adds zeros)
-        step(t, a0, b0f, a1, b1f);
-        step(t + 1, a1, b1f, a0, b0f);
+    using std::integral_constant;
+    using First = integral_constant<int, 0>;
+    using Second = integral_constant<int, 1>;
+    // in the first step of pair P the load 2 P - 1 + S goes out, in the second 2 P + S, into the slots of 2 P - 1 and 2 P
+    using OddIsA = integral_constant<bool, S % 2 != 0>;      // what 2 P - 1 + S is
+    using EvenIsA = integral_constant<bool, S % 2 == 0>;     // what 2 P + S is
+    int slot = 0;                    // of A(P)
+    for (int P = 0; P < n; P++) {
+        const int sb = next(slot, 1), sa2 = next(slot, 2), sb2 = next(slot, 3);
+        step(Second{}, OddIsA{}, P + (S - 1) / 2, place(next(slot, S - 1)), place(slot), place(sb), a0, b0f, a1, b1f);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(W1) : "memory");
+        step(First{}, EvenIsA{}, P + S / 2, place(slot), place(sa2), place(sb2), a1, b1f, a0, b0f);
+        slot = sa2;
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     settle<FI * FJ>(&acc[0][0]);
 
     // results: through a slab of LDS of the wave's own (chunk c of row r at c ^ (r % 16)), so that rows are stored in 16-byte pieces
+    constexpr int XM = WTJ / 4 < 16 ? WTJ / 4 - 1 : 15;
     AIPT_LDS char* slab = lds + wave * (SLAB * WTJ * 4);
     constexpr int LR = WTJ / 8, RPI = 64 / LR;               // lanes of a row, rows of an instruction
     const int j = j0 + wj + lane % LR * 8;
@@ -393,23 +449,26 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
 #pragma unroll
             for (int q = 0; q < FJ; q++) {
                 const int r = p * 16 + (lane & 15), c = q * 4 + (lane >> 4);
-                *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & 15)) * 16)) = acc[s * (SLAB / 16) + p][q];
+                *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & XM)) * 16)) = acc[s * (SLAB / 16) + p][q];
             }
         auto rows = [&](auto done) {
             for (int r = lane / LR; r < SLAB; r += RPI) {
                 const int i = i0 + wi + s * SLAB + r;
                 if (i >= g.I || j >= g.J) continue;
-                float z[8];
+                alignas(16) float z[8];
                 const int c = lane % LR * 2;
-                *(f32x4*)z = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & 15)) * 16));
-                *(f32x4*)(z + 4) = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + (((c + 1) ^ (r & 15)) * 16));
+                *(f32x4*)z = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & XM)) * 16));
+                *(f32x4*)(z + 4) = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + (((c + 1) ^ (r & XM)) * 16));
                 done(i, z);
             }
         };
         if (g.splits > 1) rows([&](int i, float* z) {
             float* o = g.partial + ((long long)split * g.I + i) * g.J + j;
+            if (j + 8 <= g.J && !(g.J & 3)) { *(f32x4*)o = *(f32x4*)z; *(f32x4*)(o + 4) = *(f32x4*)(z + 4); }
+            else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) if (j + e < g.J) o[e] = z[e];
+                for (int e = 0; e < 8; e++) if (j + e < g.J) o[e] = z[e];
+            }
         });
         else if (!whole) rows([&](int i, float* z) {
 #pragma unroll
@@ -422,14 +481,48 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
     }
 }
 
-// the splits of a long contraction, added in order, and the epilogue
+// the splits of a long contraction, added in order, and the epilogue: four neighbours a thread
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join(const GemmArgs g) {
-    const long long n = (long long)g.I * g.J;
+    const int per = (g.J + 3) / 4;
+    const long long quads = (long long)g.I * per, n = (long long)g.I * g.J;
+    const bool quad16 = !(g.J & 3);
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < quads; at += (long long)gridDim.x * 256) {
+        const int i = (int)(at / per), j = (int)(at - (long long)i * per) * 4;
+        const float* p = g.partial + (long long)i * g.J + j;
+        float s[4] = {};
+        if (quad16) {
+            for (int k = 0; k < g.splits; k++, p += n) {
+                const float4 v = *(const float4*)p;
+                s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+            }
+        } else {
+            for (int k = 0; k < g.splits; k++, p += n)
+#pragma unroll
+                for (int e = 0; e < 4; e++) if (j + e < g.J) s[e] += p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) if (j + e < g.J) epilogue<T>(g, i, j + e, s[e]);
+    }
+}
+
+// ---- 16-bit lines that begin anywhere, copied to lines on 16 bytes, padded with zeros: twice the operand's bytes, once, for loads of 16 bytes
+// in every tile that reads it (1375 x 909 by 303 x 909: 58 us by gemm_any)
+struct PackArgs {
+    struct { const unsigned short* p; Chunk<unsigned short>* to; long long stride, chunks; int len, line; } m[2];      // line: chunks of a line
+};
+__global__ __launch_bounds__(256) void pack_lines(const PackArgs g) {
+    const long long n = g.m[0].chunks + g.m[1].chunks;
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
-        float s = 0;
-        for (int k = 0; k < g.splits; k++) s += g.partial[k * n + at];
-        epilogue<T>(g, (int)(at / g.J), (int)(at % g.J), s);
+        const bool second = at >= g.m[0].chunks;
+        const auto& m = g.m[second];
+        const long long c = second ? at - g.m[0].chunks : at, l = c / m.line;
+        const int k = (int)(c - l * m.line) * 8;
+        const unsigned short* s = m.p + l * m.stride + k;
+        Chunk<unsigned short> q;
+#pragma unroll
+        for (int e = 0; e < 8; e++) q.v[e] = k + e < m.len ? s[e] : (unsigned short)0;
+        m.to[c] = q;
     }
 }
 
@@ -537,49 +630,115 @@ static Extent extent_of(const aipt_matrix& m, long long n0, long long n1, int es
     return {v.p, n1, ((n0 > 1 ? (n0 - 1) * v.ri : 0) + 1) * es, (n1 > 1 ? v.rj : 0) * es};
 }
 
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
 struct Plan {                        // a product as it will be launched, and the workspace it wants
     GemmArgs g = {};
     bool ak = true, bk = true;
     int tile = 0;                    // 0: gemm_any; else gemm_tile of this size
-    unsigned threads = 256;
-    size_t partial_bytes = 0, blocks = 0;
+    bool small = false;              // ... with loads of 4 bytes
+    PackArgs pack = {};              // operands that are copied first
+    size_t pack_bytes = 0, partial_bytes = 0, blocks = 0;
     bool fits = true;
+    size_t bytes() const { return pack_bytes + partial_bytes; }
 };
 
+// The sizes of gemm_tile, and what they cost: `start` microseconds for a workgroup's first loads and its results, pair[c] for a pair of its steps
+// while c + 1 workgroups share the CU (16-bit types; floats are bound by the matrix instructions, `wide` a pair).  Measured, bf16, where each
+// wins: 4096 x 4096 x 4096: 256 x 256 104 us, 128 x 128 121; 2048^3: 128 x 128 23, 64 x 64 29, 256 x 256 48; 1024^3: 64 x 64 8.4, 128 x 128
+// 12; 942080 x 32 x 64: 256 x 32 37, 64 x 64 60, 128 x 128 80; 942080 x 64 x 128: 256 x 64 86, 64 x 64 95, 128 x 128 101.
+static const struct Tile { int i, j, fit; double start, pair[3], wide; } TILES[] = {
+    {},
+    {256, 256, 1, 12, {1.4, 0, 0}, 7.6},
+    {128, 128, 2, 4.5, {0.6, 1.0, 0}, 2.0},
+    {64, 64, 3, 2.5, {0.24, 0.36, 0.55}, 0.5},
+    {256, 64, 2, 5.5, {0.8, 1.2, 0}, 2.0},
+    {256, 32, 2, 4, {0.7, 0.9, 0}, 1.0},
+};
+constexpr int NTILES = 6, CUS = 256;
+
+// The tile and how often the contraction is split, by the estimate above: rounds of workgroups, and for a split the partial sums' way out and
+// back (a join's launch and some 3.5 TB/s).  small: the lines are on 4 bytes only.
+static double pick(bool wide, bool small, long long I, long long J, long long pairs, int& tile, long long& splits) {
+    double best = 1e30;
+    for (int t = 1; t < NTILES; t++) {
+        const Tile& c = TILES[t];
+        if (small && t != 3 && t != 5) continue;
+        const long long tiles = ((I + c.i - 1) / c.i) * ((J + c.j - 1) / c.j);
+        for (int fill = 0; fill <= c.fit; fill++) {
+            long long s = fill ? std::min(CUS * fill / std::max(1ll, tiles), pairs / 2) : 1;
+            if (s < 1 || (fill && s == 1)) continue;
+            const long long n = (pairs + s - 1) / s, blocks = tiles * s, full = blocks / (CUS * c.fit), rest = blocks - full * CUS * c.fit;
+            auto round = [&](int with) { return c.start + n * (wide ? std::max(c.wide * with, c.pair[with - 1]) : c.pair[with - 1]); };
+            double us = full * round(c.fit);
+            if (rest) us += round((int)((rest + CUS - 1) / CUS));
+            if (s > 1) us += 4 + (double)(s + 1) * I * J * 4 / 3.5e6;
+            if (us < best) { best = us; tile = t; splits = s; }
+        }
+    }
+    return best;
+}
+
 // C[i][j] = sum_k A[i][k] B[j][k]; A (I x K) and B (J x K) by their strides; the result's j axis contiguous
-static Plan plan_gemm(int type, const View& a, const View& b, long long I, long long J, long long K) {
+static Plan plan_gemm(int type, View a, View b, long long I, long long J, long long K) {
     Plan p;
     const int es = type_bytes(type), E = 16 / es, ks = 8 * E;
-    p.g.a = a.p; p.g.b = b.p;
     p.ak = a.second; p.bk = b.second;
-    p.g.as = a.other; p.g.bs = b.other;
     p.g.I = (int)I; p.g.J = (int)J; p.g.K = (int)K;
+    // gemm_tile wants lines on 16 bytes that hold whole 16-byte chunks (or, in two of its sizes, on 4), and a tile's lines within 31 bits of
+    // its first
+    auto unit = [&](const View& v, long long len) {
+        if (v.other * es * 256 >= (1ll << 31)) return 0;
+        for (int w : {16, 4})
+            if (!((uintptr_t)v.p & (w - 1)) && v.other * es % w == 0 && (v.padded || len * es % w == 0)) return w;
+        return 0;
+    };
+    int w[2];
+    for (int o = 0; o < 2; o++) {
+        View& v = o ? b : a;
+        const long long rows = o ? J : I, len = v.second ? K : rows, lines = v.second ? rows : K, line = (len + E - 1) / E;
+        w[o] = unit(v, len);
+        if (!w[o] && es == 2 && I && J && K && line * 16 * 256 < (1ll << 31)) {
+            p.pack.m[o] = {(const unsigned short*)v.p, (Chunk<unsigned short>*)p.pack_bytes, v.other, lines * line, (int)len, (int)line};   // (`to`: an offset for now)
+            p.pack_bytes += up256((size_t)(lines * line) * 16);
+            v = {nullptr, v.second ? line * E : 1, v.second ? 1 : line * E, v.second, line * E, true};
+            w[o] = 16;
+        }
+    }
+    p.g.a = a.p; p.g.b = b.p;
+    p.g.as = a.other; p.g.bs = b.other;
     p.g.avec = !((uintptr_t)a.p & 15) && (a.other % E == 0);
     p.g.bvec = !((uintptr_t)b.p & 15) && (b.other % E == 0);
-    // gemm_tile wants 16-bit elements, lines on 16 bytes that hold whole 16-byte chunks, and a tile's lines within 31 bits of its first
-    auto lines_ok = [&](const View& v, bool vec, long long len) { return vec && (v.padded || len % E == 0) && v.other * 2 * 256 < (1ll << 31); };
-    if (es == 2 && K >= 32 && lines_ok(a, p.g.avec, a.second ? K : I) && lines_ok(b, p.g.bvec, b.second ? K : J)) p.tile = 256;
-    const int ts = p.tile ? p.tile : GT;
-    p.g.tiles_i = (int)((I + ts - 1) / ts); p.g.tiles_j = (int)((J + ts - 1) / ts);
-    const long long tiles = (long long)p.g.tiles_i * p.g.tiles_j, steps = (K + ks - 1) / ks;
-    // few tiles and a long contraction: split it until some 512 workgroups (two a CU) run, none with fewer than 4 steps
+    const long long pairs = (K + ks - 1) / ks;
     long long splits = 1;
-    const long long want = p.tile ? 256 : 512;
-    if (tiles > 0 && tiles < want) splits = std::max(1ll, std::min(want / tiles, steps / 4));
+    p.small = std::min(w[0], w[1]) == 4;
+    if (w[0] && w[1] && I && J) pick(es == 4, p.small, I, J, pairs, p.tile, splits);
+    const int ti = p.tile ? TILES[p.tile].i : GT, tj = p.tile ? TILES[p.tile].j : GT, step = ks;
+    p.g.tiles_i = (int)((I + ti - 1) / ti); p.g.tiles_j = (int)((J + tj - 1) / tj);
+    const long long tiles = (long long)p.g.tiles_i * p.g.tiles_j, steps = pairs;
+    // gemm_any: two workgroups a CU, none with fewer than 4 steps
+    if (!p.tile) splits = tiles > 0 && tiles < 512 ? std::max(1ll, std::min(512 / tiles, steps / 4)) : 1;
     const long long per = splits > 1 ? (steps + splits - 1) / splits : std::max(1ll, steps);
     splits = std::max(1ll, (steps + per - 1) / per);
     p.g.splits = (int)splits;
-    p.g.k_split = (int)std::min<long long>(per * ks, 0x7fffffffll - ks);
+    p.g.k_split = (int)std::min<long long>(per * step, 0x7fffffffll - step);
     p.blocks = (size_t)(tiles * splits);
     p.fits = grid_fits(p.blocks, 256);
     if (splits > 1) p.partial_bytes = (size_t)splits * I * J * sizeof(float);
     return p;
 }
 
+template <typename T, int TI, int TJ, int WI, int WJ, int S, int W> static void (*tile_kernel(const Plan& p))(GemmArgs) {
+    return p.ak ? (p.bk ? gemm_tile<T, true, true, TI, TJ, WI, WJ, S, W> : gemm_tile<T, true, false, TI, TJ, WI, WJ, S, W>)
+                : (p.bk ? gemm_tile<T, false, true, TI, TJ, WI, WJ, S, W> : gemm_tile<T, false, false, TI, TJ, WI, WJ, S, W>);
+}
 template <typename T> static void (*gemm_of(const Plan& p))(GemmArgs) {
-    if constexpr (sizeof(T) == 2) {
-        if (p.tile) return p.ak ? (p.bk ? gemm_tile<T, true, true, 256, 256, 2, 2, 4> : gemm_tile<T, true, false, 256, 256, 2, 2, 4>)
-                                : (p.bk ? gemm_tile<T, false, true, 256, 256, 2, 2, 4> : gemm_tile<T, false, false, 256, 256, 2, 2, 4>);
+    switch (p.tile) {
+        case 1: return tile_kernel<T, 256, 256, 2, 2, 5, 16>(p);
+        case 2: return tile_kernel<T, 128, 128, 2, 2, 5, 16>(p);
+        case 3: return p.small ? tile_kernel<T, 64, 64, 2, 2, 6, 4>(p) : tile_kernel<T, 64, 64, 2, 2, 6, 16>(p);
+        case 4: return tile_kernel<T, 256, 64, 4, 1, 4, 16>(p);
+        case 5: return p.small ? tile_kernel<T, 256, 32, 4, 1, 4, 4>(p) : tile_kernel<T, 256, 32, 4, 1, 4, 16>(p);
     }
     return p.ak ? (p.bk ? gemm_any<T, true, true> : gemm_any<T, true, false>) : (p.bk ? gemm_any<T, false, true> : gemm_any<T, false, false>);
 }
@@ -591,11 +750,20 @@ static int rows16(int es, const GemmArgs& g) {
 
 template <typename T> static hipError_t run_gemm_t(hipStream_t st, Plan& p, void* ws) {
     if (!p.blocks) return hipSuccess;
-    p.g.partial = (float*)ws;
+    if (p.pack_bytes) {
+        for (int o = 0; o < 2; o++) {
+            if (!p.pack.m[o].chunks) continue;
+            p.pack.m[o].to = (Chunk<unsigned short>*)((char*)ws + (size_t)p.pack.m[o].to);
+            (o ? p.g.b : p.g.a) = p.pack.m[o].to;
+        }
+        const hipError_t e = launch(pack_lines, (size_t)std::min<long long>((p.pack.m[0].chunks + p.pack.m[1].chunks + 255) / 256, 8192), 256, 0, st, p.pack);
+        if (e != hipSuccess) return e;
+    }
+    p.g.partial = (float*)((char*)ws + p.pack_bytes);
     p.g.c16 = rows16(sizeof(T), p.g);
     hipError_t e = launch(gemm_of<T>(p), p.blocks, 256, 0, st, p.g);
     if (e == hipSuccess && p.g.splits > 1)
-        e = launch(gemm_join<T>, std::min<size_t>(((size_t)p.g.I * p.g.J + 255) / 256, 4096), 256, 0, st, p.g);
+        e = launch(gemm_join<T>, std::min<size_t>(((size_t)p.g.I * ((p.g.J + 3) / 4) + 255) / 256, 4096), 256, 0, st, p.g);
     return e;
 }
 static hipError_t run_gemm(int type, hipStream_t st, Plan& p, void* ws) {
@@ -623,7 +791,6 @@ struct GradPlan {
     size_t dz_bytes = 0, part_bytes = 0, gemm_bytes = 0, dz_blocks = 0;
     size_t bytes() const { return dz_bytes + part_bytes + gemm_bytes; }
 };
-static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
     GradPlan p;
     const int es = type_bytes(a->type), E = 16 / es;
@@ -661,7 +828,7 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         p.dw = o.second ? plan_gemm(a->type, flip(d), flip(x), a->n, a->k, a->m) : plan_gemm(a->type, flip(x), flip(d), a->k, a->n, a->m);
         p.dw.g.c = a->dw.data; p.dw.g.cs = o.other;
     }
-    p.gemm_bytes = up256(std::max(p.want_dx ? p.dx.partial_bytes : 0, p.want_dw ? p.dw.partial_bytes : 0));
+    p.gemm_bytes = up256(std::max(p.want_dx ? p.dx.bytes() : 0, p.want_dw ? p.dw.bytes() : 0));
     return p;
 }
 
@@ -718,7 +885,7 @@ int aipt_linear_workspace(aipt_ctx* ctx, const aipt_linear_args* a, size_t* byte
     if (!bytes) return fail(ctx, AIPT_E_INVALID, "aipt_linear_workspace: bytes is NULL");
     const int rc = aipt::forward_check(ctx, "aipt_linear_workspace", a, false);
     if (rc) return rc;
-    *bytes = aipt::plan_forward(a).partial_bytes;
+    *bytes = aipt::plan_forward(a).bytes();
     return AIPT_OK;
 }
 
@@ -729,11 +896,11 @@ int aipt_linear(aipt_ctx* ctx, const aipt_linear_args* a, void* d_workspace, siz
     const int es = aipt::type_bytes(a->type);
     aipt::Plan p = aipt::plan_forward(a);
     if (!p.fits) return fail(ctx, AIPT_E_INVALID, "%s: %lld x %lld has too many tiles", me, a->m, a->n);
-    if (p.partial_bytes && (!d_workspace || workspace_bytes < p.partial_bytes || ((uintptr_t)d_workspace & 255)))
-        return fail(ctx, AIPT_E_INVALID, "%s: workspace of %zu bytes, %zu are wanted, 256-byte aligned", me, workspace_bytes, p.partial_bytes);
+    if (p.bytes() && (!d_workspace || workspace_bytes < p.bytes() || ((uintptr_t)d_workspace & 255)))
+        return fail(ctx, AIPT_E_INVALID, "%s: workspace of %zu bytes, %zu are wanted, 256-byte aligned", me, workspace_bytes, p.bytes());
     const aipt::Extent x = aipt::extent_of(a->x, a->m, a->k, es), w = aipt::extent_of(a->w, a->n, a->k, es), y = aipt::extent_of(a->y, a->m, a->n, es),
                        r = aipt::extent_of(a->residual, a->m, a->n, es), z = aipt::extent_of(a->preact, a->m, a->n, es), b = {(const char*)a->bias, 1, a->n * es, 0},
-                       s = {(const char*)d_workspace, 1, (long long)p.partial_bytes, 0};
+                       s = {(const char*)d_workspace, 1, (long long)p.bytes(), 0};
     const bool in_place = a->residual.data == a->y.data && a->residual.row_stride == a->y.row_stride && a->residual.col_stride == a->y.col_stride;
     for (const aipt::Extent& o : {y, z, s})
         for (const aipt::Extent& i : {x, w, b}) if (aipt::overlap(o, i)) return fail(ctx, AIPT_E_INVALID, "%s: an output overlaps an input", me);

@@ -362,7 +362,7 @@ typedef struct aipt_linear_args {
     aipt_matrix x, w, y, residual, preact;
     const void* bias;
 } aipt_linear_args;
-int aipt_linear_workspace(aipt_ctx* ctx, const aipt_linear_args* args, size_t* bytes);      /* pointers are not looked at */
+int aipt_linear_workspace(aipt_ctx* ctx, const aipt_linear_args* args, size_t* bytes);      /* of a call with these very arguments: the pointers' alignment counts */
 int aipt_linear(aipt_ctx* ctx, const aipt_linear_args* args, void* d_workspace, size_t workspace_bytes);
 
 /* Gradients: dz = dy * act'(z);  dx = dz w  [m][k];  dw = dz^T x  [n][k];  dbias = sum over rows of dz  [n].  Outputs whose data is
@@ -376,7 +376,7 @@ typedef struct aipt_linear_grad_args {
     aipt_matrix dy, x, w, preact, dx, dw;
     void* dbias;
 } aipt_linear_grad_args;
-int aipt_linear_backward_workspace(aipt_ctx* ctx, const aipt_linear_grad_args* args, size_t* bytes);   /* looks at which outputs are wanted, not where */
+int aipt_linear_backward_workspace(aipt_ctx* ctx, const aipt_linear_grad_args* args, size_t* bytes);
 int aipt_linear_backward(aipt_ctx* ctx, const aipt_linear_grad_args* args, void* d_workspace, size_t workspace_bytes);
 
 /* The norms around a residual block, with its gate and residual scale.  For every row of c channels:
