@@ -50,8 +50,13 @@ template <int LANES> struct RowSum {
     float2* lds;
     int turn = 0;
     __device__ void operator()(float& a, float& b) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+        if constexpr (LANES == 16) {
+            a = sum16(a);
+            b = sum16(b);
+            return;
+        }
+        a = wave_sum(a);
+        b = wave_sum(b);
         if constexpr (LANES > 64) {
             constexpr int W = LANES / 64;
             float2* s = lds + turn * W;
@@ -173,231 +178,373 @@ struct NormBwd {
     void *dx, *dy, *dgate;
     float* part;                     // [parts][5][c]: A, B, W, V, Q
     long long rows, per_gate, dhs, dzs, ys, hs, dxs, dys;
-    long long span;                  // rows of a part
+    long long span;                  // rows of a part (whole gates: gates)
     long long parts_per_gate;        // > 0: a part lies inside one gate's rows; 0: a part is whole gates (their dgate is written at once)
-    int c, layer, sums;              // sums: whether A, B, W, V are wanted (else dgate alone, or none)
+    int c;
 };
 
-template <typename T, int V, int N, int LANES>
+// One row in registers as it lies in memory.
+template <typename T, int V, int N> struct RawRow {
+    struct alignas(V == 1 ? sizeof(T) : 16) E { T v[V]; } e[N];
+    template <int LANES> __device__ inline void load(const void* base, long long at, int lane, int c) {
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int col = (n * LANES + lane) * V;
+            if (col < c) e[n] = *(const E*)((const T*)base + at + col);
+            else {
+#pragma unroll
+                for (int i = 0; i < V; i++) e[n].v[i] = (T)0.f;
+            }
+        }
+    }
+};
+
+// A workgroup is a part: ROWS rows at a time, LANES lanes a row.  The next row's loads go out before this one's sums are waited for (rows of few
+// registers; with 4 096 floats a row there is no room).  WHOLE: gates change within the part -- A and B are added up gate by gate; else the
+// gate is one number a column and P = sum t yhat, T = sum t give A, B and Q at the end.
+template <typename T, int V, int N, int LANES, bool LAYER, bool WHOLE>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_bwd(const NormBwd a) {
     constexpr int THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;
+    constexpr bool AHEAD = !WHOLE && N * V * sizeof(T) <= 32 && LANES <= 512, KEEP = !WHOLE && N * V <= 16 && LANES <= 512;
     __shared__ float2 lds[2 * (THREADS / 64)];
+    __shared__ float sums[LANES < 256 ? THREADS * V * N : 1];
     RowSum<LANES> row_sum{lds};
-    const int lane = threadIdx.x % LANES;
+    const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float inv_c = 1.f / (float)a.c;
-    // a part is what LANES lanes handle: rows [r0, r1), one after the other
-    const long long part = (long long)blockIdx.x * ROWS + threadIdx.x / LANES;
-    long long r0, r1;
-    if (a.parts_per_gate) {
-        const long long gate = part / a.parts_per_gate, k = part % a.parts_per_gate;
-        r0 = gate * a.per_gate + min(k * a.span, a.per_gate);
-        r1 = gate * a.per_gate + min((k + 1) * a.span, a.per_gate);
-        if (r0 > a.rows) r0 = a.rows;
-        if (r1 > a.rows) r1 = a.rows;
+    const long long part = blockIdx.x;
+    long long r0, r1, gate = 0, gates_left = 0;
+    const int stride = WHOLE ? 1 : ROWS;
+    if (WHOLE) {                     // gates sub, sub + ROWS, ... of the part's
+        const long long g0 = part * a.span + sub, g1 = min((part + 1) * a.span, a.rows / a.per_gate);
+        gate = g0;
+        gates_left = g0 < g1 ? (g1 - g0 + ROWS - 1) / ROWS : 0;
+        r0 = g0 * a.per_gate;
+        r1 = r0 + (gates_left ? a.per_gate : 0);
     } else {
-        r0 = min(part * a.span, a.rows);
-        r1 = min((part + 1) * a.span, a.rows);
+        gate = part / a.parts_per_gate;
+        const long long k = part % a.parts_per_gate;
+        r0 = gate * a.per_gate + min(k * a.span, a.per_gate) + sub;
+        r1 = gate * a.per_gate + min((k + 1) * a.span, a.per_gate);
     }
-    float A[N][V], B[N][V], W[N][V], D[N][V], Q[N][V];
+    float P[N][V], Tt[LAYER ? N : 1][V], W[N][V], D[LAYER ? N : 1][V], A[WHOLE ? N : 1][V], B[WHOLE && LAYER ? N : 1][V];
+    float k1[KEEP ? N : 1][V], k2[KEEP ? N : 1][V];
 #pragma unroll
     for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int i = 0; i < V; i++) A[n][i] = B[n][i] = W[n][i] = D[n][i] = Q[n][i] = 0;
-    long long gate_left = 0;         // rows to go of the present gate (whole gates only)
-    for (long long r = r0; r < r1; r++) {
-        const float4 st = *(const float4*)(a.stats + r * 4);
-        float t[N][V], e[N][V];
-        float s1 = 0, s2 = 0;
-        // t = dh + norm'(dz w2); e: hhat
+        for (int i = 0; i < V; i++) {
+            P[n][i] = W[n][i] = 0;
+            if constexpr (LAYER) Tt[n][i] = D[n][i] = 0;
+            if constexpr (WHOLE) A[n][i] = 0;
+            if constexpr (WHOLE && LAYER) B[n][i] = 0;
+        }
+    // scale * gate * post_weight, and pre_weight, of the lane's columns
+    auto one = [&](float* o) {
+#pragma unroll
+        for (int i = 0; i < V; i++) o[i] = 1;
+    };
+    auto factor = [&](int n, int col, float* o, bool weight) {
+        float q[V];
+        one(o);
+        if (col >= a.c) return;
+        if (a.scale) get<T, V>(a.scale, col, o);
+        if (a.gate) {
+            get<T, V>(a.gate, gate * a.c + col, q);
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] *= q[i];
+        }
+        if (weight && a.w1) {
+            get<T, V>(a.w1, col, q);
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] *= q[i];
+        }
+    };
+    auto factor2 = [&](int col, float* o) {
+        one(o);
+        if (a.w2 && col < a.c) get<T, V>(a.w2, col, o);
+    };
+    if constexpr (KEEP) {
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            const int col = (n * LANES + lane) * V;
-#pragma unroll
-            for (int i = 0; i < V; i++) t[n][i] = e[n][i] = 0;
-            if (a.dz && col < a.c) {
-                float d[V], w[V];
-                get<T, V>(a.dz, r * a.dzs + col, d);
-                get<T, V>(a.h, r * a.hs + col, e[n]);
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    e[n][i] = (e[n][i] - st.z) * st.w;
-                    W[n][i] += d[i] * e[n][i];
-                    D[n][i] += d[i];
-                }
-                if (a.w2) { get<T, V>(a.w2, col, w);
-#pragma unroll
-                    for (int i = 0; i < V; i++) d[i] *= w[i]; }
-#pragma unroll
-                for (int i = 0; i < V; i++) { t[n][i] = d[i]; s1 += d[i]; s2 += d[i] * e[n][i]; }
-            }
+            factor(n, (n * LANES + lane) * V, k1[n], true);
+            factor2((n * LANES + lane) * V, k2[n]);
         }
+    }
+    RawRow<T, V, N> dz, h, dh, y;
+    float4 st = make_float4(0, 0, 0, 0);
+    auto load = [&](long long r) {
+        st = *(const float4*)(a.stats + r * 4);
         if (a.dz) {
-            row_sum(s1, s2);
-            s1 = a.layer ? s1 * inv_c : 0.f;
-            s2 *= inv_c;
+            dz.template load<LANES>(a.dz, r * a.dzs, lane, a.c);
+            h.template load<LANES>(a.h, r * a.hs, lane, a.c);
+        }
+        if (a.dh) dh.template load<LANES>(a.dh, r * a.dhs, lane, a.c);
+        if (a.y) y.template load<LANES>(a.y, r * a.ys, lane, a.c);
+    };
+    // (rows a workgroup shares: every lane of it goes through the same rows, barriers included)
+    for (;;) {
+        if (AHEAD && r0 < r1) load(r0);
+        for (long long r = r0; r < r1; r += stride) {
+            RawRow<T, V, N> dzc, hc, dhc, yc;
+            float4 s4;
+            if constexpr (!AHEAD) load(r);
+            dzc = dz; hc = h; dhc = dh; yc = y; s4 = st;
+            if (AHEAD && r + stride < r1) load(r + stride);
+            float t[N][V], e[N][V], s1 = 0, s2 = 0;
+            if (a.dz) {
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    float w[V];
+                    if constexpr (!KEEP) factor2((n * LANES + lane) * V, w);
+                    const bool in = (n * LANES + lane) * V < a.c;
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        const float d = (float)dzc.e[n].v[i];
+                        e[n][i] = in ? ((float)hc.e[n].v[i] - s4.z) * s4.w : 0.f;
+                        W[n][i] += d * e[n][i];
+                        if constexpr (LAYER) D[n][i] += d;
+                        t[n][i] = d * (KEEP ? k2[KEEP ? n : 0][i] : w[i]);
+                        s1 += t[n][i];
+                        s2 += t[n][i] * e[n][i];
+                    }
+                }
+                row_sum(s1, s2);
+                s1 = LAYER ? s1 * inv_c : 0.f;
+                s2 *= inv_c;
+            }
 #pragma unroll
             for (int n = 0; n < N; n++)
 #pragma unroll
-                for (int i = 0; i < V; i++) t[n][i] = st.w * (t[n][i] - s1 - e[n][i] * s2);
-        }
-        const long long gate_row = a.gate || a.dgate ? r / a.per_gate * a.c : 0;
-        if (!a.parts_per_gate && a.dgate && gate_left == 0) gate_left = a.per_gate;
-        s1 = s2 = 0;
+                for (int i = 0; i < V; i++) {
+                    t[n][i] = a.dz ? s4.w * (t[n][i] - s1 - e[n][i] * s2) : 0.f;
+                    if (a.dh) t[n][i] += (float)dhc.e[n].v[i];
+                }
+            if (a.dx) {
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int col = (n * LANES + lane) * V;
-            if (col < a.c) {
-                float q[V];
-                if (a.dh) { get<T, V>(a.dh, r * a.dhs + col, q);
-#pragma unroll
-                    for (int i = 0; i < V; i++) t[n][i] += q[i]; }
-                if (a.dx) put<T, V>(a.dx, r * a.dxs + col, t[n]);
-                if (a.y) {
-                    float y[V], w[V], g[V], b[V], sc[V];
-                    get<T, V>(a.y, r * a.ys + col, y);
-#pragma unroll
-                    for (int i = 0; i < V; i++) { y[i] = (y[i] - st.x) * st.y; w[i] = 1; g[i] = 1; b[i] = 0; sc[i] = 1; }
-                    if (a.w1) get<T, V>(a.w1, col, w);
-                    if (a.b1) get<T, V>(a.b1, col, b);
-                    if (a.gate) get<T, V>(a.gate, gate_row + col, g);
-                    if (a.scale) get<T, V>(a.scale, col, sc);
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        const float ti = t[n][i], gt = g[i] * ti;
-                        A[n][i] += gt * y[i];
-                        B[n][i] += gt;
-                        Q[n][i] += ti * (w[i] * y[i] + b[i]);
-                        const float d = gt * sc[i] * w[i];
-                        t[n][i] = d; e[n][i] = y[i];
-                        s1 += d; s2 += d * y[i];
-                    }
-                    if (!a.parts_per_gate && a.dgate && gate_left == 1) {
-#pragma unroll
-                        for (int i = 0; i < V; i++) { q[i] = Q[n][i] * sc[i]; Q[n][i] = 0; }
-                        put<T, V>(a.dgate, gate_row + col, q);
-                    }
+                for (int n = 0; n < N; n++) {
+                    const int col = (n * LANES + lane) * V;
+                    if (col < a.c) put<T, V>(a.dx, r * a.dxs + col, t[n]);
                 }
             }
-        }
-        gate_left--;
-        if (a.y && a.dy) {
+            if (!a.y) continue;
+            s1 = s2 = 0;
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                float w[V];
+                const int col = (n * LANES + lane) * V;
+                if constexpr (!KEEP) factor(n, col, w, true);
+                const bool in = col < a.c;
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const float ti = in ? t[n][i] : 0.f, yh = in ? ((float)yc.e[n].v[i] - s4.x) * s4.y : 0.f;
+                    P[n][i] += ti * yh;
+                    if constexpr (LAYER) Tt[n][i] += ti;
+                    const float d = ti * (KEEP ? k1[KEEP ? n : 0][i] : w[i]);
+                    t[n][i] = d; e[n][i] = yh;
+                    s1 += d; s2 += d * yh;
+                }
+            }
+            if (!a.dy) continue;
             row_sum(s1, s2);
-            s1 = a.layer ? s1 * inv_c : 0.f;
+            s1 = LAYER ? s1 * inv_c : 0.f;
             s2 *= inv_c;
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 const int col = (n * LANES + lane) * V;
                 if (col < a.c) {
 #pragma unroll
-                    for (int i = 0; i < V; i++) t[n][i] = st.y * (t[n][i] - s1 - e[n][i] * s2);
+                    for (int i = 0; i < V; i++) t[n][i] = s4.y * (t[n][i] - s1 - e[n][i] * s2);
                     put<T, V>(a.dy, r * a.dys + col, t[n]);
                 }
             }
         }
-    }
-    if (a.part) {
-        float* p = a.part + part * 5 * a.c;
+        if constexpr (!WHOLE) break;
+        else {
+            if (gates_left <= 0) break;
 #pragma unroll
-        for (int n = 0; n < N; n++)
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int col = (n * LANES + lane) * V + i;
+            for (int n = 0; n < N; n++) {
+                const int col = (n * LANES + lane) * V;
                 if (col < a.c) {
-                    if (a.sums) { p[col] = A[n][i]; p[a.c + col] = B[n][i]; p[2 * a.c + col] = W[n][i]; p[3 * a.c + col] = D[n][i]; }
-                    if (a.parts_per_gate) p[4 * a.c + col] = Q[n][i];
+                    float g[V], s[V], w[V], b[V];
+                    one(g); one(s); one(w);
+#pragma unroll
+                    for (int i = 0; i < V; i++) b[i] = 0;
+                    if (a.gate) get<T, V>(a.gate, gate * a.c + col, g);
+                    if (a.scale) get<T, V>(a.scale, col, s);
+                    if (a.w1) get<T, V>(a.w1, col, w);
+                    if (a.b1) get<T, V>(a.b1, col, b);
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        const float tt = LAYER ? Tt[LAYER ? n : 0][i] : 0.f;
+                        A[n][i] += g[i] * P[n][i];
+                        if constexpr (LAYER) { B[n][i] += g[i] * tt; Tt[n][i] = 0; }
+                        s[i] *= w[i] * P[n][i] + b[i] * tt;
+                        P[n][i] = 0;
+                    }
+                    if (a.dgate) put<T, V>(a.dgate, gate * a.c + col, s);
                 }
             }
+            gates_left--;
+            gate += ROWS;
+            r0 = gate * a.per_gate;
+            r1 = r0 + (gates_left > 0 ? a.per_gate : 0);
+        }
+    }
+    if (!a.part) return;
+    // the workgroup's sums: where several rows were handled side by side, added through LDS
+    auto write = [&](int which, auto value) {
+        float* o = a.part + (part * 5 + which) * a.c;
+        if constexpr (LANES >= 256) {
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const int col = (n * LANES + lane) * V + i;
+                    if (col < a.c) o[col] = value(n, i, col);
+                }
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const int col = (n * LANES + lane) * V + i;
+                    sums[sub * (LANES * N * V) + col] = col < a.c ? value(n, i, col) : 0.f;
+                }
+            __syncthreads();
+            for (int col = threadIdx.x; col < a.c; col += THREADS) {
+                float s = 0;
+#pragma unroll
+                for (int k = 0; k < ROWS; k++) s += sums[k * (LANES * N * V) + col];
+                o[col] = s;
+            }
+        }
+    };
+    auto vec = [&](const void* p, long long at, float other) { return p ? (float)((const T*)p)[at] : other; };
+    if (a.y) {
+        if constexpr (WHOLE) {
+            write(0, [&](int n, int i, int) { return A[n][i]; });
+            if constexpr (LAYER) write(1, [&](int n, int i, int) { return B[n][i]; });
+        } else {
+            write(0, [&](int n, int i, int col) { return P[n][i] * vec(a.gate, gate * a.c + col, 1.f); });
+            if constexpr (LAYER) write(1, [&](int n, int i, int col) { return Tt[n][i] * vec(a.gate, gate * a.c + col, 1.f); });
+            if (a.dgate) write(4, [&](int n, int i, int col) { return P[n][i] * vec(a.w1, col, 1.f) + (LAYER ? Tt[LAYER ? n : 0][i] * vec(a.b1, col, 0.f) : 0.f); });
+        }
+    }
+    if (a.dz) {
+        write(2, [&](int n, int i, int) { return W[n][i]; });
+        if constexpr (LAYER) write(3, [&](int n, int i, int) { return D[n][i]; });
     }
 }
 
-// the vectors' gradients from the parts: blockIdx.y 0 adds A, B, W, V over all parts, blockIdx.y 1 + j adds Q over the parts of gate j.
-// 64 columns x 4 lanes of parts, added in a fixed order.
+// The vectors' gradients from the parts, added in a fixed order by 64 columns x 16 lanes of parts.  Job 0: of post_*, 1: of pre_*, 2 + j: dgate's row j.
 struct NormEnd {
     const float* part;
     const void *scale, *w1, *b1;
     void *dgate, *dscale, *dw1, *db1, *dw2, *db2;
     long long parts, parts_per_gate;
-    int c, col_blocks;
+    int c, col_blocks, layer, post, pre;
 };
 template <typename T>
-__global__ __launch_bounds__(256) void block_norm_end(const NormEnd a) {
-    __shared__ float lds[4][4][64];
+__global__ __launch_bounds__(1024) void block_norm_end(const NormEnd a) {
+    __shared__ float lds[2][16][64];
     const int cb = blockIdx.x % a.col_blocks;
     const long long job = blockIdx.x / a.col_blocks;
     const int k = threadIdx.x >> 6, lane = threadIdx.x & 63, col = cb * 64 + lane;
-    const bool in = col < a.c;
-    const bool gates = job > 0;
-    const long long p0 = gates ? (job - 1) * a.parts_per_gate : 0, p1 = gates ? p0 + a.parts_per_gate : a.parts;
-    float s[4] = {};
-    if (in)
-        for (long long p = p0 + k; p < p1; p += 4) {
-            const float* q = a.part + p * 5 * a.c + col;
-            if (gates) s[0] += q[4 * (long long)a.c];
-            else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) s[j] += q[j * (long long)a.c];
-            }
+    if ((job == 0 && !a.post) || (job == 1 && !a.pre)) return;
+    const long long p0 = job > 1 ? (job - 2) * a.parts_per_gate : 0, p1 = job > 1 ? p0 + a.parts_per_gate : a.parts;
+    const int first = job > 1 ? 4 : (int)job * 2;
+    const bool two = job < 2 && a.layer;
+    float s0 = 0, s1 = 0;
+    if (col < a.c) {
+        const float* q = a.part + first * (long long)a.c + col;
+        const long long step = 5 * (long long)a.c;
+#pragma unroll 8
+        for (long long p = p0 + k; p < p1; p += 16) s0 += q[p * step];
+        if (two) {
+#pragma unroll 8
+            for (long long p = p0 + k; p < p1; p += 16) s1 += q[p * step + a.c];
         }
-#pragma unroll
-    for (int j = 0; j < 4; j++) lds[k][j][lane] = s[j];
+    }
+    lds[0][k][lane] = s0;
+    lds[1][k][lane] = s1;
     __syncthreads();
-    if (k || !in) return;
+    if (k || col >= a.c) return;
+    s0 = s1 = 0;
 #pragma unroll
-    for (int j = 0; j < 4; j++) s[j] = (lds[0][j][lane] + lds[1][j][lane]) + (lds[2][j][lane] + lds[3][j][lane]);
+    for (int i = 0; i < 16; i++) { s0 += lds[0][i][lane]; s1 += lds[1][i][lane]; }
     const float sc = a.scale ? (float)((const T*)a.scale)[col] : 1.f;
-    if (gates) {
-        ((T*)a.dgate)[(job - 1) * a.c + col] = (T)(s[0] * sc);
+    if (job > 1) {
+        ((T*)a.dgate)[(job - 2) * a.c + col] = (T)(s0 * sc);
+        return;
+    }
+    if (job == 1) {
+        if (a.dw2) ((T*)a.dw2)[col] = (T)s0;
+        if (a.db2) ((T*)a.db2)[col] = (T)s1;
         return;
     }
     const float w = a.w1 ? (float)((const T*)a.w1)[col] : 1.f, b = a.b1 ? (float)((const T*)a.b1)[col] : 0.f;
-    if (a.dscale) ((T*)a.dscale)[col] = (T)(w * s[0] + b * s[1]);
-    if (a.dw1) ((T*)a.dw1)[col] = (T)(sc * s[0]);
-    if (a.db1) ((T*)a.db1)[col] = (T)(sc * s[1]);
-    if (a.dw2) ((T*)a.dw2)[col] = (T)s[2];
-    if (a.db2) ((T*)a.db2)[col] = (T)s[3];
+    if (a.dscale) ((T*)a.dscale)[col] = (T)(w * s0 + b * s1);
+    if (a.dw1) ((T*)a.dw1)[col] = (T)(sc * s0);
+    if (a.db1) ((T*)a.db1)[col] = (T)(sc * s1);
 }
 
 static_assert(sizeof(aipt_block_norm_args) == 152 && sizeof(aipt_block_norm_grad_args) == 224, "argument records (api.py packs them by field)");
 
 // ---- which kernel: the fewest lanes that hold a row, 16-byte accesses where every row begins at 16 bytes
 struct NormShape { int v, n, lanes; };
-template <int VEC> static NormShape norm_shape(int c, bool wide) {
-    const int v = wide ? VEC : 1;
-    static const struct { int n, lanes; } wides[] = {{1, 64}, {2, 64}, {4, 64}, {2, 256}, {4, 256}, {2, 1024}, {4, 1024}},
-                                          ones[] = {{1, 64}, {2, 64}, {4, 64}, {8, 64}, {4, 256}, {8, 256}, {4, 1024}, {16, 1024}};
-    if (wide) { for (auto& s : wides) if (s.n * s.lanes * v >= c) return {v, s.n, s.lanes}; }
-    else { for (auto& s : ones) if (s.n * s.lanes >= c) return {v, s.n, s.lanes}; }
+template <int S> static NormShape norm_shape(int c, int v, const int (&shapes)[S][2]) {
+    for (auto& s : shapes) if (s[0] * s[1] * v >= c) return {v, s[1], s[0]};
     return {0, 0, 0};
 }
+static NormShape fwd_shape(int es, int c, bool wide) {
+    static const int wides[][2] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}},
+                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}};
+    return wide ? norm_shape(c, 16 / es, wides) : norm_shape(c, 1, ones);
+}
+static NormShape bwd_shape(int es, int c, bool wide, bool whole) {
+    static const int w2[][2] = {{16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}}, w4[][2] = {{16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}},
+                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 8}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}};
+    static const int g2[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 2}}, g4[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 4}}, gones[][2] = {{16, 4}, {64, 8}, {256, 8}, {512, 16}, {1024, 16}};
+    if (whole) return !wide ? norm_shape(c, 1, gones) : es == 2 ? norm_shape(c, 8, g2) : norm_shape(c, 4, g4);
+    return !wide ? norm_shape(c, 1, ones) : es == 2 ? norm_shape(c, 8, w2) : norm_shape(c, 4, w4);
+}
 
-#define AIPT_NORM_KERNELS(NAME, ARGS)                                                              \
-    template <typename T> static void (*NAME##_kernel(NormShape s))(ARGS) {                        \
-        constexpr int V = 16 / sizeof(T);                                                          \
-        if (s.v == V) {                                                                            \
-            if (s.lanes == 64) return s.n == 1 ? NAME<T, V, 1, 64> : s.n == 2 ? NAME<T, V, 2, 64> : NAME<T, V, 4, 64>; \
-            if (s.lanes == 256) return s.n == 2 ? NAME<T, V, 2, 256> : NAME<T, V, 4, 256>;         \
-            return s.n == 2 ? NAME<T, V, 2, 1024> : NAME<T, V, 4, 1024>;                           \
-        }                                                                                          \
-        if (s.lanes == 64) return s.n == 1 ? NAME<T, 1, 1, 64> : s.n == 2 ? NAME<T, 1, 2, 64> : s.n == 4 ? NAME<T, 1, 4, 64> : NAME<T, 1, 8, 64>; \
-        if (s.lanes == 256) return s.n == 4 ? NAME<T, 1, 4, 256> : NAME<T, 1, 8, 256>;             \
-        return s.n == 4 ? NAME<T, 1, 4, 1024> : NAME<T, 1, 16, 1024>;                              \
-    }
-AIPT_NORM_KERNELS(block_norm_fwd, NormFwd)
-AIPT_NORM_KERNELS(block_norm_bwd, NormBwd)
+template <typename T> static void (*fwd_kernel(NormShape s))(NormFwd) {
+    constexpr int V = 16 / sizeof(T);
+#define AIPT_FWD(VV, NN, LL) if (s.v == VV && s.n == NN && s.lanes == LL) return block_norm_fwd<T, VV, NN, LL>;
+    AIPT_FWD(V, 1, 16) AIPT_FWD(V, 2, 16) AIPT_FWD(V, 1, 64) AIPT_FWD(V, 2, 64) AIPT_FWD(V, 4, 64) AIPT_FWD(V, 2, 256) AIPT_FWD(V, 4, 256) AIPT_FWD(V, 2, 1024)
+    if constexpr (V == 4) { AIPT_FWD(V, 4, 1024) }
+    AIPT_FWD(1, 2, 16) AIPT_FWD(1, 4, 16) AIPT_FWD(1, 8, 16) AIPT_FWD(1, 4, 64) AIPT_FWD(1, 8, 64) AIPT_FWD(1, 4, 256) AIPT_FWD(1, 8, 256) AIPT_FWD(1, 8, 512) AIPT_FWD(1, 16, 512)
+    return block_norm_fwd<T, 1, 16, 1024>;
+#undef AIPT_FWD
+}
+template <typename T, bool LAYER> static void (*bwd_kernel(NormShape s, bool whole))(NormBwd) {
+    constexpr int V = 16 / sizeof(T);
+#define AIPT_BWD(VV, NN, LL, GG) if (s.v == VV && s.n == NN && s.lanes == LL && whole == GG) return block_norm_bwd<T, VV, NN, LL, LAYER, GG>;
+    AIPT_BWD(V, 1, 16, false) AIPT_BWD(V, 2, 16, false) AIPT_BWD(V, 2, 64, false) AIPT_BWD(V, 1, 256, false) AIPT_BWD(V, 2, 256, false)
+    if constexpr (V == 8) { AIPT_BWD(V, 2, 512, false) AIPT_BWD(V, 2, 1024, false) AIPT_BWD(V, 2, 1024, true) }
+    else { AIPT_BWD(V, 4, 256, false) AIPT_BWD(V, 4, 512, false) AIPT_BWD(V, 4, 1024, false) AIPT_BWD(V, 4, 1024, true) }
+    AIPT_BWD(V, 1, 16, true) AIPT_BWD(V, 2, 64, true) AIPT_BWD(V, 2, 256, true)
+    AIPT_BWD(1, 2, 16, false) AIPT_BWD(1, 4, 16, false) AIPT_BWD(1, 8, 16, false) AIPT_BWD(1, 8, 64, false) AIPT_BWD(1, 8, 256, false) AIPT_BWD(1, 8, 512, false) AIPT_BWD(1, 16, 512, false) AIPT_BWD(1, 16, 1024, false)
+    AIPT_BWD(1, 4, 16, true) AIPT_BWD(1, 8, 64, true) AIPT_BWD(1, 8, 256, true) AIPT_BWD(1, 16, 512, true)
+    return block_norm_bwd<T, 1, 16, 1024, LAYER, true>;
+#undef AIPT_BWD
+}
 
-// parts of the backward pass: enough for every CU to hold several, none shorter than 4 rows where there are rows enough
+// Parts of the backward pass (a workgroup each): 1 024 of 256 threads, 256 of 1 024, none shorter than 4 rows for each row handled at a time.  Gates
+// fewer than that are split into parts; more, and a part takes whole gates.
 struct NormParts { long long parts, span, per_gate_parts; };
+static bool norm_whole(long long groups) { return groups >= 512; }
 static NormParts norm_parts(long long rows, long long groups, int lanes) {
-    const long long want = lanes == 64 ? 4096 : lanes == 256 ? 1024 : 256;
+    const long long want = lanes <= 64 ? 1024 : lanes == 256 ? 512 : 256, at_once = lanes < 256 ? 256 / lanes : 1;
     const long long per = std::max(1ll, rows / groups);
     NormParts p;
-    if (groups >= want) {                                    // whole gates
-        const long long gates = (groups + want - 1) / want;
-        p.span = gates * per;
-        p.parts = (groups + gates - 1) / gates;
+    if (norm_whole(groups)) {
+        p.span = std::max(at_once, (groups + want - 1) / want);
+        p.parts = (groups + p.span - 1) / p.span;
         p.per_gate_parts = 0;
     } else {
-        long long k = std::max(1ll, std::min(want / groups, (per + 3) / 4));
+        long long k = std::max(1ll, std::min(want / groups, per / (4 * at_once)));
         p.span = (per + k - 1) / k;
         k = (per + p.span - 1) / p.span;
         p.parts = k * groups;
@@ -456,13 +603,13 @@ int aipt_block_norm(aipt_ctx* ctx, const aipt_block_norm_args* a) {
     const int vec = 16 / es;
     const bool wide = a->c % vec == 0 && on16({a->x, a->y, a->h, a->z, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->pre_bias}) &&
                       (a->rows == 1 || (!(a->x_stride % vec) && !(a->h_stride % vec) && !(a->y && a->y_stride % vec) && !(a->z && a->z_stride % vec)));
-    const aipt::NormShape s = vec == 4 ? aipt::norm_shape<4>(a->c, wide) : aipt::norm_shape<8>(a->c, wide);
+    const aipt::NormShape s = aipt::fwd_shape(es, a->c, wide);
     const aipt::NormFwd f = {a->x, a->y, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->pre_bias, a->h, a->z, a->stats,
                              a->rows, a->rows / (a->gate ? a->groups : 1), a->x_stride, a->y_stride, a->h_stride, a->z_stride, a->c, a->kind == AIPT_NORM_LAYER, a->eps};
     const int threads = std::max(256, s.lanes), per = threads / s.lanes;
     const long long want = (a->rows + per - 1) / per;
     const size_t blocks = (size_t)std::min(want, 1ll << 20);
-    auto* k = a->type == AIPT_TYPE_F32 ? aipt::block_norm_fwd_kernel<float>(s) : a->type == AIPT_TYPE_BF16 ? aipt::block_norm_fwd_kernel<aipt::bf16>(s) : aipt::block_norm_fwd_kernel<aipt::f16>(s);
+    auto* k = a->type == AIPT_TYPE_F32 ? aipt::fwd_kernel<float>(s) : a->type == AIPT_TYPE_BF16 ? aipt::fwd_kernel<aipt::bf16>(s) : aipt::fwd_kernel<aipt::f16>(s);
     AIPT_NEED_CTX(ctx);
     aipt::DeviceScope dev(ctx->device);
     AIPT_HIP(ctx, dev.err);
@@ -490,12 +637,12 @@ int aipt_block_norm_backward_workspace(aipt_ctx* ctx, const aipt_block_norm_grad
     if (!bytes) return fail(ctx, AIPT_E_INVALID, "%s: bytes is NULL", me);
     const int rc = norm_grad_check(ctx, me, a);
     if (rc) return rc;
+    const long long groups = norm_gated(a) ? a->groups : 1;
     size_t most = 0;
     for (bool wide : {false, true}) {
-        const aipt::NormShape s = aipt::type_bytes(a->type) == 4 ? aipt::norm_shape<4>(a->c, wide) : aipt::norm_shape<8>(a->c, wide);
-        const int per = std::max(256, s.lanes) / s.lanes;
-        const aipt::NormParts p = aipt::norm_parts(std::max(1ll, a->rows), norm_gated(a) ? a->groups : 1, s.lanes);
-        most = std::max(most, (size_t)((p.parts + per - 1) / per * per) * 5 * a->c * sizeof(float));
+        const aipt::NormShape s = aipt::bwd_shape(aipt::type_bytes(a->type), a->c, wide, aipt::norm_whole(groups));
+        const aipt::NormParts p = aipt::norm_parts(std::max(1ll, a->rows), groups, s.lanes);
+        most = std::max(most, (size_t)p.parts * 5 * a->c * sizeof(float));
     }
     *bytes = most;
     return AIPT_OK;
@@ -550,18 +697,21 @@ int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* a, 
         for (long long s : strides) wide = wide && !(s % vec);
         wide = wide && !(a->dx && a->dx_stride % vec) && !(a->dy && a->dy_stride % vec);
     }
-    const aipt::NormShape s = vec == 4 ? aipt::norm_shape<4>(a->c, wide) : aipt::norm_shape<8>(a->c, wide);
-    const int threads = std::max(256, s.lanes), per = threads / s.lanes;
     const long long groups = norm_gated(a) ? a->groups : 1;
-    aipt::NormParts p = aipt::norm_parts(std::max(1ll, a->rows), groups, s.lanes);
-    const size_t blocks = (size_t)((p.parts + per - 1) / per);
+    const bool whole = aipt::norm_whole(groups);
+    const aipt::NormShape s = aipt::bwd_shape(es, a->c, wide, whole);
+    const int threads = std::max(256, s.lanes);
+    const aipt::NormParts p = aipt::norm_parts(a->rows, groups, s.lanes);
+    const size_t blocks = (size_t)p.parts;
     const bool part = sums || (a->dgate && p.per_gate_parts);
-    const size_t need = part ? blocks * per * 5 * a->c * sizeof(float) : 0;
+    const size_t need = part ? blocks * 5 * a->c * sizeof(float) : 0;
     if (need && (!d_workspace || workspace_bytes < need)) return fail(ctx, AIPT_E_INVALID, "%s: workspace of %zu bytes, %zu are wanted", me, workspace_bytes, need);
     const aipt::NormBwd b = {a->dh, a->dz, a->y, a->h, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->stats, a->dx, a->dy, a->dgate,
                              part ? (float*)d_workspace : nullptr, a->rows, std::max(1ll, a->rows / groups), a->dh_stride, a->dz_stride, a->y_stride, a->h_stride, a->dx_stride, a->dy_stride,
-                             p.span, p.per_gate_parts, a->c, a->kind == AIPT_NORM_LAYER, sums};
-    auto* k = a->type == AIPT_TYPE_F32 ? aipt::block_norm_bwd_kernel<float>(s) : a->type == AIPT_TYPE_BF16 ? aipt::block_norm_bwd_kernel<aipt::bf16>(s) : aipt::block_norm_bwd_kernel<aipt::f16>(s);
+                             p.span, p.per_gate_parts, a->c};
+    const bool layer = a->kind == AIPT_NORM_LAYER;
+    auto pick = [&](auto t) { return layer ? aipt::bwd_kernel<decltype(t), true>(s, whole) : aipt::bwd_kernel<decltype(t), false>(s, whole); };
+    auto* k = a->type == AIPT_TYPE_F32 ? pick(0.f) : a->type == AIPT_TYPE_BF16 ? pick((aipt::bf16)0.f) : pick((aipt::f16)0.f);
     if (!aipt::grid_fits(blocks, threads)) return fail(ctx, AIPT_E_INVALID, "%s: %lld rows of %lld groups are too many", me, a->rows, a->groups);
     AIPT_NEED_CTX(ctx);
     aipt::DeviceScope dev(ctx->device);
@@ -571,10 +721,10 @@ int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* a, 
         const int cb = (a->c + 63) / 64;
         const bool gates = a->dgate && p.per_gate_parts;
         const aipt::NormEnd e = {(const float*)d_workspace, a->scale, a->post_weight, a->post_bias, a->dgate, a->dscale, a->dpost_weight, a->dpost_bias, a->dpre_weight, a->dpre_bias,
-                                 sums ? p.parts : 0, p.per_gate_parts, a->c, cb};
-        const size_t jobs = 1 + (gates ? (size_t)a->groups : 0);
+                                 p.parts, p.per_gate_parts, a->c, cb, layer, a->dscale || a->dpost_weight || a->dpost_bias, a->dpre_weight || a->dpre_bias};
+        const size_t jobs = 2 + (gates ? (size_t)a->groups : 0);
         auto* ke = a->type == AIPT_TYPE_F32 ? aipt::block_norm_end<float> : a->type == AIPT_TYPE_BF16 ? aipt::block_norm_end<aipt::bf16> : aipt::block_norm_end<aipt::f16>;
-        AIPT_HIP(ctx, aipt::launch(ke, jobs * cb, 256, 0, ctx->stream, e));
+        AIPT_HIP(ctx, aipt::launch(ke, jobs * cb, 1024, 0, ctx->stream, e));
     }
     return AIPT_OK;
 }

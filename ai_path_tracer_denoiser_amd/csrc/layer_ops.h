@@ -65,16 +65,31 @@ inline bool overlap(const Extent& a, const Extent& b) {
     return true;
 }
 
-// sum over the 64 lanes of a wave, the same value in each; always the same order
+// Sums over 16 neighbouring lanes (rotations within a row of 16, which the vector unit does itself) and over the 64 of a wave: the same value in
+// each lane, always added in the same order.
+template <int N> __device__ inline float rotate16(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true));
+}
+__device__ inline float sum16(float v) {
+    v += rotate16<8>(v);
+    v += rotate16<4>(v);
+    v += rotate16<2>(v);
+    v += rotate16<1>(v);
+    return v;
+}
 __device__ inline float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    v = sum16(v);
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
     return v;
 }
 __device__ inline float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    v = fmaxf(v, rotate16<8>(v));
+    v = fmaxf(v, rotate16<4>(v));
+    v = fmaxf(v, rotate16<2>(v));
+    v = fmaxf(v, rotate16<1>(v));
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
 }
 
 }  // namespace aipt
