@@ -2,9 +2,9 @@
 //
 // What it cannot do without: p in and out, the gradient, the state in and out -- 28 bytes a parameter with fp32 state and gradients,
 // 14 with 8-bit state and bf16 gradients -- and some 40 operations on them: memory bounds it, and for small sets the launch.  So: ONE
-// launch over all tensors (their pointers travel in the kernel arguments, up to TENSORS of them, which a captured graph keeps by
-// itself), a wave per 256-element block (16-byte accesses, and the block's scale is a wave's own maximum), and the step number on the
-// device, advanced by the last workgroup, so that neither the host nor a second launch has a part in it.
+// launch over all tensors, a wave per 256-element block (16-byte accesses, and the block's scale is a wave's own maximum), and the step
+// number on the device, advanced by the last workgroup, so that neither the host nor a second launch has a part in it.  The table of tensors
+// lies in device memory, read by scalar loads: the kernel arguments of a launch hold a hundred at most.
 #include "layer_ops.h"
 
 #include <cmath>
@@ -13,7 +13,6 @@
 namespace aipt {
 
 constexpr int BLOCK = 256;           // elements that share a scale; what one wave handles at a time
-constexpr int TENSORS = 112;         // of one launch: 112 x 33 bytes + the scalars stay below 4 KB of kernel arguments
 constexpr int GRID = 2048;           // most workgroups of a launch: 8 a CU; the blocks beyond 4 a workgroup go round
 constexpr size_t SCRATCH = 256;      // bytes of the workspace before the partial sums
 constexpr float TOP = 448.f;         // largest e4m3
@@ -23,32 +22,29 @@ struct AdamTensor {
     float* p;
     const void* g;
     void* copy;
-    unsigned first;                  // its first block in the launch's numbering
+    long long count;
+    unsigned first;                  // its first block
     float decay;
 };
 
-struct AdamTable {
-    AdamTensor t[TENSORS];
-    unsigned char tail[TENSORS];     // elements of its last block, less one
-    int n;
-    unsigned blocks;                 // of this launch
-};
+// The table is written once, before any launch that reads it, and never by a kernel: constant memory to the compiler, so that a wave's look-ups are scalar.
+typedef const __attribute__((address_space(4))) AdamTensor* AdamTable;
 
 struct AdamArgs {
-    AdamTable tab;
-    unsigned long long state0;       // the first block's place among the state's blocks
+    const AdamTensor* tab;
+    int n;
+    unsigned blocks;
     void *m, *v;
     float *ms, *vs;
     int* step;
     const float* clip;               // {norm, factor}, or NULL
-    unsigned* ticket;                // workgroups done; non-NULL on the step's last launch: advances `step`
-    double b1, b2;                   // the powers are taken of the betas as given ...
+    unsigned* ticket;                // workgroups done: the last one advances `step`
+    double ln1, ln2;                 // logarithms of the betas
     float lr, beta1, beta2, eps;
-    float omb1, omb2;                // ... and 1 - beta is rounded once: 1 - 0.999f is 5e-5 off 0.001
+    float omb1, omb2;                // 1 - beta, rounded once: 1 - 0.999f is 5e-5 off 0.001
     unsigned seed;
     int pad;
 };
-static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
 template <typename G> __device__ inline void load4(const G* g, float* o);
 template <> __device__ inline void load4<float>(const float* g, float* o) {
@@ -97,20 +93,23 @@ __device__ inline float chance_e4m3(float x, float u) {
 
 // Where block b lies: `ti` its tensor (blocks only grow, so a wave's search goes on from its last one's), `at` the lane's first element,
 // the return value how many of the lane's four exist (<= 0: none).
-__device__ inline int locate(const AdamTable& tab, unsigned b, int lane, int& ti, long long& at) {
-    int hi = tab.n;
+__device__ inline int locate(AdamTable tab, int n, unsigned b, int lane, int& ti, long long& at) {
+    int hi = n;
     while (hi - ti > 1) {
         const int mid = (ti + hi) >> 1;
-        if (tab.t[mid].first <= b) ti = mid; else hi = mid;
+        if (tab[mid].first <= b) ti = mid; else hi = mid;
     }
-    const unsigned next = ti + 1 < tab.n ? tab.t[ti + 1].first : tab.blocks;
-    at = (long long)(b - tab.t[ti].first) * BLOCK + lane * 4;
-    return (b + 1 == next ? (int)tab.tail[ti] + 1 : BLOCK) - lane * 4;
+    at = (long long)(b - tab[ti].first) * BLOCK + lane * 4;
+    const long long left = tab[ti].count - at;
+    return left > 4 ? 4 : (int)left;
 }
 
+// two blocks of a wave at a time: the second one's loads are under way while the first is worked on
 template <typename G, typename C, int BITS>
 __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
+    constexpr int U = 2;
     __shared__ float bias[2];
+    const AdamTable tab = (AdamTable)(uintptr_t)a.tab;
     float factor = 1.f;
     bool skip = false;
     if (a.clip) {
@@ -118,10 +117,7 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
         skip = !(a.clip[0] <= 3.4028235e38f);                              // inf and NaN
     }
     const int step = *a.step + 1;
-    if (threadIdx.x < 2) {                                                 // 1 - beta^t without the cancellation, in fp64
-        const double b = threadIdx.x ? a.b2 : a.b1;
-        bias[threadIdx.x] = (float)-expm1((double)step * log(b));
-    }
+    if (threadIdx.x < 2) bias[threadIdx.x] = (float)-expm1((double)step * (threadIdx.x ? a.ln2 : a.ln1));    // 1 - beta^t without the cancellation
     __syncthreads();
     const float rate = a.lr / bias[0], root2 = 1.f / sqrtf(bias[1]);
     const unsigned key = a.seed + (unsigned)step * 0x9E3779B1u;
@@ -129,84 +125,116 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
     const unsigned waves = gridDim.x * 4;
     int ti = 0;
     if (!skip)
-        for (unsigned b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b < a.tab.blocks; b += waves) {
-            long long at;
-            const int left = locate(a.tab, b, lane, ti, at);
-            const AdamTensor& t = a.tab.t[ti];
-            const unsigned long long sb = a.state0 + b, place = sb * BLOCK + lane * 4;
-            const G* gp = (const G*)t.g + at;
-            float* pp = t.p + at;
-            C* cp = t.copy ? (C*)t.copy + at : nullptr;
-            const bool wide = left >= 4 && !(((uintptr_t)t.p & 15) | ((uintptr_t)t.g & (4 * sizeof(G) - 1)) | ((uintptr_t)t.copy & (4 * sizeof(C) - 1)));
-            float p[4] = {}, g[4] = {}, m[4], v[4];
-            if (wide) {
-                load4<float>(pp, p);
-                load4<G>(gp, g);
-            } else {
+        for (unsigned b0 = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b0 < a.blocks; b0 += waves * U) {
+            float p[U][4], g[U][4], m[U][4], v[U][4], ms[U], vs[U], decay[U];
+            unsigned mq[U], vq[U];
+            float* pp[U];
+            C* cp[U];
+            int left[U];
+            bool wide[U];
 #pragma unroll
-                for (int i = 0; i < 4; i++) if (i < left) { p[i] = pp[i]; g[i] = (float)gp[i]; }
-            }
-            if constexpr (BITS == 32) {
-                load4<float>((const float*)a.m + place, m);
-                load4<float>((const float*)a.v + place, v);
-            } else {
-                from_e4m3(((const unsigned*)a.m)[place >> 2], m);
-                from_e4m3(((const unsigned*)a.v)[place >> 2], v);
-                const float ms = a.ms[sb], vs = a.vs[sb];
+            for (int u = 0; u < U; u++) {
+                const unsigned b = b0 + u * waves;
+                left[u] = 0;
+                wide[u] = false;
+                if (b >= a.blocks) continue;
+                long long at;
+                left[u] = locate(tab, a.n, b, lane, ti, at);
+                float* const tp = tab[ti].p;
+                const void* const tg = tab[ti].g;
+                void* const tc = tab[ti].copy;
+                decay[u] = tab[ti].decay;
+                pp[u] = tp + at;
+                cp[u] = tc ? (C*)tc + at : nullptr;
+                const G* gp = (const G*)tg + at;
+                wide[u] = left[u] >= 4 && !(((uintptr_t)tp & 15) | ((uintptr_t)tg & (4 * sizeof(G) - 1)) | ((uintptr_t)tc & (4 * sizeof(C) - 1)));
+                if (wide[u]) {
+                    load4<float>(pp[u], p[u]);
+                    load4<G>(gp, g[u]);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) { m[i] *= ms; v[i] *= vs; v[i] *= v[i]; }
-            }
-            const float keep = 1.f - a.lr * t.decay;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float gi = g[i] * factor;
-                m[i] = m[i] * a.beta1 + gi * a.omb1;
-                v[i] = v[i] * a.beta2 + gi * gi * a.omb2;
-                p[i] = p[i] * keep - rate * m[i] / (sqrtf(v[i]) * root2 + a.eps);
-            }
-            if (wide) {
-                *(float4*)pp = make_float4(p[0], p[1], p[2], p[3]);
-                if (cp) {
-                    struct alignas(4 * sizeof(C)) Q { C v[4]; } q;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) q.v[i] = (C)p[i];
-                    *(Q*)cp = q;
+                    for (int i = 0; i < 4; i++) { p[u][i] = i < left[u] ? pp[u][i] : 0.f; g[u][i] = i < left[u] ? (float)gp[i] : 0.f; }
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) if (i < left) { pp[i] = p[i]; if (cp) cp[i] = (C)p[i]; }
+                const unsigned long long place = (unsigned long long)b * BLOCK + lane * 4;
+                if constexpr (BITS == 32) {
+                    load4<float>((const float*)a.m + place, m[u]);
+                    load4<float>((const float*)a.v + place, v[u]);
+                } else {
+                    mq[u] = ((const unsigned*)a.m)[place >> 2];
+                    vq[u] = ((const unsigned*)a.v)[place >> 2];
+                    ms[u] = a.ms[b];
+                    vs[u] = a.vs[b];
+                }
             }
-            if constexpr (BITS == 32) {
-                *(float4*)((float*)a.m + place) = make_float4(m[0], m[1], m[2], m[3]);
-                *(float4*)((float*)a.v + place) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-                float mt = 0, vt = 0;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const unsigned b = b0 + u * waves;
+                if (b >= a.blocks) break;
+                const unsigned long long place = (unsigned long long)b * BLOCK + lane * 4;
+                if constexpr (BITS == 8) {
+                    from_e4m3(mq[u], m[u]);
+                    from_e4m3(vq[u], v[u]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) { m[u][i] *= ms[u]; v[u][i] *= vs[u]; v[u][i] *= v[u][i]; }
+                }
+                const float keep = 1.f - a.lr * decay[u];
+                float r[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if (i >= left) { m[i] = 0; v[i] = 0; }                 // the padding stays zero whatever was in it
-                    v[i] = sqrtf(v[i]);
-                    mt = fmaxf(mt, fabsf(m[i])); vt = fmaxf(vt, v[i]);
+                    const float gi = g[u][i] * factor;
+                    m[u][i] = m[u][i] * a.beta1 + gi * a.omb1;
+                    v[u][i] = v[u][i] * a.beta2 + gi * gi * a.omb2;
+                    // the chip's root and reciprocal, an ulp each: the step is within 6 ulp of itself, far below the parameter's own
+                    r[i] = __builtin_amdgcn_sqrtf(v[u][i]);
+                    p[u][i] = p[u][i] * keep - rate * m[u][i] * __builtin_amdgcn_rcpf(r[i] * root2 + a.eps);
                 }
-                mt = wave_max(mt); vt = wave_max(vt);
-                const float mi = mt >= LIVE ? TOP / mt : 0.f, vi = vt >= LIVE ? TOP / vt : 0.f;
+                if (wide[u]) {
+                    *(float4*)pp[u] = make_float4(p[u][0], p[u][1], p[u][2], p[u][3]);
+                    if (cp[u]) {
+                        struct alignas(4 * sizeof(C)) Q { C v[4]; } q;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    m[i] = fminf(fmaxf(m[i] * mi, -TOP), TOP);
-                    const float c = chance_e4m3(v[i] * vi, uniform(place + i, key));
-                    v[i] = c == 0.f && v[i] > 0.f && vi > 0.f ? 0x1p-9f : c;
+                        for (int i = 0; i < 4; i++) q.v[i] = (C)p[u][i];
+                        *(Q*)cp[u] = q;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) if (i < left[u]) { pp[u][i] = p[u][i]; if (cp[u]) cp[u][i] = (C)p[u][i]; }
                 }
-                ((unsigned*)a.m)[place >> 2] = to_e4m3(m);
-                ((unsigned*)a.v)[place >> 2] = to_e4m3(v);
-                if (lane == 0) {
-                    a.ms[sb] = mt >= LIVE ? mt / TOP : 0.f;
-                    a.vs[sb] = vt >= LIVE ? vt / TOP : 0.f;
+                if constexpr (BITS == 32) {
+                    if (left[u] < 4) {                                     // the padding stays as it is: zero
+#pragma unroll
+                        for (int i = 0; i < 4; i++) if (i >= left[u]) m[u][i] = v[u][i] = 0;
+                    }
+                    *(float4*)((float*)a.m + place) = make_float4(m[u][0], m[u][1], m[u][2], m[u][3]);
+                    *(float4*)((float*)a.v + place) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+                } else {
+                    float mt = 0, vt = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (i >= left[u]) m[u][i] = r[i] = 0;
+                        mt = fmaxf(mt, fabsf(m[u][i])); vt = fmaxf(vt, r[i]);
+                    }
+                    mt = wave_max(mt); vt = wave_max(vt);
+                    const float mi = mt >= LIVE ? TOP / mt : 0.f, vi = vt >= LIVE ? TOP / vt : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        m[u][i] = fminf(fmaxf(m[u][i] * mi, -TOP), TOP);
+                        const float c = chance_e4m3(r[i] * vi, uniform(place + i, key));
+                        v[u][i] = c == 0.f && r[i] > 0.f && vi > 0.f ? 0x1p-9f : c;
+                    }
+                    ((unsigned*)a.m)[place >> 2] = to_e4m3(m[u]);
+                    ((unsigned*)a.v)[place >> 2] = to_e4m3(v[u]);
+                    if (lane == 0) {
+                        a.ms[b] = mt >= LIVE ? mt / TOP : 0.f;
+                        a.vs[b] = vt >= LIVE ? vt / TOP : 0.f;
+                    }
                 }
             }
         }
-    // the last workgroup of the step's last launch advances the step number: every workgroup has read it before it takes its ticket
-    if (a.ticket && threadIdx.x == 0) {
-        __threadfence();
-        if (atomicAdd(a.ticket, 1u) == gridDim.x - 1) {
+    // The last workgroup advances the step number: every workgroup has read it (and waited for what it read) before it takes its ticket.  Nothing is
+    // handed from one to another, so there is no fence: a release writes the L2s back, workgroup by workgroup (50 us here).
+    if (threadIdx.x == 0) {
+        if (__hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
             *a.ticket = 0;
             if (!skip) *a.step = step;
         }
@@ -216,22 +244,25 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
 // ---- the norm of all gradients: partial sums of squares in fixed places, then one workgroup.  It reads the gradients once more than the
 // step itself would, and there is no way round it: no parameter may change before the last gradient has been seen.
 struct NormArgs {
-    AdamTable tab;
+    const AdamTensor* tab;
+    int n;
+    unsigned blocks;
     float* partial;                  // one for each workgroup
 };
 template <typename G>
 __global__ __launch_bounds__(256) void grad_square(const NormArgs a) {
+    const AdamTable tab = (AdamTable)(uintptr_t)a.tab;
     const int lane = threadIdx.x & 63;
     const unsigned waves = gridDim.x * 4;
     int ti = 0;
     float s = 0;
-    for (unsigned b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b < a.tab.blocks; b += waves) {
+    for (unsigned b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b < a.blocks; b += waves) {
         long long at;
-        const int left = locate(a.tab, b, lane, ti, at);
-        const AdamTensor& t = a.tab.t[ti];
-        const G* gp = (const G*)t.g + at;
+        const int left = locate(tab, a.n, b, lane, ti, at);
+        const void* const tg = tab[ti].g;
+        const G* gp = (const G*)tg + at;
         float g[4] = {};
-        if (left >= 4 && !((uintptr_t)t.g & (4 * sizeof(G) - 1))) load4<G>(gp, g);
+        if (left >= 4 && !((uintptr_t)tg & (4 * sizeof(G) - 1))) load4<G>(gp, g);
         else {
 #pragma unroll
             for (int i = 0; i < 4; i++) if (i < left) g[i] = (float)gp[i];
@@ -277,14 +308,9 @@ static_assert(sizeof(aipt_adamw_tensor) == 40, "argument record (api.py packs it
 struct aipt_adamw {
     aipt_ctx* ctx = nullptr;
     int grad_type = 0, copy_type = 0, bits = 0;
-    std::vector<aipt::AdamArgs> launches;
-    std::vector<unsigned> grids, norm_grids;
-    long long blocks = 0;
-    unsigned* ticket = nullptr;      // the caller's workspace: ticket, clip[2] at 64, partial sums at SCRATCH
-    float* clip = nullptr;
-    float* partial = nullptr;
-    int npartial = 0;
-    float* norm = nullptr;
+    aipt::AdamArgs args = {};
+    unsigned grid = 0;
+    float *clip = nullptr, *partial = nullptr, *norm = nullptr;      // the first two in the caller's workspace
 };
 
 namespace aipt {
@@ -314,10 +340,7 @@ long long aipt_adamw_state_elements(const long long* counts, int n) {
 
 long long aipt_adamw_workspace(const long long* counts, int n) {
     if (aipt_adamw_state_elements(counts, n) < 0) return AIPT_E_INVALID;
-    // a partial sum for each workgroup of each launch; a launch ends with TENSORS tensors or where the next would not fit its block count
-    const size_t blocks = (size_t)aipt_adamw_state_elements(counts, n) / aipt::BLOCK;
-    const size_t launches = 1 + (size_t)n / aipt::TENSORS + 2 * (blocks / 0xf0000000ull);
-    return (long long)(aipt::SCRATCH + launches * aipt::GRID * sizeof(float));
+    return (long long)(aipt::SCRATCH + aipt::GRID * sizeof(float) + (size_t)n * sizeof(aipt::AdamTensor));
 }
 
 int aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, int grad_type, int copy_type, int state_bits,
@@ -375,48 +398,41 @@ int aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, in
             return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
         }
     }
+    if (blocks > 0xffffff00ll) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: %lld blocks of 256 elements are too many", blocks);
+    const size_t need = aipt::SCRATCH + aipt::GRID * sizeof(float) + (size_t)n * sizeof(aipt::AdamTensor);
+    if (workspace_bytes < need) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: workspace of %zu bytes, %zu are wanted", workspace_bytes, need);
     AIPT_NEED_CTX(ctx);
-    aipt_adamw* a = new (std::nothrow) aipt_adamw();
-    if (!a) return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
-    a->ctx = ctx; a->grad_type = grad_type; a->copy_type = copy_type; a->bits = state_bits; a->blocks = blocks; a->norm = norm;
+    std::vector<aipt::AdamTensor> tab;
+    aipt_adamw* a = nullptr;
     try {
-        unsigned long long state0 = 0;
-        for (int i = 0; i < n;) {
-            aipt::AdamArgs l = {};
-            l.state0 = state0; l.m = m; l.v = v; l.ms = m_scale; l.vs = v_scale; l.step = step;
-            unsigned long long nb = 0;
-            for (; i < n && l.tab.n < aipt::TENSORS; i++) {
-                const aipt_adamw_tensor& t = tensors[i];
-                const unsigned long long tb = (unsigned long long)((t.count + aipt::BLOCK - 1) / aipt::BLOCK);
-                if (!tb) continue;
-                if (nb + tb > 0xf0000000ull) {
-                    if (l.tab.n) break;                                        // its own launch
-                    delete a;
-                    return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: tensor %d has %lld elements", i, t.count);
-                }
-                l.tab.tail[l.tab.n] = (unsigned char)((t.count - 1) % aipt::BLOCK);
-                l.tab.t[l.tab.n++] = {t.param, t.grad, t.copy, (unsigned)nb, t.weight_decay};
-                nb += tb;
-            }
-            if (!l.tab.n) break;
-            l.tab.blocks = (unsigned)nb;
-            state0 += nb;
-            a->launches.push_back(l);
-            a->grids.push_back((unsigned)std::min<unsigned long long>((nb + 3) / 4, aipt::GRID));
+        unsigned first = 0;
+        for (int i = 0; i < n; i++) {
+            const aipt_adamw_tensor& t = tensors[i];
+            if (!t.count) continue;
+            tab.push_back({t.param, t.grad, t.copy, t.count, first, t.weight_decay});
+            first += (unsigned)((t.count + aipt::BLOCK - 1) / aipt::BLOCK);
         }
-        for (unsigned g : a->grids) a->npartial += (int)g;
+        a = new aipt_adamw();
     } catch (const std::bad_alloc&) {
-        delete a;
         return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
     }
-    const size_t need = aipt::SCRATCH + sizeof(float) * (size_t)a->npartial;
-    if (workspace_bytes < need) {
-        delete a;
-        return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: workspace of %zu bytes, %zu are wanted", workspace_bytes, need);
-    }
-    a->ticket = (unsigned*)d_workspace;
+    a->ctx = ctx; a->grad_type = grad_type; a->copy_type = copy_type; a->bits = state_bits; a->norm = norm;
     a->clip = (float*)d_workspace + 16;
     a->partial = (float*)((char*)d_workspace + aipt::SCRATCH);
+    aipt::AdamTensor* d_tab = (aipt::AdamTensor*)(a->partial + aipt::GRID);
+    a->args.tab = d_tab; a->args.n = (int)tab.size(); a->args.blocks = (unsigned)blocks;
+    a->args.m = m; a->args.v = v; a->args.ms = m_scale; a->args.vs = v_scale; a->args.step = step; a->args.ticket = (unsigned*)d_workspace;
+    a->grid = (unsigned)std::min<long long>((blocks + 3) / 4, aipt::GRID);
+    if (!tab.empty()) {
+        aipt::DeviceScope dev(ctx->device);
+        hipError_t e = dev.err;
+        if (e == hipSuccess) e = hipMemcpyAsync(d_tab, tab.data(), tab.size() * sizeof(tab[0]), hipMemcpyHostToDevice, ctx->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+        if (e != hipSuccess) {
+            delete a;
+            return fail(ctx, AIPT_E_HIP, "aipt_adamw_create: the table's upload: %s", hipGetErrorString(e));
+        }
+    }
     *out = a;
     return AIPT_OK;
 }
@@ -425,34 +441,25 @@ int aipt_adamw_step(aipt_ctx* ctx, aipt_adamw* a, double lr, double beta1, doubl
     if (!a || a->ctx != ctx) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_step: no plan of this context");
     if (!std::isfinite(lr) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !std::isfinite(eps) || std::isnan(max_norm))
         return fail(ctx, AIPT_E_INVALID, "aipt_adamw_step: lr %g, beta1 %g, beta2 %g, eps %g, max_norm %g", lr, beta1, beta2, eps, max_norm);
-    if (a->launches.empty()) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_step: the plan holds no elements");
-    AIPT_NEED_CTX(ctx);
+    if (!a->grid) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_step: the plan holds no elements");
     aipt::DeviceScope dev(ctx->device);
     AIPT_HIP(ctx, dev.err);
     const bool clip = max_norm > 0;
-    const size_t nl = a->launches.size();
+    aipt::AdamArgs l = a->args;
+    const int t = a->grad_type;
     if (clip) {
-        aipt::NormKernel k = a->grad_type == AIPT_TYPE_F32 ? aipt::grad_square<float> : a->grad_type == AIPT_TYPE_BF16 ? aipt::grad_square<aipt::bf16> : aipt::grad_square<aipt::f16>;
-        float* partial = a->partial;
-        for (size_t i = 0; i < nl; i++) {
-            aipt::NormArgs na;
-            na.tab = a->launches[i].tab; na.partial = partial;
-            AIPT_HIP(ctx, aipt::launch(k, a->grids[i], 256, 0, ctx->stream, na));
-            partial += a->grids[i];
-        }
-        AIPT_HIP(ctx, aipt::launch(aipt::grad_norm_end, 1, 256, 0, ctx->stream, aipt::NormEndArgs{a->partial, a->npartial, (float)max_norm, a->clip, a->norm}));
+        aipt::NormKernel k = t == AIPT_TYPE_F32 ? aipt::grad_square<float> : t == AIPT_TYPE_BF16 ? aipt::grad_square<aipt::bf16> : aipt::grad_square<aipt::f16>;
+        AIPT_HIP(ctx, aipt::launch(k, a->grid, 256, 0, ctx->stream, aipt::NormArgs{l.tab, l.n, l.blocks, a->partial}));
+        AIPT_HIP(ctx, aipt::launch(aipt::grad_norm_end, 1, 256, 0, ctx->stream, aipt::NormEndArgs{a->partial, (int)a->grid, (float)max_norm, a->clip, a->norm}));
+        l.clip = a->clip;
     }
-    aipt::AdamKernel k = a->grad_type == AIPT_TYPE_F32 ? aipt::adam_of<float>(a->copy_type, a->bits) : a->grad_type == AIPT_TYPE_BF16 ? aipt::adam_of<aipt::bf16>(a->copy_type, a->bits)
-                                                                                                   : aipt::adam_of<aipt::f16>(a->copy_type, a->bits);
-    for (size_t i = 0; i < nl; i++) {
-        aipt::AdamArgs l = a->launches[i];
-        l.clip = clip ? a->clip : nullptr;
-        l.ticket = i + 1 == nl ? a->ticket : nullptr;
-        l.b1 = beta1; l.b2 = beta2; l.lr = (float)lr; l.beta1 = (float)beta1; l.beta2 = (float)beta2; l.eps = (float)eps;
-        l.omb1 = (float)(1.0 - beta1); l.omb2 = (float)(1.0 - beta2);
-        l.seed = seed;
-        AIPT_HIP(ctx, aipt::launch(k, a->grids[i], 256, 0, ctx->stream, l));
-    }
+    l.ln1 = std::log(beta1); l.ln2 = std::log(beta2);
+    l.lr = (float)lr; l.beta1 = (float)beta1; l.beta2 = (float)beta2; l.eps = (float)eps;
+    l.omb1 = (float)(1.0 - beta1); l.omb2 = (float)(1.0 - beta2);
+    l.seed = seed;
+    aipt::AdamKernel k = t == AIPT_TYPE_F32 ? aipt::adam_of<float>(a->copy_type, a->bits) : t == AIPT_TYPE_BF16 ? aipt::adam_of<aipt::bf16>(a->copy_type, a->bits)
+                                                                                               : aipt::adam_of<aipt::f16>(a->copy_type, a->bits);
+    AIPT_HIP(ctx, aipt::launch(k, a->grid, 256, 0, ctx->stream, l));
     return AIPT_OK;
 }
 

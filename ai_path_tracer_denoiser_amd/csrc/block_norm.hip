@@ -498,13 +498,13 @@ template <int S> static NormShape norm_shape(int c, int v, const int (&shapes)[S
 }
 static NormShape fwd_shape(int es, int c, bool wide) {
     static const int wides[][2] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}},
-                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}};
+                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}};
     return wide ? norm_shape(c, 16 / es, wides) : norm_shape(c, 1, ones);
 }
 static NormShape bwd_shape(int es, int c, bool wide, bool whole) {
     static const int w2[][2] = {{16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}}, w4[][2] = {{16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}},
-                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 8}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}};
-    static const int g2[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 2}}, g4[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 4}}, gones[][2] = {{16, 4}, {64, 8}, {256, 8}, {512, 16}, {1024, 16}};
+                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 8}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}};
+    static const int g2[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 2}}, g4[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 4}}, gones[][2] = {{16, 4}, {64, 8}, {256, 8}, {1024, 8}, {1024, 16}};
     if (whole) return !wide ? norm_shape(c, 1, gones) : es == 2 ? norm_shape(c, 8, g2) : norm_shape(c, 4, g4);
     return !wide ? norm_shape(c, 1, ones) : es == 2 ? norm_shape(c, 8, w2) : norm_shape(c, 4, w4);
 }
@@ -514,7 +514,7 @@ template <typename T> static void (*fwd_kernel(NormShape s))(NormFwd) {
 #define AIPT_FWD(VV, NN, LL) if (s.v == VV && s.n == NN && s.lanes == LL) return block_norm_fwd<T, VV, NN, LL>;
     AIPT_FWD(V, 1, 16) AIPT_FWD(V, 2, 16) AIPT_FWD(V, 1, 64) AIPT_FWD(V, 2, 64) AIPT_FWD(V, 4, 64) AIPT_FWD(V, 2, 256) AIPT_FWD(V, 4, 256) AIPT_FWD(V, 2, 1024)
     if constexpr (V == 4) { AIPT_FWD(V, 4, 1024) }
-    AIPT_FWD(1, 2, 16) AIPT_FWD(1, 4, 16) AIPT_FWD(1, 8, 16) AIPT_FWD(1, 4, 64) AIPT_FWD(1, 8, 64) AIPT_FWD(1, 4, 256) AIPT_FWD(1, 8, 256) AIPT_FWD(1, 8, 512) AIPT_FWD(1, 16, 512)
+    AIPT_FWD(1, 2, 16) AIPT_FWD(1, 4, 16) AIPT_FWD(1, 8, 16) AIPT_FWD(1, 4, 64) AIPT_FWD(1, 8, 64) AIPT_FWD(1, 4, 256) AIPT_FWD(1, 8, 256) AIPT_FWD(1, 8, 512) AIPT_FWD(1, 8, 1024)
     return block_norm_fwd<T, 1, 16, 1024>;
 #undef AIPT_FWD
 }
@@ -525,8 +525,8 @@ template <typename T, bool LAYER> static void (*bwd_kernel(NormShape s, bool who
     if constexpr (V == 8) { AIPT_BWD(V, 2, 512, false) AIPT_BWD(V, 2, 1024, false) AIPT_BWD(V, 2, 1024, true) }
     else { AIPT_BWD(V, 4, 256, false) AIPT_BWD(V, 4, 512, false) AIPT_BWD(V, 4, 1024, false) AIPT_BWD(V, 4, 1024, true) }
     AIPT_BWD(V, 1, 16, true) AIPT_BWD(V, 2, 64, true) AIPT_BWD(V, 2, 256, true)
-    AIPT_BWD(1, 2, 16, false) AIPT_BWD(1, 4, 16, false) AIPT_BWD(1, 8, 16, false) AIPT_BWD(1, 8, 64, false) AIPT_BWD(1, 8, 256, false) AIPT_BWD(1, 8, 512, false) AIPT_BWD(1, 16, 512, false) AIPT_BWD(1, 16, 1024, false)
-    AIPT_BWD(1, 4, 16, true) AIPT_BWD(1, 8, 64, true) AIPT_BWD(1, 8, 256, true) AIPT_BWD(1, 16, 512, true)
+    AIPT_BWD(1, 2, 16, false) AIPT_BWD(1, 4, 16, false) AIPT_BWD(1, 8, 16, false) AIPT_BWD(1, 8, 64, false) AIPT_BWD(1, 8, 256, false) AIPT_BWD(1, 8, 512, false) AIPT_BWD(1, 8, 1024, false) AIPT_BWD(1, 16, 1024, false)
+    AIPT_BWD(1, 4, 16, true) AIPT_BWD(1, 8, 64, true) AIPT_BWD(1, 8, 256, true) AIPT_BWD(1, 8, 1024, true)
     return block_norm_bwd<T, 1, 16, 1024, LAYER, true>;
 #undef AIPT_BWD
 }
