@@ -14,7 +14,8 @@ namespace aipt {
 
 constexpr int BLOCK = 256;           // elements that share a scale; what one wave handles at a time
 constexpr int GRID = 2048;           // most workgroups of a launch: 8 a CU; the blocks beyond 4 a workgroup go round
-constexpr size_t SCRATCH = 256;      // bytes of the workspace before the partial sums
+constexpr int COUNTERS = 32;         // of finished workgroups, a 128-byte line each
+constexpr size_t SCRATCH = (COUNTERS + 1) * 128;             // bytes of the workspace before the partial sums
 constexpr float TOP = 448.f;         // largest e4m3
 constexpr float LIVE = 0x1p-100f;    // blocks below this are kept as zeros (448 / top stays finite)
 
@@ -37,7 +38,10 @@ struct AdamArgs {
     void *m, *v;
     float *ms, *vs;
     int* step;
-    const float* clip;               // {norm, factor}, or NULL
+    const float* partial;            // sums of the gradients' squares to clip by, or NULL
+    float* norm;                     // receives their root
+    int npartial;
+    float max_norm;
     unsigned* ticket;                // workgroups done: the last one advances `step`
     double ln1, ln2;                 // logarithms of the betas
     float lr, beta1, beta2, eps;
@@ -74,21 +78,14 @@ __device__ inline unsigned to_e4m3(const float* o) {
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(o[2], o[3], q, true);
 }
 
-// 24 random bits as a number in [0, 1) from a place and a key: multiplications by odd constants (fractions of the golden ratio and of
-// the roots of 3 and 5) carry low bits up, the shifts bring high ones down
-__device__ inline float uniform(unsigned long long place, unsigned key) {
+// 32 random bits from a place and a key: multiplications by odd constants (fractions of the golden ratio and of the roots of 3 and 5)
+// carry low bits up, the shifts bring high ones down
+__device__ inline unsigned hash(unsigned long long place, unsigned key) {
     unsigned x = (unsigned)(place ^ (place >> 32)) ^ key;
     x *= 0x9E3779B1u; x ^= x >> 15;
     x *= 0xBB67AE85u; x ^= x >> 13;
-    x *= 0x3C6EF373u; x ^= x >> 16;
-    return (float)(x >> 8) * 0x1p-24f;
-}
-
-// x >= 0 to one of the two e4m3 values around it, up with the probability of its distance from the lower one: the mean is x
-__device__ inline float chance_e4m3(float x, float u) {
-    const int e = max((int)(__float_as_uint(x) >> 23) - 127, -6);          // below 2^-6 the steps stay 2^-9
-    const float unit = __uint_as_float((unsigned)(e - 3 + 127) << 23), inv = __uint_as_float((unsigned)(3 - e + 127) << 23);
-    return fminf(floorf(x * inv + u) * unit, TOP);
+    x *= 0x3C6EF373u;
+    return x ^ (x >> 16);
 }
 
 // Where block b lies: `ti` its tensor (blocks only grow, so a wave's search goes on from its last one's), `at` the lane's first element,
@@ -104,144 +101,156 @@ __device__ inline int locate(AdamTable tab, int n, unsigned b, int lane, int& ti
     return left > 4 ? 4 : (int)left;
 }
 
-// two blocks of a wave at a time: the second one's loads are under way while the first is worked on
+// what a wave holds of a block: a lane four elements
+template <typename C, int BITS> struct AdamBlock {
+    float p[4], g[4], m[4], v[4], ms, vs, decay;
+    unsigned mq, vq;
+    float* pp;
+    C* cp;
+    int left;
+    bool wide;
+};
+
+// The next block's loads are under way while one is worked on; the first one's, while the bias and the clipping are worked out.
 template <typename G, typename C, int BITS>
 __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
-    constexpr int U = 2;
-    __shared__ float bias[2];
+    __shared__ double norms[4];
     const AdamTable tab = (AdamTable)(uintptr_t)a.tab;
-    float factor = 1.f;
-    bool skip = false;
-    if (a.clip) {
-        factor = a.clip[1];
-        skip = !(a.clip[0] <= 3.4028235e38f);                              // inf and NaN
-    }
-    const int step = *a.step + 1;
-    if (threadIdx.x < 2) bias[threadIdx.x] = (float)-expm1((double)step * (threadIdx.x ? a.ln2 : a.ln1));    // 1 - beta^t without the cancellation
-    __syncthreads();
-    const float rate = a.lr / bias[0], root2 = 1.f / sqrtf(bias[1]);
-    const unsigned key = a.seed + (unsigned)step * 0x9E3779B1u;
     const int lane = threadIdx.x & 63;
     const unsigned waves = gridDim.x * 4;
     int ti = 0;
-    if (!skip)
-        for (unsigned b0 = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b0 < a.blocks; b0 += waves * U) {
-            float p[U][4], g[U][4], m[U][4], v[U][4], ms[U], vs[U], decay[U];
-            unsigned mq[U], vq[U];
-            float* pp[U];
-            C* cp[U];
-            int left[U];
-            bool wide[U];
+    using Block = AdamBlock<C, BITS>;
+    auto load = [&](unsigned b, Block& q) {
+        long long at;
+        q.left = locate(tab, a.n, b, lane, ti, at);
+        float* const tp = tab[ti].p;
+        const void* const tg = tab[ti].g;
+        void* const tc = tab[ti].copy;
+        q.decay = tab[ti].decay;
+        q.pp = tp + at;
+        q.cp = tc ? (C*)tc + at : nullptr;
+        const G* gp = (const G*)tg + at;
+        q.wide = q.left >= 4 && !(((uintptr_t)tp & 15) | ((uintptr_t)tg & (4 * sizeof(G) - 1)) | ((uintptr_t)tc & (4 * sizeof(C) - 1)));
+        if (q.wide) {
+            load4<float>(q.pp, q.p);
+            load4<G>(gp, q.g);
+        } else {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const unsigned b = b0 + u * waves;
-                left[u] = 0;
-                wide[u] = false;
-                if (b >= a.blocks) continue;
-                long long at;
-                left[u] = locate(tab, a.n, b, lane, ti, at);
-                float* const tp = tab[ti].p;
-                const void* const tg = tab[ti].g;
-                void* const tc = tab[ti].copy;
-                decay[u] = tab[ti].decay;
-                pp[u] = tp + at;
-                cp[u] = tc ? (C*)tc + at : nullptr;
-                const G* gp = (const G*)tg + at;
-                wide[u] = left[u] >= 4 && !(((uintptr_t)tp & 15) | ((uintptr_t)tg & (4 * sizeof(G) - 1)) | ((uintptr_t)tc & (4 * sizeof(C) - 1)));
-                if (wide[u]) {
-                    load4<float>(pp[u], p[u]);
-                    load4<G>(gp, g[u]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) { p[u][i] = i < left[u] ? pp[u][i] : 0.f; g[u][i] = i < left[u] ? (float)gp[i] : 0.f; }
-                }
-                const unsigned long long place = (unsigned long long)b * BLOCK + lane * 4;
-                if constexpr (BITS == 32) {
-                    load4<float>((const float*)a.m + place, m[u]);
-                    load4<float>((const float*)a.v + place, v[u]);
-                } else {
-                    mq[u] = ((const unsigned*)a.m)[place >> 2];
-                    vq[u] = ((const unsigned*)a.v)[place >> 2];
-                    ms[u] = a.ms[b];
-                    vs[u] = a.vs[b];
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const unsigned b = b0 + u * waves;
-                if (b >= a.blocks) break;
-                const unsigned long long place = (unsigned long long)b * BLOCK + lane * 4;
-                if constexpr (BITS == 8) {
-                    from_e4m3(mq[u], m[u]);
-                    from_e4m3(vq[u], v[u]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) { m[u][i] *= ms[u]; v[u][i] *= vs[u]; v[u][i] *= v[u][i]; }
-                }
-                const float keep = 1.f - a.lr * decay[u];
-                float r[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float gi = g[u][i] * factor;
-                    m[u][i] = m[u][i] * a.beta1 + gi * a.omb1;
-                    v[u][i] = v[u][i] * a.beta2 + gi * gi * a.omb2;
-                    // the chip's root and reciprocal, an ulp each: the step is within 6 ulp of itself, far below the parameter's own
-                    r[i] = __builtin_amdgcn_sqrtf(v[u][i]);
-                    p[u][i] = p[u][i] * keep - rate * m[u][i] * __builtin_amdgcn_rcpf(r[i] * root2 + a.eps);
-                }
-                if (wide[u]) {
-                    *(float4*)pp[u] = make_float4(p[u][0], p[u][1], p[u][2], p[u][3]);
-                    if (cp[u]) {
-                        struct alignas(4 * sizeof(C)) Q { C v[4]; } q;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) q.v[i] = (C)p[u][i];
-                        *(Q*)cp[u] = q;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) if (i < left[u]) { pp[u][i] = p[u][i]; if (cp[u]) cp[u][i] = (C)p[u][i]; }
-                }
-                if constexpr (BITS == 32) {
-                    if (left[u] < 4) {                                     // the padding stays as it is: zero
-#pragma unroll
-                        for (int i = 0; i < 4; i++) if (i >= left[u]) m[u][i] = v[u][i] = 0;
-                    }
-                    *(float4*)((float*)a.m + place) = make_float4(m[u][0], m[u][1], m[u][2], m[u][3]);
-                    *(float4*)((float*)a.v + place) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
-                } else {
-                    float mt = 0, vt = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (i >= left[u]) m[u][i] = r[i] = 0;
-                        mt = fmaxf(mt, fabsf(m[u][i])); vt = fmaxf(vt, r[i]);
-                    }
-                    mt = wave_max(mt); vt = wave_max(vt);
-                    const float mi = mt >= LIVE ? TOP / mt : 0.f, vi = vt >= LIVE ? TOP / vt : 0.f;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        m[u][i] = fminf(fmaxf(m[u][i] * mi, -TOP), TOP);
-                        const float c = chance_e4m3(r[i] * vi, uniform(place + i, key));
-                        v[u][i] = c == 0.f && r[i] > 0.f && vi > 0.f ? 0x1p-9f : c;
-                    }
-                    ((unsigned*)a.m)[place >> 2] = to_e4m3(m[u]);
-                    ((unsigned*)a.v)[place >> 2] = to_e4m3(v[u]);
-                    if (lane == 0) {
-                        a.ms[b] = mt >= LIVE ? mt / TOP : 0.f;
-                        a.vs[b] = vt >= LIVE ? vt / TOP : 0.f;
-                    }
-                }
-            }
+            for (int i = 0; i < 4; i++) { q.p[i] = i < q.left ? q.pp[i] : 0.f; q.g[i] = i < q.left ? (float)gp[i] : 0.f; }
         }
-    // The last workgroup advances the step number: every workgroup has read it (and waited for what it read) before it takes its ticket.  Nothing is
-    // handed from one to another, so there is no fence: a release writes the L2s back, workgroup by workgroup (50 us here).
+        const unsigned long long place = (unsigned long long)b * BLOCK + lane * 4;
+        if constexpr (BITS == 32) {
+            load4<float>((const float*)a.m + place, q.m);
+            load4<float>((const float*)a.v + place, q.v);
+        } else {
+            q.mq = ((const unsigned*)a.m)[place >> 2];
+            q.vq = ((const unsigned*)a.v)[place >> 2];
+            q.ms = a.ms[b];
+            q.vs = a.vs[b];
+        }
+    };
+    unsigned b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    Block q;
+    if (b < a.blocks) load(b, q);
+
+    const int step = *a.step + 1;
+    // 1 - beta^t without the cancellation: lane 0 of beta1, lane 1 of beta2
+    const float bias = lane < 2 ? (float)-expm1((double)step * (lane ? a.ln2 : a.ln1)) : 1.f;
+    const float rate = a.lr / __shfl(bias, 0), root2 = 1.f / sqrtf(__shfl(bias, 1));
+    float factor = 1.f;
+    bool skip = false;
+    if (a.partial) {                 // every workgroup adds the partial sums, in the same order: cheaper than a launch of its own
+        double s = 0;
+        for (int i = threadIdx.x; i < a.npartial; i += 256) s += (double)a.partial[i];
+#pragma unroll
+        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+        if (lane == 0) norms[threadIdx.x >> 6] = s;
+        __syncthreads();
+        const float norm = (float)sqrt((norms[0] + norms[1]) + (norms[2] + norms[3]));
+        factor = fminf(1.f, a.max_norm / (norm + 1e-6f));
+        skip = !(norm <= 3.4028235e38f);                                   // inf and NaN
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
+    }
+    const unsigned key = a.seed + (unsigned)step * 0x9E3779B1u;
+    if (!skip)
+        for (; b < a.blocks; b += waves) {
+            Block nq;
+            if (b + waves < a.blocks) load(b + waves, nq);
+            const unsigned long long place = (unsigned long long)b * BLOCK + lane * 4;
+            if constexpr (BITS == 8) {
+                from_e4m3(q.mq, q.m);
+                from_e4m3(q.vq, q.v);
+#pragma unroll
+                for (int i = 0; i < 4; i++) { q.m[i] *= q.ms; q.v[i] *= q.vs; q.v[i] *= q.v[i]; }
+            }
+            const float keep = 1.f - a.lr * q.decay;
+            float r[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float gi = q.g[i] * factor;
+                q.m[i] = q.m[i] * a.beta1 + gi * a.omb1;
+                q.v[i] = q.v[i] * a.beta2 + gi * gi * a.omb2;
+                // the chip's root and reciprocal, an ulp each: the step is within 6 ulp of itself, far below the parameter's own
+                r[i] = __builtin_amdgcn_sqrtf(q.v[i]);
+                q.p[i] = q.p[i] * keep - rate * q.m[i] * __builtin_amdgcn_rcpf(r[i] * root2 + a.eps);
+            }
+            if (q.wide) {
+                *(float4*)q.pp = make_float4(q.p[0], q.p[1], q.p[2], q.p[3]);
+                if (q.cp) {
+                    struct alignas(4 * sizeof(C)) Q { C v[4]; } c;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) c.v[i] = (C)q.p[i];
+                    *(Q*)q.cp = c;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (i < q.left) { q.pp[i] = q.p[i]; if (q.cp) q.cp[i] = (C)q.p[i]; }
+            }
+            if (q.left < 4) {                                              // the padding is zero and stays so
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (i >= q.left) q.m[i] = q.v[i] = r[i] = 0;
+            }
+            if constexpr (BITS == 32) {
+                *(float4*)((float*)a.m + place) = make_float4(q.m[0], q.m[1], q.m[2], q.m[3]);
+                *(float4*)((float*)a.v + place) = make_float4(q.v[0], q.v[1], q.v[2], q.v[3]);
+            } else {
+                const float mt = wave_max(fmaxf(fmaxf(fabsf(q.m[0]), fabsf(q.m[1])), fmaxf(fabsf(q.m[2]), fabsf(q.m[3]))));
+                const float vt = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
+                const float mi = mt >= LIVE ? TOP / mt : 0.f, vi = vt >= LIVE ? TOP / vt : 0.f, least = vt >= LIVE ? 0x1p-9f : 0.f;
+                unsigned vq = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) q.m[i] = fminf(fmaxf(q.m[i] * mi, -TOP), TOP);
+                // up or down by chance is an instruction of the chip's (it adds 20 of the bits below the mantissa's last, subnormals included); what is
+                // not zero begins at the least e4m3, so that it stays so
+#define AIPT_CHANCE(i) vq = __builtin_amdgcn_cvt_sr_fp8_f32(r[i] > 0.f ? fminf(fmaxf(r[i] * vi, least), TOP) : 0.f, hash(place + i, key), vq, i);
+                AIPT_CHANCE(0) AIPT_CHANCE(1) AIPT_CHANCE(2) AIPT_CHANCE(3)
+#undef AIPT_CHANCE
+                ((unsigned*)a.m)[place >> 2] = to_e4m3(q.m);
+                ((unsigned*)a.v)[place >> 2] = vq;
+                if (lane == 0) {
+                    a.ms[b] = mt >= LIVE ? mt / TOP : 0.f;
+                    a.vs[b] = vt >= LIVE ? vt / TOP : 0.f;
+                }
+            }
+            q = nq;
+        }
+    // The last workgroup advances the step number: every workgroup has read it (and waited for what it read) before it counts itself.  Nothing is
+    // handed from one to another, so there is no fence: a release writes the L2s back, workgroup by workgroup (50 us here).  One counter
+    // for all would take 15 ns a workgroup, one after the other: each counts at one of 32, and the last of those at the last.
     if (threadIdx.x == 0) {
-        if (__hip_atomic_fetch_add(a.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
-            *a.ticket = 0;
-            if (!skip) *a.step = step;
+        auto count = [&](int at) { return __hip_atomic_fetch_add(a.ticket + at * 32, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        const unsigned c = blockIdx.x % COUNTERS, mine = (gridDim.x - c + COUNTERS - 1) / COUNTERS, used = min((unsigned)COUNTERS, gridDim.x);
+        if (count((int)c) == mine - 1) {
+            a.ticket[c * 32] = 0;
+            if (count(COUNTERS) == used - 1) {
+                a.ticket[COUNTERS * 32] = 0;
+                if (!skip) *a.step = step;
+            }
         }
     }
 }
 
-// ---- the norm of all gradients: partial sums of squares in fixed places, then one workgroup.  It reads the gradients once more than the
+// ---- the norm of all gradients: partial sums of squares in fixed places, which the step adds.  It reads the gradients once more than the
 // step itself would, and there is no way round it: no parameter may change before the last gradient has been seen.
 struct NormArgs {
     const AdamTensor* tab;
@@ -276,30 +285,6 @@ __global__ __launch_bounds__(256) void grad_square(const NormArgs a) {
     __syncthreads();
     if (threadIdx.x == 0) a.partial[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
-struct NormEndArgs {
-    const float* partial;
-    int n;
-    float max_norm;
-    float* clip;
-    float* norm;
-};
-__global__ __launch_bounds__(256) void grad_norm_end(const NormEndArgs a) {
-    double s = 0;
-    for (int i = threadIdx.x; i < a.n; i += 256) s += (double)a.partial[i];
-    __shared__ double part[256];
-    part[threadIdx.x] = s;
-    __syncthreads();
-    for (int o = 128; o; o >>= 1) {
-        if ((int)threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        const float norm = (float)sqrt(part[0]);
-        a.clip[0] = norm;
-        a.clip[1] = fminf(1.f, a.max_norm / (norm + 1e-6f));
-        *a.norm = norm;
-    }
-}
 
 }  // namespace aipt
 
@@ -310,7 +295,7 @@ struct aipt_adamw {
     int grad_type = 0, copy_type = 0, bits = 0;
     aipt::AdamArgs args = {};
     unsigned grid = 0;
-    float *clip = nullptr, *partial = nullptr, *norm = nullptr;      // the first two in the caller's workspace
+    float* partial = nullptr;        // in the caller's workspace
 };
 
 namespace aipt {
@@ -416,12 +401,11 @@ int aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, in
     } catch (const std::bad_alloc&) {
         return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
     }
-    a->ctx = ctx; a->grad_type = grad_type; a->copy_type = copy_type; a->bits = state_bits; a->norm = norm;
-    a->clip = (float*)d_workspace + 16;
+    a->ctx = ctx; a->grad_type = grad_type; a->copy_type = copy_type; a->bits = state_bits;
     a->partial = (float*)((char*)d_workspace + aipt::SCRATCH);
     aipt::AdamTensor* d_tab = (aipt::AdamTensor*)(a->partial + aipt::GRID);
     a->args.tab = d_tab; a->args.n = (int)tab.size(); a->args.blocks = (unsigned)blocks;
-    a->args.m = m; a->args.v = v; a->args.ms = m_scale; a->args.vs = v_scale; a->args.step = step; a->args.ticket = (unsigned*)d_workspace;
+    a->args.m = m; a->args.v = v; a->args.ms = m_scale; a->args.vs = v_scale; a->args.step = step; a->args.ticket = (unsigned*)d_workspace; a->args.norm = norm;
     a->grid = (unsigned)std::min<long long>((blocks + 3) / 4, aipt::GRID);
     if (!tab.empty()) {
         aipt::DeviceScope dev(ctx->device);
@@ -450,8 +434,7 @@ int aipt_adamw_step(aipt_ctx* ctx, aipt_adamw* a, double lr, double beta1, doubl
     if (clip) {
         aipt::NormKernel k = t == AIPT_TYPE_F32 ? aipt::grad_square<float> : t == AIPT_TYPE_BF16 ? aipt::grad_square<aipt::bf16> : aipt::grad_square<aipt::f16>;
         AIPT_HIP(ctx, aipt::launch(k, a->grid, 256, 0, ctx->stream, aipt::NormArgs{l.tab, l.n, l.blocks, a->partial}));
-        AIPT_HIP(ctx, aipt::launch(aipt::grad_norm_end, 1, 256, 0, ctx->stream, aipt::NormEndArgs{a->partial, (int)a->grid, (float)max_norm, a->clip, a->norm}));
-        l.clip = a->clip;
+        l.partial = a->partial; l.npartial = (int)a->grid; l.max_norm = (float)max_norm;
     }
     l.ln1 = std::log(beta1); l.ln2 = std::log(beta2);
     l.lr = (float)lr; l.beta1 = (float)beta1; l.beta2 = (float)beta2; l.eps = (float)eps;
