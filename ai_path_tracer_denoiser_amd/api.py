@@ -521,7 +521,8 @@ class Context:
             # (ExternalStream takes 0 for "none given" and makes a new stream)
             self._ext = torch.cuda.ExternalStream(self._stream, device=self.device) if self._stream else torch.cuda.default_stream(self.device)
         if torch._C._cuda_getCurrentRawStream(self.device) == self._stream:
-            return self._ck(entry(self._h, *args))
+            rc = entry(self._h, *args)
+            return self._ck(rc) if rc else None
         now = torch.cuda.current_stream(self.device)
         if not self._stream and torch.cuda.is_current_stream_capturing():
             raise AiptError("a context on the default stream cannot take part in a capture: make one with stream=<the capturing stream's handle>")
@@ -534,33 +535,37 @@ class Context:
         """(memory or None, its address, bytes) of an operator's workspace: torch's, so that a captured graph keeps its own"""
         n = C.c_size_t()
         self._ck(entry(self._h, record, C.byref(n)))
-        if not n.value:
+        size = n.value
+        if not size:
             return None, None, 0
         import torch
-        t = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", self.device))
-        return t, t.data_ptr(), n.value
+        t = torch.empty(size, dtype=torch.uint8, device=self.device)
+        return t, t.data_ptr(), size
 
     def _type(self, t):
         kind = _types().get(t.dtype)
-        if kind is None or not t.is_cuda or t.get_device() != self.device:
+        if kind is None or t.get_device() != self.device:
             raise AiptError(f"a {t.dtype} tensor on {t.device}: float32, bfloat16 or float16 on cuda:{self.device} is wanted")
         return kind
 
+    # (get_device() is -1 of a CPU tensor; a shape compares like a tuple)
     def _want(self, name, t, dtype, *shape):
-        if t.dtype != dtype or not t.is_cuda or t.get_device() != self.device or tuple(t.shape) != shape:
+        if t.dtype is not dtype or t.get_device() != self.device or t.shape != shape:
             raise AiptError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}; {dtype} {shape} on cuda:{self.device} is wanted")
 
     def _matrix(self, name, t, dtype, rows, cols):
         """(address, row stride, column stride) of an optional matrix"""
         if t is None:
             return 0, 0, 0
-        self._want(name, t, dtype, rows, cols)
+        if t.dtype is not dtype or t.get_device() != self.device or t.shape != (rows, cols):
+            self._want(name, t, dtype, rows, cols)
         return (t.data_ptr(), *t.stride())
 
     def _vector(self, name, t, dtype, n):
         if t is None:
             return 0
-        self._want(name, t, dtype, n)
+        if t.dtype is not dtype or t.get_device() != self.device or t.shape != (n,):
+            self._want(name, t, dtype, n)
         if n > 1 and t.stride(0) != 1:
             raise AiptError(f"{name}: stride {t.stride(0)}")
         return t.data_ptr()

@@ -30,6 +30,7 @@ struct GemmArgs {
     long long ri, rj;
     void* pre;
     long long pi, pj;
+    int turned;                      // gemm_rows: A and B are the result's j and i
     int c16;                         // rows of c, res and pre lie on 16 bytes, j contiguous
 };
 
@@ -522,6 +523,45 @@ __global__ __launch_bounds__(256) void gemm_join(const GemmArgs g) {
     }
 }
 
+// ---- a few rows (at most 8): every line of the many is read once, 16 bytes a lane, by the wave that its results belong to: no tile, no split, one
+// launch.  R lines a wave (their loads are under way together), M rows; the rows stay in the first-level cache.
+template <typename T, int M, int R>
+__global__ __launch_bounds__(256) void gemm_rows(const GemmArgs g) {
+    constexpr int E = 16 / sizeof(T);
+    const int lane = threadIdx.x & 63, j0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * R;
+    if (j0 >= g.J) return;
+    float acc[M][R] = {};
+    const T* b[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) b[r] = (const T*)g.b + (long long)min(j0 + r, g.J - 1) * g.bs;
+#pragma unroll 4
+    for (int k = lane * E; k < g.K; k += 64 * E) {
+        Chunk<T> w[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) w[r] = *(const Chunk<T>*)(b[r] + k);
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            const Chunk<T> x = *(const Chunk<T>*)((const T*)g.a + (long long)min(m, g.I - 1) * g.as + k);
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int e = 0; e < E; e++) acc[m][r] = fmaf((float)x.v[e], (float)w[r].v[e], acc[m][r]);
+        }
+    }
+    float mine = 0;                  // lane m R + r: row m, line r
+#pragma unroll
+    for (int m = 0; m < M; m++)
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float z = wave_sum(acc[m][r]);
+            if (lane == m * R + r) mine = z;
+        }
+    const int m = lane / R, j = j0 + lane % R;
+    if (m >= M || m >= g.I || j >= g.J) return;
+    if (g.turned) epilogue<T>(g, j, m, mine);
+    else epilogue<T>(g, m, j, mine);
+}
+
 // ---- 16-bit lines that begin anywhere, copied to lines on 16 bytes, padded with zeros: twice the operand's bytes, once, for loads of 16 bytes
 // in every tile that reads it (1375 x 909 by 303 x 909: 58 us by gemm_any)
 struct PackArgs {
@@ -542,40 +582,69 @@ __global__ __launch_bounds__(256) void pack_lines(const PackArgs g) {
     }
 }
 
-// ---- dz = dy * act'(z), rounded to the element type, and its sums over rows: both read dy once.  Tiles of 64 (contiguous axis) x 64.
+// ---- dz = dy * act'(z), rounded to the element type, and its sums over rows: dy is read once for both.  A workgroup takes `high` rows by 64
+// lanes' columns -- V elements (16 bytes) a lane where lines lie on 16 bytes, else one -- or, where rows are the contiguous axis, the
+// transpose of that.
 struct DzArgs {
     const void *dy, *z;
     void* dz;
-    float* part;                     // [row tiles][N] sums over 64 rows, or NULL
-    long long dyi, dyj, zi, zj, dzi, dzj;
-    int M, N, tiles_n, turned;       // turned: rows are the contiguous axis
+    float* part;                     // [ceil(M / high)][N] sums over a workgroup's rows, or NULL
+    long long dys, zs, zi, zj, dzs;  // strides from line to line (and both of z's, which may lie the other way)
+    int M, N;                        // rows and columns of dy
     int line;                        // dz's lines, with their padding (of zeros)
-    int act;
+    int high, tiles_n, act;
     float slope;
 };
-template <typename T>
+template <typename T, int V, bool TURNED>
 __global__ __launch_bounds__(256) void act_backward(const DzArgs g) {
-    __shared__ float lds[64][65];
-    const int m0 = (int)(blockIdx.x / g.tiles_n) * 64, n0 = (int)(blockIdx.x % g.tiles_n) * 64;
-    const int x = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int y = w; y < 64; y += 4) {
-        const int m = m0 + (g.turned ? x : y), n = n0 + (g.turned ? y : x);
-        float d = 0;
-        if (m < g.M && n < g.N) {
-            d = (float)((const T*)g.dy)[m * g.dyi + n * g.dyj];
-            if (g.act != AIPT_ACT_NONE) d *= act_slope_of((float)((const T*)g.z)[m * g.zi + n * g.zj], g.act, g.slope);
+    struct alignas(V == 1 ? sizeof(T) : 16) E { T v[V]; };
+    __shared__ float lds[4][64 * V];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int tm = (int)(blockIdx.x / g.tiles_n), tn = (int)(blockIdx.x % g.tiles_n);
+    // lines of the tile, and the lane's first element of a line
+    const int lines = TURNED ? g.N : g.M, len = TURNED ? g.M : g.N;
+    const int l0 = TURNED ? tn * 64 : tm * g.high, l1 = min(lines, l0 + (TURNED ? 64 : g.high));
+    const int c0 = TURNED ? tm * g.high : tn * 64 * V, c1 = min(max(len, g.line), TURNED ? c0 + g.high : c0 + 64 * V);
+    float sum[V] = {};
+    for (int l = l0 + w; l < l1; l += 4) {
+        float along = 0;
+        for (int c = c0 + lane * V; c < c1; c += 64 * V) {
+            float d[V] = {};
+            if (c < len) {                                   // (V > 1: len is whole loads)
+                const E dy = *(const E*)((const T*)g.dy + l * g.dys + c);
+#pragma unroll
+                for (int i = 0; i < V; i++) d[i] = (float)dy.v[i];
+                if (g.act != AIPT_ACT_NONE) {
+                    E z;
+                    if (V > 1) z = *(const E*)((const T*)g.z + l * g.zs + c);
+                    else z.v[0] = ((const T*)g.z)[(TURNED ? c : l) * g.zi + (TURNED ? l : c) * g.zj];
+#pragma unroll
+                    for (int i = 0; i < V; i++) d[i] *= act_slope_of((float)z.v[i], g.act, g.slope);
+                }
+            }
+            if (g.dz && c < g.line) {
+                E o;
+#pragma unroll
+                for (int i = 0; i < V; i++) o.v[i] = (T)d[i];
+                *(E*)((T*)g.dz + l * g.dzs + c) = o;
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                if (TURNED) along += d[i];
+                else sum[i] += d[i];
+            }
         }
-        if (g.dz && (g.turned ? n < g.N && m < g.line : m < g.M && n < g.line)) ((T*)g.dz)[m * g.dzi + n * g.dzj] = (T)d;
-        lds[g.turned ? x : y][g.turned ? y : x] = d;
+        if (TURNED && g.part) {
+            along = wave_sum(along);
+            if (lane == 0) g.part[(long long)tm * g.N + l] = along;
+        }
     }
-    if (!g.part) return;
+    if (TURNED || !g.part) return;
+#pragma unroll
+    for (int i = 0; i < V; i++) lds[w][lane * V + i] = sum[i];
     __syncthreads();
-    float s = 0;
-    for (int y = w; y < 64; y += 4) s += lds[y][x];
-    __syncthreads();
-    lds[w][x] = s;
-    __syncthreads();
-    if (w == 0 && n0 + x < g.N) g.part[(long long)(m0 / 64) * g.N + n0 + x] = (lds[0][x] + lds[1][x]) + (lds[2][x] + lds[3][x]);
+    for (int c = threadIdx.x; c < 64 * V && c0 + c < g.N; c += 256)
+        g.part[(long long)tm * g.N + c0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
 }
 struct SumArgs {
     const float* part;
@@ -583,14 +652,21 @@ struct SumArgs {
     int parts, N;
 };
 template <typename T>
-__global__ __launch_bounds__(256) void sum_parts(const SumArgs g) {
-    __shared__ float lds[4][64];
+__global__ __launch_bounds__(1024) void sum_parts(const SumArgs g) {
+    __shared__ float lds[16][64];
     const int x = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + x;
     float s = 0;
-    if (n < g.N) for (int p = w; p < g.parts; p += 4) s += g.part[(long long)p * g.N + n];
+    if (n < g.N) {
+#pragma unroll 8
+        for (int p = w; p < g.parts; p += 16) s += g.part[(long long)p * g.N + n];
+    }
     lds[w][x] = s;
     __syncthreads();
-    if (w == 0 && n < g.N) ((T*)g.out)[n] = (T)((lds[0][x] + lds[1][x]) + (lds[2][x] + lds[3][x]));
+    if (w || n >= g.N) return;
+    s = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s += lds[i][x];
+    ((T*)g.out)[n] = (T)s;
 }
 
 struct FillArgs { unsigned short* p; size_t n; };
@@ -651,8 +727,9 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct Plan {                        // a product as it will be launched, and the workspace it wants
     GemmArgs g = {};
     bool ak = true, bk = true;
-    int tile = 0;                    // 0: gemm_any; else gemm_tile of this size
+    int tile = 0;                    // 0: gemm_any; -1: gemm_rows; else gemm_tile of this size
     bool small = false;              // ... with loads of 4 bytes
+    int rows = 0;                    // of gemm_rows
     PackArgs pack = {};              // operands that are copied first
     size_t pack_bytes = 0, partial_bytes = 0, blocks = 0;
     bool fits = true;
@@ -728,7 +805,22 @@ static Plan plan_gemm(int type, View a, View b, long long I, long long J, long l
     const long long pairs = (K + ks - 1) / ks;
     long long splits = 1;
     p.small = std::min(w[0], w[1]) == 4;
-    if (w[0] && w[1] && I && J) pick(es == 4, p.small, I, J, pairs, p.tile, splits);
+    if (w[0] && w[1] && I && J) {
+        const double us = pick(es == 4, p.small, I, J, pairs, p.tile, splits);
+        // gemm_rows: lines of k on 16 bytes.  3 us and the many lines at 4 TB/s, but no faster than a wave goes along its lines
+        const long long few = std::min(I, J), many = std::max(I, J);
+        if (p.ak && p.bk && w[0] == 16 && w[1] == 16 && K % E == 0 && !p.pack_bytes && few <= 8 && K &&
+            3 + std::max(many * K * es / 4e6, (double)K / (64 * E) * 0.1 * few) < us) {
+            p.tile = -1;
+            p.g.splits = 1;
+            p.g.turned = J < I;
+            if (p.g.turned) { std::swap(p.g.a, p.g.b); std::swap(p.g.as, p.g.bs); std::swap(p.g.I, p.g.J); }
+            p.rows = few <= 1 ? 1 : few <= 2 ? 2 : few <= 4 ? 4 : 8;
+            p.blocks = (size_t)((many + 4 * (p.rows <= 2 ? 2 : 4) - 1) / (4 * (p.rows <= 2 ? 2 : 4)));
+            p.fits = grid_fits(p.blocks, 256);
+            return p;
+        }
+    }
     const int ti = p.tile ? TILES[p.tile].i : GT, tj = p.tile ? TILES[p.tile].j : GT, step = ks;
     p.g.tiles_i = (int)((I + ti - 1) / ti); p.g.tiles_j = (int)((J + tj - 1) / tj);
     const long long tiles = (long long)p.g.tiles_i * p.g.tiles_j, steps = pairs;
@@ -750,6 +842,7 @@ template <typename T, int TI, int TJ, int WI, int WJ, int S, int W> static void 
 }
 template <typename T> static void (*gemm_of(const Plan& p))(GemmArgs) {
     switch (p.tile) {
+        case -1: return p.rows == 1 ? gemm_rows<T, 1, 2> : p.rows == 2 ? gemm_rows<T, 2, 2> : p.rows == 4 ? gemm_rows<T, 4, 4> : gemm_rows<T, 8, 4>;
         case 1: return tile_kernel<T, 256, 256, 2, 2, 5, 16>(p);
         case 2: return tile_kernel<T, 128, 128, 2, 2, 5, 16>(p);
         case 3: return p.small ? tile_kernel<T, 64, 64, 2, 2, 6, 4>(p) : tile_kernel<T, 64, 64, 2, 2, 6, 16>(p);
@@ -804,6 +897,8 @@ struct GradPlan {
     Plan dx, dw;
     DzArgs dz = {};
     bool want_dx = false, want_dw = false, want_db = false, make_dz = false;
+    bool dz_vec = false, dz_turned = false;
+    int parts = 0;
     size_t dz_bytes = 0, part_bytes = 0, gemm_bytes = 0, dz_blocks = 0;
     size_t bytes() const { return dz_bytes + part_bytes + gemm_bytes; }
 };
@@ -822,16 +917,25 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         p.dz.line = (int)ld;
         d = {ws, dy.second ? ld : 1, dy.second ? 1 : ld, dy.second, ld, true};
     }
-    const long long tm = (a->m + 63) / 64, tn = (a->n + 63) / 64;
+    // 64 rows a workgroup, or so many that there are at most 1 024 partial sums a column
+    const long long high = std::max(1ll, ((a->m + 1023) / 1024 + 63) / 64) * 64, tm = (a->m + high - 1) / high;
+    p.parts = (int)tm;
     if (p.want_db) p.part_bytes = up256((size_t)tm * a->n * sizeof(float));
     if (p.make_dz || p.want_db) {
         DzArgs& g = p.dz;
+        const bool turned = !dy.second;
+        const long long len = turned ? a->m : a->n, zline = turned ? z.rj : z.ri;
+        const bool z_same = a->act == AIPT_ACT_NONE || (z.second == dy.second && !((uintptr_t)z.p & 15) && zline % E == 0);
+        p.dz_vec = !((uintptr_t)dy.p & 15) && dy.other % E == 0 && len % E == 0 && z_same;
+        p.dz_turned = turned;
         g.dy = a->dy.data; g.z = a->preact.data; g.dz = p.make_dz ? d.p : nullptr;
         g.part = p.want_db ? (float*)(ws + p.dz_bytes) : nullptr;
-        g.dyi = dy.ri; g.dyj = dy.rj; g.zi = z.ri; g.zj = z.rj; g.dzi = d.ri; g.dzj = d.rj;
-        g.M = (int)a->m; g.N = (int)a->n; g.tiles_n = (int)tn; g.turned = !dy.second;
+        g.dys = dy.other; g.zs = zline; g.zi = z.ri; g.zj = z.rj; g.dzs = d.other;
+        g.M = (int)a->m; g.N = (int)a->n; g.high = (int)high;
+        const long long wide = turned ? 64 : 64 * (p.dz_vec ? E : 1);
+        g.tiles_n = (int)((std::max<long long>(a->n, turned ? 0 : g.line) + wide - 1) / wide);
         g.act = a->act; g.slope = a->slope;
-        p.dz_blocks = (size_t)(tm * tn);
+        p.dz_blocks = (size_t)tm * g.tiles_n;
     }
     auto flip = [](View v) { std::swap(v.ri, v.rj); v.second = !v.second; return v; };
     if (p.want_dx) {                 // dx[m][k] = sum_n dz[m][n] w[n][k]
@@ -846,6 +950,11 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
     }
     p.gemm_bytes = up256(std::max(p.want_dx ? p.dx.bytes() : 0, p.want_dw ? p.dw.bytes() : 0));
     return p;
+}
+
+template <typename T> static void (*dz_kernel(const GradPlan& p))(DzArgs) {
+    constexpr int V = 16 / sizeof(T);
+    return p.dz_vec ? (p.dz_turned ? act_backward<T, V, true> : act_backward<T, V, false>) : (p.dz_turned ? act_backward<T, 1, true> : act_backward<T, 1, false>);
 }
 
 static int linear_check(aipt_ctx* ctx, const char* me, int type, int act, float slope, int reserved, long long m, long long n, long long k) {
@@ -963,10 +1072,10 @@ int aipt_linear_backward(aipt_ctx* ctx, const aipt_linear_grad_args* a, void* d_
     const hipStream_t st = ctx->stream;
     const int t = a->type;
     if (p.dz_blocks)
-        AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::act_backward<float> : t == AIPT_TYPE_BF16 ? aipt::act_backward<aipt::bf16> : aipt::act_backward<aipt::f16>, p.dz_blocks, 256, 0, st, p.dz));
+        AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::dz_kernel<float>(p) : t == AIPT_TYPE_BF16 ? aipt::dz_kernel<aipt::bf16>(p) : aipt::dz_kernel<aipt::f16>(p), p.dz_blocks, 256, 0, st, p.dz));
     if (p.want_db) {
-        if (a->m) AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::sum_parts<float> : t == AIPT_TYPE_BF16 ? aipt::sum_parts<aipt::bf16> : aipt::sum_parts<aipt::f16>, (size_t)((a->n + 63) / 64), 256, 0, st,
-                                             aipt::SumArgs{p.dz.part, a->dbias, (int)((a->m + 63) / 64), (int)a->n}));
+        if (a->m) AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::sum_parts<float> : t == AIPT_TYPE_BF16 ? aipt::sum_parts<aipt::bf16> : aipt::sum_parts<aipt::f16>, (size_t)((a->n + 63) / 64), 1024, 0, st,
+                                             aipt::SumArgs{p.dz.part, a->dbias, p.parts, (int)a->n}));
         else AIPT_HIP(ctx, aipt::zero_fill(st, a->dbias, (size_t)a->n * es));
     }
     char* gemm_ws = (char*)d_workspace + p.dz_bytes + p.part_bytes;
