@@ -78,6 +78,15 @@ __device__ inline unsigned to_e4m3(const float* o) {
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(o[2], o[3], q, true);
 }
 
+// x > 0 to one of the two e4m3 values around it, up with the probability of its distance from the lower one: the mean is x.  Steps of 2^-9 below
+// 2^-6, of an eighth of the binade above; `random`: 24 of its bits count.  (The chip's own conversion by chance takes 20, truncated; this
+// one is the formula in fp32, so that whoever works it out gets the same bits.)
+__device__ inline unsigned chance_e4m3(float x, unsigned random) {
+    const int e = max(__builtin_amdgcn_frexp_expf(x), -5);                 // x < 2^e
+    const float q = __builtin_amdgcn_ldexpf(x, 4 - e) + (float)(random >> 8) * 0x1p-24f;
+    return min((unsigned)((e + 5) * 8 + (int)q), 126u);                    // exponent field and mantissa at once, carries included; 126: 448
+}
+
 // 32 random bits from a place and a key: multiplications by odd constants (fractions of the golden ratio and of the roots of 3 and 5)
 // carry low bits up, the shifts bring high ones down
 __device__ inline unsigned hash(unsigned long long place, unsigned key) {
@@ -166,7 +175,7 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
         for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
         if (lane == 0) norms[threadIdx.x >> 6] = s;
         __syncthreads();
-        const float norm = (float)sqrt((norms[0] + norms[1]) + (norms[2] + norms[3]));
+        const float norm = sqrtf((float)((norms[0] + norms[1]) + (norms[2] + norms[3])));
         factor = fminf(1.f, a.max_norm / (norm + 1e-6f));
         skip = !(norm <= 3.4028235e38f);                                   // inf and NaN
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
@@ -190,8 +199,8 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
                 const float gi = q.g[i] * factor;
                 q.m[i] = q.m[i] * a.beta1 + gi * a.omb1;
                 q.v[i] = q.v[i] * a.beta2 + gi * gi * a.omb2;
-                // the chip's root and reciprocal, an ulp each: the step is within 6 ulp of itself, far below the parameter's own
-                r[i] = __builtin_amdgcn_sqrtf(q.v[i]);
+                // the chip's root and reciprocal, an ulp each: the step is within 6 ulp of itself, far below the parameter's own (a root that is stored is exact)
+                r[i] = BITS == 8 ? sqrtf(q.v[i]) : __builtin_amdgcn_sqrtf(q.v[i]);
                 q.p[i] = q.p[i] * keep - rate * q.m[i] * __builtin_amdgcn_rcpf(r[i] * root2 + a.eps);
             }
             if (q.wide) {
@@ -216,20 +225,21 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
             } else {
                 const float mt = wave_max(fmaxf(fmaxf(fabsf(q.m[0]), fabsf(q.m[1])), fmaxf(fabsf(q.m[2]), fabsf(q.m[3]))));
                 const float vt = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
-                const float mi = mt >= LIVE ? TOP / mt : 0.f, vi = vt >= LIVE ? TOP / vt : 0.f, least = vt >= LIVE ? 0x1p-9f : 0.f;
+                const bool ml = mt >= LIVE, vl = vt >= LIVE;
+                const float mi = ml ? 1.f / mt * TOP : 0.f, vi = vl ? 1.f / vt * TOP : 0.f;
                 unsigned vq = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) q.m[i] = fminf(fmaxf(q.m[i] * mi, -TOP), TOP);
-                // up or down by chance is an instruction of the chip's (it adds 20 of the bits below the mantissa's last, subnormals included); what is
-                // not zero begins at the least e4m3, so that it stays so
-#define AIPT_CHANCE(i) vq = __builtin_amdgcn_cvt_sr_fp8_f32(r[i] > 0.f ? fminf(fmaxf(r[i] * vi, least), TOP) : 0.f, hash(place + i, key), vq, i);
-                AIPT_CHANCE(0) AIPT_CHANCE(1) AIPT_CHANCE(2) AIPT_CHANCE(3)
-#undef AIPT_CHANCE
+                for (int i = 0; i < 4; i++) {
+                    q.m[i] = fminf(fmaxf(q.m[i] * mi, -TOP), TOP);
+                    // what is not zero begins at the least e4m3, so that it stays so
+                    const unsigned code = chance_e4m3(fmaxf(r[i] * vi, 0x1p-9f), hash(place + i, key));
+                    vq |= (r[i] > 0.f && vl ? code : 0u) << (8 * i);
+                }
                 ((unsigned*)a.m)[place >> 2] = to_e4m3(q.m);
                 ((unsigned*)a.v)[place >> 2] = vq;
                 if (lane == 0) {
-                    a.ms[b] = mt >= LIVE ? mt / TOP : 0.f;
-                    a.vs[b] = vt >= LIVE ? vt / TOP : 0.f;
+                    a.ms[b] = ml ? mt * (1.f / TOP) : 0.f;
+                    a.vs[b] = vl ? vt * (1.f / TOP) : 0.f;
                 }
             }
             q = nq;
