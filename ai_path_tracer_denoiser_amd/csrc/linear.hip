@@ -31,7 +31,7 @@ struct GemmArgs {
     void* pre;
     long long pi, pj;
     int turned;                      // gemm_rows: A and B are the result's j and i
-    int c16;                         // rows of c, res and pre lie on 16 bytes, j contiguous
+    int cv;                          // elements that move together: 8 (rows of c, res and pre on 16 bytes, j contiguous), 2 (on two elements) or 1
 };
 
 // 1 / (1 + e^-z) by the chip's exponential and reciprocal (an ulp each): z is within 2^-24 |z| of what it should be in the exponent
@@ -256,18 +256,25 @@ template <int ES, bool KC, int R, int NT, int W> struct TileLoad {
             }
         }
     }
-    // which group of line k lies where: as many values as a line has groups, 8 (4) at most
+    // Which group of line k lies where.  16 bits: the eight lines that 32 lanes read together (k = 0 .. 3, 8 .. 11) begin at as many of the
+    // eight 32-byte places of all banks; where lines are shorter than those, by their own places too.  Floats: the four lines of a wave's 64 lanes.
     static __device__ inline int swap(int k) {
-        constexpr int G = R / 16;
-        return ES == 2 ? ((k & 3) | ((k >> 1) & 4)) & (G < 8 ? G - 1 : 7) : (k >> 2) & (G < 4 ? G - 1 : 3);
+        if (ES == 4) return (k >> 2) & (R / 16 < 4 ? R / 16 - 1 : 3);
+        if (R == 64) return ((k >> 1) & 1) | ((k >> 2) & 2);
+        if (R == 32) return (k >> 3) & 1;
+        return (k & 3) | ((k >> 1) & 4);
     }
-    // where pair t lies; load i of it, `left` of k being left
-    __device__ inline __amdgpu_buffer_rsrc_t at(int t) const { return __builtin_amdgcn_make_buffer_rsrc((void*)(base + t * step), 0, 0x7fffffff, 0x00027000); }
-    __device__ inline void one(int i, __amdgpu_buffer_rsrc_t rs, int left, AIPT_LDS char* lds, int wave) const {
+    // where pair t lies, as a buffer (raw, 2 GiB - 1); load i of it, `left` of k being left.  In assembly: the compiler waits for every load to LDS
+    // before a transposing read (vmcnt(0)), and so for loads that are meant for later pairs; the waits are at the barriers.
+    __device__ inline i32x4 at(int t) const {
+        const unsigned long long p = (unsigned long long)(base + t * step);
+        return i32x4{__builtin_amdgcn_readfirstlane((int)p), __builtin_amdgcn_readfirstlane((int)(p >> 32) & 0xffff), 0x7fffffff, 0x00027000};
+    }
+    __device__ inline void one(int i, i32x4 rs, int left, AIPT_LDS char* lds, int wave) const {
         const unsigned o = kof[i] < left ? off[i] : 0x80000000u;
-        AIPT_LDS void* to = (AIPT_LDS void*)(lds + (i * NT + wave * 64) * W);
-        if constexpr (W == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, to, 16, o, 0, 0, 0);
-        else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, to, 4, o, 0, 0, 0);
+        const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds + (i * NT + wave * 64) * W));
+        if constexpr (W == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(o), "s"(rs) : "memory", "m0");
+        else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(o), "s"(rs) : "memory", "m0");
     }
 };
 
@@ -455,10 +462,49 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
     AIPT_LDS char* slab = lds + wave * (SLAB * WTJ * 4);
     constexpr int LR = WTJ / 8, RPI = 64 / LR;               // lanes of a row, rows of an instruction
     const int j = j0 + wj + lane % LR * 8;
-    const bool whole = j + 8 <= g.J && g.c16;
+    const bool whole = j + 8 <= g.J;
     float bias_j[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) bias_j[e] = g.bias && !g.bias_i && g.splits == 1 && j + e < g.J ? (float)((const T*)g.bias)[j + e] : 0.f;
+    // rows that begin anywhere: neighbouring lanes, EV neighbouring elements each
+    auto narrow = [&](auto ev, int s) {
+        constexpr int EV = decltype(ev)::value, LN = WTJ / EV < 64 ? WTJ / EV : 64, RS = 64 / LN;
+        struct alignas(EV * sizeof(T)) E { T v[EV]; };
+#pragma unroll
+        for (int h = 0; h < WTJ / (EV * LN); h++) {
+            const int c = (h * LN + lane % LN) * EV, jj = j0 + wj + c;
+            if (jj >= g.J) continue;                         // (EV = 2: J is even)
+            float bias[EV];
+#pragma unroll
+            for (int e = 0; e < EV; e++) bias[e] = g.bias && !g.bias_i ? (float)((const T*)g.bias)[jj + e] : 0.f;
+            const int r0 = lane / LN, ii = i0 + wi + s * SLAB + r0, end = min(SLAB, g.I - (i0 + wi + s * SLAB));
+            T* o = (T*)g.c + (long long)ii * g.cs + jj;
+            T* pre = g.pre ? (T*)g.pre + ii * g.pi + jj * g.pj : nullptr;
+            const T* res = g.res ? (const T*)g.res + ii * g.ri + jj * g.rj : nullptr;
+#pragma unroll 4
+            for (int r = r0; r < end; r += RS, o += RS * g.cs) {
+                float z[EV];
+#pragma unroll
+                for (int e = 0; e < EV; e++) z[e] = *(AIPT_LDS float*)(slab + r * (WTJ * 4) + (((c >> 2) ^ (r & XM)) * 16) + (c & 3) * 4 + e * 4);
+                E q;
+                const float bi = g.bias && g.bias_i ? (float)((const T*)g.bias)[ii - r0 + r] : 0.f;
+#pragma unroll
+                for (int e = 0; e < EV; e++) { z[e] += g.bias_i ? bi : bias[e]; q.v[e] = (T)z[e]; }
+                if (pre) { *(E*)pre = q; pre += RS * g.pi; }
+#pragma unroll
+                for (int e = 0; e < EV; e++) z[e] = act_of(z[e], g.act, g.slope);
+                if (res) {
+                    const E v = *(const E*)res;
+#pragma unroll
+                    for (int e = 0; e < EV; e++) z[e] += (float)v.v[e];
+                    res += RS * g.ri;
+                }
+#pragma unroll
+                for (int e = 0; e < EV; e++) q.v[e] = (T)z[e];
+                *(E*)o = q;
+            }
+        }
+    };
 #pragma unroll
     for (int s = 0; s < WTI / SLAB; s++) {
 #pragma unroll
@@ -487,7 +533,10 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
                 for (int e = 0; e < 8; e++) if (j + e < g.J) o[e] = z[e];
             }
         });
-        else if (!whole) rows([&](int i, float* z) {
+        else if (g.cv == 2) narrow(integral_constant<int, 2>{}, s);
+        else if (g.cv == 1) {
+            narrow(integral_constant<int, 1>{}, s);
+        } else if (!whole) rows([&](int i, float* z) {
 #pragma unroll
             for (int e = 0; e < 8; e++) if (j + e < g.J) epilogue<T>(g, i, j + e, z[e]);
         });
@@ -498,28 +547,50 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
     }
 }
 
-// the splits of a long contraction, added in order, and the epilogue: four neighbours a thread
-template <typename T>
+// The splits of a long contraction, added in a fixed order, and the epilogue: four neighbours a thread.  SIDE threads share a result's splits
+// (many splits of a small result: one thread for each result ran for 245 us at 368 splits of 64 x 46).
+template <typename T, int SIDE>
 __global__ __launch_bounds__(256) void gemm_join(const GemmArgs g) {
-    const int per = (g.J + 3) / 4;
+    constexpr int QUADS = 256 / SIDE;
+    __shared__ float4 lds[SIDE > 1 ? SIDE : 1][QUADS];
+    const int per = (g.J + 3) / 4, x = threadIdx.x % QUADS, side = threadIdx.x / QUADS;
     const long long quads = (long long)g.I * per, n = (long long)g.I * g.J;
     const bool quad16 = !(g.J & 3);
-    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < quads; at += (long long)gridDim.x * 256) {
+    for (long long q0 = (long long)blockIdx.x * QUADS; q0 < quads; q0 += (long long)gridDim.x * QUADS) {
+        const long long at = q0 + x;
         const int i = (int)(at / per), j = (int)(at - (long long)i * per) * 4;
-        const float* p = g.partial + (long long)i * g.J + j;
         float s[4] = {};
-        if (quad16) {
-            for (int k = 0; k < g.splits; k++, p += n) {
-                const float4 v = *(const float4*)p;
+        if (at < quads) {
+            const float* p = g.partial + (long long)i * g.J + j;
+            if (quad16) {
+#pragma unroll 4
+                for (int k = side; k < g.splits; k += SIDE) {
+                    const float4 v = *(const float4*)(p + k * n);
+                    s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+                }
+            } else {
+#pragma unroll 4
+                for (int k = side; k < g.splits; k += SIDE)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[e] += p[k * n + (j + e < g.J ? e : 0)];        // (beyond the line: not stored)
+            }
+        }
+        if constexpr (SIDE > 1) {
+            __syncthreads();
+            lds[side][x] = make_float4(s[0], s[1], s[2], s[3]);
+            __syncthreads();
+            if (side) continue;
+            s[0] = s[1] = s[2] = s[3] = 0;
+#pragma unroll
+            for (int k = 0; k < SIDE; k++) {
+                const float4 v = lds[k][x];
                 s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
             }
-        } else {
-            for (int k = 0; k < g.splits; k++, p += n)
-#pragma unroll
-                for (int e = 0; e < 4; e++) if (j + e < g.J) s[e] += p[e];
         }
+        if (at < quads) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) if (j + e < g.J) epilogue<T>(g, i, j + e, s[e]);
+            for (int e = 0; e < 4; e++) if (j + e < g.J) epilogue<T>(g, i, j + e, s[e]);
+        }
     }
 }
 
@@ -562,7 +633,7 @@ __global__ __launch_bounds__(256) void gemm_rows(const GemmArgs g) {
     else epilogue<T>(g, m, j, mine);
 }
 
-// ---- 16-bit lines that begin anywhere, copied to lines on 16 bytes, padded with zeros: twice the operand's bytes, once, for loads of 16 bytes
+// ---- lines that begin anywhere (of halves: an element is one or two), copied to lines on 16 bytes, padded with zeros: twice the operand's bytes, once, for loads of 16 bytes
 // in every tile that reads it (1375 x 909 by 303 x 909: 58 us by gemm_any)
 struct PackArgs {
     struct { const unsigned short* p; Chunk<unsigned short>* to; long long stride, chunks; int len, line; } m[2];      // line: chunks of a line
@@ -582,69 +653,90 @@ __global__ __launch_bounds__(256) void pack_lines(const PackArgs g) {
     }
 }
 
-// ---- dz = dy * act'(z), rounded to the element type, and its sums over rows: dy is read once for both.  A workgroup takes `high` rows by 64
-// lanes' columns -- V elements (16 bytes) a lane where lines lie on 16 bytes, else one -- or, where rows are the contiguous axis, the
-// transpose of that.
+// ---- dz = dy * act'(z), rounded to the element type, and its sums over rows: dy is read once for both.  V elements (16 bytes) a lane where lines
+// lie on 16 bytes, else one.  A workgroup takes `high` rows; `across` lanes (a power of two) share a row, so that narrow rows too fill a
+// wave, and a lane's columns stay its own.  Where rows are the contiguous axis (TURNED): 64 lines (columns) of `high` rows, a wave each.
 struct DzArgs {
     const void *dy, *z;
     void* dz;
     float* part;                     // [ceil(M / high)][N] sums over a workgroup's rows, or NULL
+    void* sum;                       // ... or, where one workgroup has all rows, the sums themselves
     long long dys, zs, zi, zj, dzs;  // strides from line to line (and both of z's, which may lie the other way)
     int M, N;                        // rows and columns of dy
     int line;                        // dz's lines, with their padding (of zeros)
-    int high, tiles_n, act;
+    int high, tiles_n, across, act;
     float slope;
 };
 template <typename T, int V, bool TURNED>
 __global__ __launch_bounds__(256) void act_backward(const DzArgs g) {
     struct alignas(V == 1 ? sizeof(T) : 16) E { T v[V]; };
-    __shared__ float lds[4][64 * V];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __shared__ float lds[TURNED ? 1 : 256 * V];
     const int tm = (int)(blockIdx.x / g.tiles_n), tn = (int)(blockIdx.x % g.tiles_n);
-    // lines of the tile, and the lane's first element of a line
-    const int lines = TURNED ? g.N : g.M, len = TURNED ? g.M : g.N;
-    const int l0 = TURNED ? tn * 64 : tm * g.high, l1 = min(lines, l0 + (TURNED ? 64 : g.high));
-    const int c0 = TURNED ? tm * g.high : tn * 64 * V, c1 = min(max(len, g.line), TURNED ? c0 + g.high : c0 + 64 * V);
-    float sum[V] = {};
-    for (int l = l0 + w; l < l1; l += 4) {
-        float along = 0;
-        for (int c = c0 + lane * V; c < c1; c += 64 * V) {
-            float d[V] = {};
-            if (c < len) {                                   // (V > 1: len is whole loads)
-                const E dy = *(const E*)((const T*)g.dy + l * g.dys + c);
+    auto one = [&](int l, int c, int len, float* d) {         // elements c .. of line l
+        if (c < len) {                                       // (V > 1: len is whole loads)
+            const E dy = *(const E*)((const T*)g.dy + l * g.dys + c);
 #pragma unroll
-                for (int i = 0; i < V; i++) d[i] = (float)dy.v[i];
-                if (g.act != AIPT_ACT_NONE) {
-                    E z;
-                    if (V > 1) z = *(const E*)((const T*)g.z + l * g.zs + c);
-                    else z.v[0] = ((const T*)g.z)[(TURNED ? c : l) * g.zi + (TURNED ? l : c) * g.zj];
+            for (int i = 0; i < V; i++) d[i] = (float)dy.v[i];
+            if (g.act != AIPT_ACT_NONE) {
+                E z;
+                if (V > 1) z = *(const E*)((const T*)g.z + l * g.zs + c);
+                else z.v[0] = ((const T*)g.z)[(TURNED ? c : l) * g.zi + (TURNED ? l : c) * g.zj];
 #pragma unroll
-                    for (int i = 0; i < V; i++) d[i] *= act_slope_of((float)z.v[i], g.act, g.slope);
+                for (int i = 0; i < V; i++) d[i] *= act_slope_of((float)z.v[i], g.act, g.slope);
+            }
+        }
+        if (g.dz && c < g.line) {
+            E o;
+#pragma unroll
+            for (int i = 0; i < V; i++) o.v[i] = (T)d[i];
+            *(E*)((T*)g.dz + l * g.dzs + c) = o;
+        }
+    };
+    if constexpr (TURNED) {
+        const int lane = threadIdx.x & 63, l1 = min(g.N, tn * 64 + 64), c0 = tm * g.high, c1 = min(max(g.M, g.line), c0 + g.high);
+        for (int l = tn * 64 + (threadIdx.x >> 6); l < l1; l += 4) {
+            float along = 0;
+#pragma unroll 2
+            for (int c = c0 + lane * V; c < c1; c += 64 * V) {
+                float d[V] = {};
+                one(l, c, g.M, d);
+#pragma unroll
+                for (int i = 0; i < V; i++) along += d[i];
+            }
+            if (g.part || g.sum) {
+                along = wave_sum(along);
+                if (lane == 0) {
+                    if (g.sum) ((T*)g.sum)[l] = (T)along;
+                    else g.part[(long long)tm * g.N + l] = along;
                 }
             }
-            if (g.dz && c < g.line) {
-                E o;
+        }
+    } else {
+        const int x = threadIdx.x % g.across, y = threadIdx.x / g.across, down = 256 / g.across;
+        const int c = (tn * g.across + x) * V, l1 = min(g.M, (tm + 1) * g.high);
+        float sum[V] = {};
+        if (c < max(g.N, g.line)) {
+#pragma unroll 4
+            for (int l = tm * g.high + y; l < l1; l += down) {
+                float d[V] = {};
+                one(l, c, g.N, d);
 #pragma unroll
-                for (int i = 0; i < V; i++) o.v[i] = (T)d[i];
-                *(E*)((T*)g.dz + l * g.dzs + c) = o;
-            }
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                if (TURNED) along += d[i];
-                else sum[i] += d[i];
+                for (int i = 0; i < V; i++) sum[i] += d[i];
             }
         }
-        if (TURNED && g.part) {
-            along = wave_sum(along);
-            if (lane == 0) g.part[(long long)tm * g.N + l] = along;
+        if (!g.part && !g.sum) return;
+#pragma unroll
+        for (int i = 0; i < V; i++) lds[(y * g.across + x) * V + i] = sum[i];
+        __syncthreads();
+        for (int k = threadIdx.x; k < g.across * V; k += 256) {
+            const int n = tn * g.across * V + k;
+            if (n >= g.N) continue;
+            float s = 0;
+            for (int d = 0; d < down; d++) s += lds[d * g.across * V + k];
+            if (g.sum) ((T*)g.sum)[n] = (T)s;
+            else g.part[(long long)tm * g.N + n] = s;
         }
     }
-    if (TURNED || !g.part) return;
-#pragma unroll
-    for (int i = 0; i < V; i++) lds[w][lane * V + i] = sum[i];
-    __syncthreads();
-    for (int c = threadIdx.x; c < 64 * V && c0 + c < g.N; c += 256)
-        g.part[(long long)tm * g.N + c0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
 }
 struct SumArgs {
     const float* part;
@@ -737,16 +829,17 @@ struct Plan {                        // a product as it will be launched, and th
 };
 
 // The sizes of gemm_tile, and what they cost: `start` microseconds for a workgroup's first loads and its results, pair[c] for a pair of its steps
-// while c + 1 workgroups share the CU (16-bit types; floats are bound by the matrix instructions, `wide` a pair).  Measured, bf16, where each
-// wins: 4096 x 4096 x 4096: 256 x 256 104 us, 128 x 128 121; 2048^3: 128 x 128 23, 64 x 64 29, 256 x 256 48; 1024^3: 64 x 64 8.4, 128 x 128
-// 12; 942080 x 32 x 64: 256 x 32 37, 64 x 64 60, 128 x 128 80; 942080 x 64 x 128: 256 x 64 86, 64 x 64 95, 128 x 128 101.
-static const struct Tile { int i, j, fit; double start, pair[3], wide; } TILES[] = {
+// while c + 1 workgroups share the CU, of 16-bit types and of floats (whose matrix instructions bind).  Measured, bf16, where each wins:
+// 4096^3: 256 x 256 101 us, 128 x 128 121; 2048^3: 128 x 128 23, 64 x 64 29, 256 x 256 41; 1024^3: 64 x 64 8.4, 128 x 128 12; 942080 x 32 x 64:
+// 256 x 32 37, 64 x 64 60, 128 x 128 80; 942080 x 64 x 128: 256 x 64 86, 64 x 64 95, 128 x 128 101.  Floats, 2048^3: 256 x 32 137, 64 x 64 140,
+// 128 x 128 142; 942080 x 32 x 64: 256 x 32 93, 256 x 64 and 64 x 64 125.
+static const struct Tile { int i, j, fit; double start, pair[2][3]; } TILES[] = {
     {},
-    {256, 256, 1, 12, {1.4, 0, 0}, 7.6},
-    {128, 128, 2, 4.5, {0.6, 1.0, 0}, 2.0},
-    {64, 64, 3, 2.5, {0.24, 0.36, 0.55}, 0.5},
-    {256, 64, 2, 5.5, {0.8, 1.2, 0}, 2.0},
-    {256, 32, 2, 4, {0.7, 0.9, 0}, 1.0},
+    {256, 256, 1, 12, {{1.4, 0, 0}, {8.0, 0, 0}}},
+    {128, 128, 2, 4.5, {{0.6, 1.0, 0}, {2.1, 3.7, 0}}},
+    {64, 64, 3, 2.5, {{0.26, 0.36, 0.55}, {0.7, 1.1, 1.4}}},
+    {256, 64, 2, 5.5, {{0.8, 1.2, 0}, {2.1, 3.8, 0}}},
+    {256, 32, 2, 4, {{0.7, 0.9, 0}, {1.1, 2.0, 0}}},
 };
 constexpr int NTILES = 6, CUS = 256;
 
@@ -762,7 +855,7 @@ static double pick(bool wide, bool small, long long I, long long J, long long pa
             long long s = fill ? std::min(CUS * fill / std::max(1ll, tiles), pairs / 2) : 1;
             if (s < 1 || (fill && s == 1)) continue;
             const long long n = (pairs + s - 1) / s, blocks = tiles * s, full = blocks / (CUS * c.fit), rest = blocks - full * CUS * c.fit;
-            auto round = [&](int with) { return c.start + n * (wide ? std::max(c.wide * with, c.pair[with - 1]) : c.pair[with - 1]); };
+            auto round = [&](int with) { return c.start + n * c.pair[wide][with - 1]; };
             double us = full * round(c.fit);
             if (rest) us += round((int)((rest + CUS - 1) / CUS));
             if (s > 1) us += 4 + (double)(s + 1) * I * J * 4 / 3.5e6;
@@ -787,12 +880,15 @@ static Plan plan_gemm(int type, View a, View b, long long I, long long J, long l
         return 0;
     };
     int w[2];
+    for (int o = 0; o < 2; o++) w[o] = unit(o ? b : a, (o ? b : a).second ? K : o ? J : I);
     for (int o = 0; o < 2; o++) {
         View& v = o ? b : a;
         const long long rows = o ? J : I, len = v.second ? K : rows, lines = v.second ? rows : K, line = (len + E - 1) / E;
-        w[o] = unit(v, len);
-        if (!w[o] && es == 2 && I && J && K && line * 16 * 256 < (1ll << 31)) {
-            p.pack.m[o] = {(const unsigned short*)v.p, (Chunk<unsigned short>*)p.pack_bytes, v.other, lines * line, (int)len, (int)line};   // (`to`: an offset for now)
+        // copied to lines of 16 bytes: 16-bit lines on less than 4, and a small operand for whose sake the other would go by 4 too
+        const bool small = w[o] != 16 && w[1 - o] == 16 && lines * line * 16 <= std::max(1ll << 20, (o ? I : J) * K * es / 4);
+        if (I && J && K && ((!w[o] && es == 2) || small) && line * 16 * 256 < (1ll << 31)) {
+            const int h = es / 2;                            // halves of an element
+            p.pack.m[o] = {(const unsigned short*)v.p, (Chunk<unsigned short>*)p.pack_bytes, v.other * h, lines * line, (int)len * h, (int)line};   // (`to`: an offset for now)
             p.pack_bytes += up256((size_t)(lines * line) * 16);
             v = {nullptr, v.second ? line * E : 1, v.second ? 1 : line * E, v.second, line * E, true};
             w[o] = 16;
@@ -851,10 +947,13 @@ template <typename T> static void (*gemm_of(const Plan& p))(GemmArgs) {
     }
     return p.ak ? (p.bk ? gemm_any<T, true, true> : gemm_any<T, true, false>) : (p.bk ? gemm_any<T, false, true> : gemm_any<T, false, false>);
 }
-// whether the epilogue may move 16 bytes at a time
-static int rows16(int es, const GemmArgs& g) {
-    const long long e = 16 / es;
-    return !(((uintptr_t)g.c | (uintptr_t)g.res | (uintptr_t)g.pre) & 15) && g.cs % e == 0 && (!g.res || (g.rj == 1 && g.ri % e == 0)) && (!g.pre || (g.pj == 1 && g.pi % e == 0));
+// how many elements the epilogue may move together
+static int row_unit(int es, const GemmArgs& g) {
+    auto on = [&](int bytes) {
+        const long long e = bytes / es;
+        return !(((uintptr_t)g.c | (uintptr_t)g.res | (uintptr_t)g.pre) & (bytes - 1)) && g.cs % e == 0 && (!g.res || (g.rj == 1 && g.ri % e == 0)) && (!g.pre || (g.pj == 1 && g.pi % e == 0));
+    };
+    return on(16) ? 8 : g.J % 2 == 0 && on(2 * es) ? 2 : 1;
 }
 
 template <typename T> static hipError_t run_gemm_t(hipStream_t st, Plan& p, void* ws) {
@@ -869,10 +968,13 @@ template <typename T> static hipError_t run_gemm_t(hipStream_t st, Plan& p, void
         if (e != hipSuccess) return e;
     }
     p.g.partial = (float*)((char*)ws + p.pack_bytes);
-    p.g.c16 = rows16(sizeof(T), p.g);
+    p.g.cv = row_unit(sizeof(T), p.g);
     hipError_t e = launch(gemm_of<T>(p), p.blocks, 256, 0, st, p.g);
     if (e == hipSuccess && p.g.splits > 1)
-        e = launch(gemm_join<T>, std::min<size_t>(((size_t)p.g.I * ((p.g.J + 3) / 4) + 255) / 256, 4096), 256, 0, st, p.g);
+    {
+        const size_t quads = (size_t)p.g.I * ((p.g.J + 3) / 4);
+        e = p.g.splits > 8 ? launch(gemm_join<T, 16>, std::min<size_t>((quads + 15) / 16, 8192), 256, 0, st, p.g) : launch(gemm_join<T, 1>, std::min<size_t>((quads + 255) / 256, 4096), 256, 0, st, p.g);
+    }
     return e;
 }
 static hipError_t run_gemm(int type, hipStream_t st, Plan& p, void* ws) {
@@ -917,10 +1019,6 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         p.dz.line = (int)ld;
         d = {ws, dy.second ? ld : 1, dy.second ? 1 : ld, dy.second, ld, true};
     }
-    // 64 rows a workgroup, or so many that there are at most 1 024 partial sums a column
-    const long long high = std::max(1ll, ((a->m + 1023) / 1024 + 63) / 64) * 64, tm = (a->m + high - 1) / high;
-    p.parts = (int)tm;
-    if (p.want_db) p.part_bytes = up256((size_t)tm * a->n * sizeof(float));
     if (p.make_dz || p.want_db) {
         DzArgs& g = p.dz;
         const bool turned = !dy.second;
@@ -928,12 +1026,22 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         const bool z_same = a->act == AIPT_ACT_NONE || (z.second == dy.second && !((uintptr_t)z.p & 15) && zline % E == 0);
         p.dz_vec = !((uintptr_t)dy.p & 15) && dy.other % E == 0 && len % E == 0 && z_same;
         p.dz_turned = turned;
+        const long long wide = std::max<long long>(a->n, turned ? 0 : g.line), v = p.dz_vec ? E : 1;
+        g.across = 4;
+        while (g.across < 256 && g.across * v < wide) g.across *= 2;
+        g.tiles_n = (int)(turned ? (a->n + 63) / 64 : (wide + g.across * v - 1) / (g.across * v));
+        // some 2 048 workgroups, each with 4 rows a thread at least, and no more than 1 024 partial sums a column
+        const long long unit = turned ? 64 * v : 256 / g.across, fair = (a->m * g.tiles_n + 2047) / 2048;
+        const long long high = (std::max({4 * unit, fair, (a->m + 1023) / 1024}) + unit - 1) / unit * unit;
+        const long long tm = (a->m + high - 1) / high;
+        g.high = (int)std::min(high, 0x40000000ll);
+        p.parts = (int)tm;
+        if (p.want_db && tm > 1) p.part_bytes = up256((size_t)tm * a->n * sizeof(float));
         g.dy = a->dy.data; g.z = a->preact.data; g.dz = p.make_dz ? d.p : nullptr;
-        g.part = p.want_db ? (float*)(ws + p.dz_bytes) : nullptr;
+        g.part = p.want_db && tm > 1 ? (float*)(ws + p.dz_bytes) : nullptr;
+        g.sum = p.want_db && tm == 1 ? a->dbias : nullptr;
         g.dys = dy.other; g.zs = zline; g.zi = z.ri; g.zj = z.rj; g.dzs = d.other;
-        g.M = (int)a->m; g.N = (int)a->n; g.high = (int)high;
-        const long long wide = turned ? 64 : 64 * (p.dz_vec ? E : 1);
-        g.tiles_n = (int)((std::max<long long>(a->n, turned ? 0 : g.line) + wide - 1) / wide);
+        g.M = (int)a->m; g.N = (int)a->n;
         g.act = a->act; g.slope = a->slope;
         p.dz_blocks = (size_t)tm * g.tiles_n;
     }
@@ -1074,9 +1182,9 @@ int aipt_linear_backward(aipt_ctx* ctx, const aipt_linear_grad_args* a, void* d_
     if (p.dz_blocks)
         AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::dz_kernel<float>(p) : t == AIPT_TYPE_BF16 ? aipt::dz_kernel<aipt::bf16>(p) : aipt::dz_kernel<aipt::f16>(p), p.dz_blocks, 256, 0, st, p.dz));
     if (p.want_db) {
-        if (a->m) AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::sum_parts<float> : t == AIPT_TYPE_BF16 ? aipt::sum_parts<aipt::bf16> : aipt::sum_parts<aipt::f16>, (size_t)((a->n + 63) / 64), 1024, 0, st,
+        if (p.parts > 1) AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::sum_parts<float> : t == AIPT_TYPE_BF16 ? aipt::sum_parts<aipt::bf16> : aipt::sum_parts<aipt::f16>, (size_t)((a->n + 63) / 64), 1024, 0, st,
                                              aipt::SumArgs{p.dz.part, a->dbias, p.parts, (int)a->n}));
-        else AIPT_HIP(ctx, aipt::zero_fill(st, a->dbias, (size_t)a->n * es));
+        else if (!a->m) AIPT_HIP(ctx, aipt::zero_fill(st, a->dbias, (size_t)a->n * es));
     }
     char* gemm_ws = (char*)d_workspace + p.dz_bytes + p.part_bytes;
     if (p.want_dx) AIPT_HIP(ctx, aipt::run_gemm(t, st, p.dx, gemm_ws));
