@@ -653,15 +653,15 @@ __global__ __launch_bounds__(256) void pack_lines(const PackArgs g) {
     }
 }
 
-// ---- dz = dy * act'(z), rounded to the element type, and its sums over rows: dy is read once for both.  V elements (16 bytes) a lane where lines
-// lie on 16 bytes, else one.  A workgroup takes `high` rows; `across` lanes (a power of two) share a row, so that narrow rows too fill a
+// ---- dz = dy * act'(z), rounded to the element type, and its sums over rows: dy is read once for both.  V elements a lane: 16 bytes where lines
+// lie on 16 bytes, two where they lie on two, else one.  A workgroup takes `high` rows; `across` lanes (a power of two) share a row, so that narrow rows too fill a
 // wave, and a lane's columns stay its own.  Where rows are the contiguous axis (TURNED): 64 lines (columns) of `high` rows, a wave each.
 struct DzArgs {
     const void *dy, *z;
     void* dz;
     float* part;                     // [ceil(M / high)][N] sums over a workgroup's rows, or NULL
     void* sum;                       // ... or, where one workgroup has all rows, the sums themselves
-    long long dys, zs, zi, zj, dzs;  // strides from line to line (and both of z's, which may lie the other way)
+    long long dys, zi, zj, dzs;      // strides from line to line, and both of z's, which may lie the other way
     int M, N;                        // rows and columns of dy
     int line;                        // dz's lines, with their padding (of zeros)
     int high, tiles_n, across, act;
@@ -669,37 +669,39 @@ struct DzArgs {
 };
 template <typename T, int V, bool TURNED>
 __global__ __launch_bounds__(256) void act_backward(const DzArgs g) {
-    struct alignas(V == 1 ? sizeof(T) : 16) E { T v[V]; };
+    struct alignas(V * sizeof(T)) E { T v[V]; };
     __shared__ float lds[TURNED ? 1 : 256 * V];
     const int tm = (int)(blockIdx.x / g.tiles_n), tn = (int)(blockIdx.x % g.tiles_n);
-    auto one = [&](int l, int c, int len, float* d) {         // elements c .. of line l
-        if (c < len) {                                       // (V > 1: len is whole loads)
-            const E dy = *(const E*)((const T*)g.dy + l * g.dys + c);
+    // V elements: in [is there an element], out [is there one of dz, padding included]
+    auto one = [&](const T* dyp, const T* zp, T* dzp, bool in, bool out, float* d) {
+        if (in) {
+            const E dy = *(const E*)dyp;
 #pragma unroll
             for (int i = 0; i < V; i++) d[i] = (float)dy.v[i];
             if (g.act != AIPT_ACT_NONE) {
-                E z;
-                if (V > 1) z = *(const E*)((const T*)g.z + l * g.zs + c);
-                else z.v[0] = ((const T*)g.z)[(TURNED ? c : l) * g.zi + (TURNED ? l : c) * g.zj];
+                const E z = *(const E*)zp;
 #pragma unroll
                 for (int i = 0; i < V; i++) d[i] *= act_slope_of((float)z.v[i], g.act, g.slope);
             }
         }
-        if (g.dz && c < g.line) {
+        if (out) {
             E o;
 #pragma unroll
             for (int i = 0; i < V; i++) o.v[i] = (T)d[i];
-            *(E*)((T*)g.dz + l * g.dzs + c) = o;
+            *(E*)dzp = o;
         }
     };
     if constexpr (TURNED) {
         const int lane = threadIdx.x & 63, l1 = min(g.N, tn * 64 + 64), c0 = tm * g.high, c1 = min(max(g.M, g.line), c0 + g.high);
         for (int l = tn * 64 + (threadIdx.x >> 6); l < l1; l += 4) {
+            const T* dyp = (const T*)g.dy + l * g.dys;
+            const T* zp = (const T*)g.z + l * g.zj;
+            T* dzp = (T*)g.dz + l * g.dzs;
             float along = 0;
 #pragma unroll 2
             for (int c = c0 + lane * V; c < c1; c += 64 * V) {
                 float d[V] = {};
-                one(l, c, g.M, d);
+                one(dyp + c, zp + c * g.zi, dzp + c, c < g.M, g.dz && c < g.line, d);
 #pragma unroll
                 for (int i = 0; i < V; i++) along += d[i];
             }
@@ -713,15 +715,45 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g) {
         }
     } else {
         const int x = threadIdx.x % g.across, y = threadIdx.x / g.across, down = 256 / g.across;
-        const int c = (tn * g.across + x) * V, l1 = min(g.M, (tm + 1) * g.high);
+        const int c = (tn * g.across + x) * V, l0 = tm * g.high + y, l1 = min(g.M, (tm + 1) * g.high);
         float sum[V] = {};
         if (c < max(g.N, g.line)) {
-#pragma unroll 4
-            for (int l = tm * g.high + y; l < l1; l += down) {
-                float d[V] = {};
-                one(l, c, g.N, d);
+            const T* dyp = (const T*)g.dy + l0 * g.dys + c;
+            const T* zp = (const T*)g.z + l0 * g.zi + c * g.zj;
+            T* dzp = (T*)g.dz + l0 * g.dzs + c;
+            const long long dyd = down * g.dys, zd = down * g.zi, dzd = down * g.dzs;
+            const bool in = c < g.N, out = g.dz && c < g.line;
+            // U rows' loads before the first one's result (which might, for all the compiler knows, be what the next row reads)
+            constexpr int U = V * sizeof(T) == 16 ? 2 : 4;
+            for (int l = l0; l < l1; l += U * down) {
+                E dy[U], z[U];
 #pragma unroll
-                for (int i = 0; i < V; i++) sum[i] += d[i];
+                for (int u = 0; u < U; u++) {
+                    if (in && l + u * down < l1) {
+                        dy[u] = *(const E*)(dyp + u * dyd);
+                        if (g.act != AIPT_ACT_NONE) z[u] = *(const E*)(zp + u * zd);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (l + u * down >= l1) break;
+                    float d[V] = {};
+                    if (in) {
+#pragma unroll
+                        for (int i = 0; i < V; i++) {
+                            d[i] = (float)dy[u].v[i];
+                            if (g.act != AIPT_ACT_NONE) d[i] *= act_slope_of((float)z[u].v[i], g.act, g.slope);
+                            sum[i] += d[i];
+                        }
+                    }
+                    if (out) {
+                        E o;
+#pragma unroll
+                        for (int i = 0; i < V; i++) o.v[i] = (T)d[i];
+                        *(E*)(dzp + u * dzd) = o;
+                    }
+                }
+                dyp += U * dyd; zp += U * zd; dzp += U * dzd;
             }
         }
         if (!g.part && !g.sum) return;
@@ -999,7 +1031,8 @@ struct GradPlan {
     Plan dx, dw;
     DzArgs dz = {};
     bool want_dx = false, want_dw = false, want_db = false, make_dz = false;
-    bool dz_vec = false, dz_turned = false;
+    bool dz_turned = false;
+    int dz_v = 1;
     int parts = 0;
     size_t dz_bytes = 0, part_bytes = 0, gemm_bytes = 0, dz_blocks = 0;
     size_t bytes() const { return dz_bytes + part_bytes + gemm_bytes; }
@@ -1023,10 +1056,13 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         DzArgs& g = p.dz;
         const bool turned = !dy.second;
         const long long len = turned ? a->m : a->n, zline = turned ? z.rj : z.ri;
-        const bool z_same = a->act == AIPT_ACT_NONE || (z.second == dy.second && !((uintptr_t)z.p & 15) && zline % E == 0);
-        p.dz_vec = !((uintptr_t)dy.p & 15) && dy.other % E == 0 && len % E == 0 && z_same;
         p.dz_turned = turned;
-        const long long wide = std::max<long long>(a->n, turned ? 0 : g.line), v = p.dz_vec ? E : 1;
+        p.dz_v = 1;
+        for (int v : {2, E}) {
+            const bool z_same = a->act == AIPT_ACT_NONE || (z.second == dy.second && !((uintptr_t)z.p & (v * es - 1)) && zline % v == 0);
+            if (!((uintptr_t)dy.p & (v * es - 1)) && dy.other % v == 0 && len % v == 0 && z_same) p.dz_v = v;
+        }
+        const long long wide = std::max<long long>(a->n, turned ? 0 : g.line), v = p.dz_v;
         g.across = 4;
         while (g.across < 256 && g.across * v < wide) g.across *= 2;
         g.tiles_n = (int)(turned ? (a->n + 63) / 64 : (wide + g.across * v - 1) / (g.across * v));
@@ -1040,7 +1076,7 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         g.dy = a->dy.data; g.z = a->preact.data; g.dz = p.make_dz ? d.p : nullptr;
         g.part = p.want_db && tm > 1 ? (float*)(ws + p.dz_bytes) : nullptr;
         g.sum = p.want_db && tm == 1 ? a->dbias : nullptr;
-        g.dys = dy.other; g.zs = zline; g.zi = z.ri; g.zj = z.rj; g.dzs = d.other;
+        g.dys = dy.other; g.zi = z.ri; g.zj = z.rj; g.dzs = d.other;
         g.M = (int)a->m; g.N = (int)a->n;
         g.act = a->act; g.slope = a->slope;
         p.dz_blocks = (size_t)tm * g.tiles_n;
@@ -1062,7 +1098,9 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
 
 template <typename T> static void (*dz_kernel(const GradPlan& p))(DzArgs) {
     constexpr int V = 16 / sizeof(T);
-    return p.dz_vec ? (p.dz_turned ? act_backward<T, V, true> : act_backward<T, V, false>) : (p.dz_turned ? act_backward<T, 1, true> : act_backward<T, 1, false>);
+    if (p.dz_v == V) return p.dz_turned ? act_backward<T, V, true> : act_backward<T, V, false>;
+    if (p.dz_v == 2) return p.dz_turned ? act_backward<T, 2, true> : act_backward<T, 2, false>;
+    return p.dz_turned ? act_backward<T, 1, true> : act_backward<T, 1, false>;
 }
 
 static int linear_check(aipt_ctx* ctx, const char* me, int type, int act, float slope, int reserved, long long m, long long n, long long k) {
