@@ -25,24 +25,35 @@ struct NormFwd {
     float eps;
 };
 
-// V elements from p: one 16-byte load, or one element
+// V elements by one load: 16 bytes, two 16-bit elements, or one element
+template <typename T, int V> struct alignas(V * sizeof(T)) Few { T v[V]; };
 template <typename T, int V> __device__ inline void get(const void* base, long long at, float* o) {
-    if constexpr (V == 1) o[0] = (float)((const T*)base)[at];
-    else {
-        const Chunk<T> q = *(const Chunk<T>*)((const T*)base + at);
+    const Few<T, V> q = *(const Few<T, V>*)((const T*)base + at);
 #pragma unroll
-        for (int i = 0; i < V; i++) o[i] = (float)q.v[i];
-    }
+    for (int i = 0; i < V; i++) o[i] = (float)q.v[i];
 }
 template <typename T, int V> __device__ inline void put(void* base, long long at, const float* v) {
-    if constexpr (V == 1) ((T*)base)[at] = (T)v[0];
-    else {
-        Chunk<T> q;
+    Few<T, V> q;
 #pragma unroll
-        for (int i = 0; i < V; i++) q.v[i] = (T)v[i];
-        *(Chunk<T>*)((T*)base + at) = q;
-    }
+    for (int i = 0; i < V; i++) q.v[i] = (T)v[i];
+    *(Few<T, V>*)((T*)base + at) = q;
 }
+
+// One row in registers as it lies in memory.
+template <typename T, int V, int N> struct RawRow {
+    Few<T, V> e[N];
+    template <int LANES> __device__ inline void load(const void* base, long long at, int lane, int c) {
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int col = (n * LANES + lane) * V;
+            if (col < c) e[n] = *(const Few<T, V>*)((const T*)base + at + col);
+            else {
+#pragma unroll
+                for (int i = 0; i < V; i++) e[n].v[i] = (T)0.f;
+            }
+        }
+    }
+};
 
 // two sums over the LANES lanes that share a row, the same values in each.  More than a wave: through LDS, `buf` used in turn so that one
 // barrier an exchange is enough (a wave can be at most one exchange ahead of another).
@@ -50,9 +61,9 @@ template <int LANES> struct RowSum {
     float2* lds;
     int turn = 0;
     __device__ void operator()(float& a, float& b) {
-        if constexpr (LANES == 16) {
-            a = sum16(a);
-            b = sum16(b);
+        if constexpr (LANES <= 16) {
+            a = LANES == 4 ? sum4(a) : sum16(a);
+            b = LANES == 4 ? sum4(b) : sum16(b);
             return;
         }
         a = wave_sum(a);
@@ -70,35 +81,92 @@ template <int LANES> struct RowSum {
     }
 };
 
+// A workgroup goes through rows, ROWS at a time, LANES lanes a row.  With up to 16 columns a lane (8 in a workgroup of 1 024, which has half the
+// registers), what multiplies and adds to a column (scale * gate * w1, scale * gate * b1, w2, b2) stays in registers until the gate changes, and
+// the next row's loads go out before this one's sums are waited for: 74 400 x 902 fp16 457 -> 111 us (106 at the rate of a copy), where the six
+// vectors were read again for each row in accesses as narrow as the rows'; 16 384 x 4 096 bf16 114 -> 101 us.
 template <typename T, int V, int N, int LANES>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_fwd(const NormFwd a) {
     constexpr int THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;
+    constexpr bool KEEP = N * V <= (LANES == 1024 ? 8 : 16);
     __shared__ float2 lds[2 * (THREADS / 64)];
     RowSum<LANES> row_sum{lds};
     const int lane = threadIdx.x % LANES;
     const float inv_c = 1.f / (float)a.c;
-    for (long long r = (long long)blockIdx.x * ROWS + threadIdx.x / LANES; r < a.rows; r += (long long)gridDim.x * ROWS) {
-        float v[N][V];
-        float mean_y = 0, rstd_y = 0;
-        if (a.y) {
-            float s = 0, none = 0;
+    const long long step = (long long)gridDim.x * ROWS;
+    long long r = (long long)blockIdx.x * ROWS + threadIdx.x / LANES, gate_end = 0, gate_row = 0;
+    float k1[KEEP ? N : 1][V], k0[KEEP ? N : 1][V], k3[KEEP ? N : 1][V], k2[KEEP ? N : 1][V];
+    auto fill = [&](float* o, float v) {
 #pragma unroll
-            for (int n = 0; n < N; n++) {
-                const int col = (n * LANES + lane) * V;
-                if (col < a.c) get<T, V>(a.y, r * a.ys + col, v[n]);
-                else {
+        for (int i = 0; i < V; i++) o[i] = v;
+    };
+    auto times = [&](float* o, const void* p, long long at) {
+        if (!p) return;
+        float q[V];
+        get<T, V>(p, at, q);
 #pragma unroll
-                    for (int i = 0; i < V; i++) v[n][i] = 0;
-                }
+        for (int i = 0; i < V; i++) o[i] *= q[i];
+    };
+    // u = k1 yhat + k0, scale and gate included
+    auto factors = [&](int col, float* w, float* b) {
+        float g[V];
+        fill(g, 1);
+        fill(w, 1);
+        fill(b, 0);
+        if (col >= a.c) return;
+        times(g, a.gate, gate_row + col);
+        times(g, a.scale, col);
+        times(w, a.w1, col);
+        if (a.b1) get<T, V>(a.b1, col, b);
 #pragma unroll
-                for (int i = 0; i < V; i++) s += v[n][i];
+        for (int i = 0; i < V; i++) { w[i] *= g[i]; b[i] *= g[i]; }
+    };
+    auto factors2 = [&](int col, float* w, float* b) {
+        fill(w, 1);
+        fill(b, 0);
+        if (col >= a.c) return;
+        times(w, a.w2, col);
+        if (a.b2) get<T, V>(a.b2, col, b);
+    };
+    if constexpr (KEEP) {
+        if (a.z) {
+#pragma unroll
+            for (int n = 0; n < N; n++) factors2((n * LANES + lane) * V, k3[n], k2[n]);
+        }
+    }
+    RawRow<T, V, N> y, x;
+    auto load = [&](long long r) {
+        if (a.y) y.template load<LANES>(a.y, r * a.ys, lane, a.c);
+        x.template load<LANES>(a.x, r * a.xs, lane, a.c);
+    };
+    if (KEEP && r < a.rows) load(r);
+    for (; r < a.rows; r += step) {
+        if constexpr (!KEEP) load(r);
+        const RawRow<T, V, N> yc = y, xc = x;
+        if (KEEP && r + step < a.rows) load(r + step);
+        if (a.y && r >= gate_end) {
+            if (a.gate) {
+                const long long g = r / a.per_gate;
+                gate_row = g * a.c;
+                gate_end = (g + 1) * a.per_gate;
+            } else gate_end = a.rows;
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int n = 0; n < N; n++) factors((n * LANES + lane) * V, k1[n], k0[n]);
             }
+        }
+        float v[N][V];
+        float mean_y = 0, rstd_y = 0, s = 0, none = 0;
+        if (a.y) {
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int i = 0; i < V; i++) { v[n][i] = (float)yc.e[n].v[i]; s += v[n][i]; }
             if (a.layer) { row_sum(s, none); mean_y = s * inv_c; }
             s = 0;
 #pragma unroll
             for (int n = 0; n < N; n++) {
-                const int col = (n * LANES + lane) * V;
-                if (col < a.c) {
+                if ((n * LANES + lane) * V < a.c) {
 #pragma unroll
                     for (int i = 0; i < V; i++) { v[n][i] -= mean_y; s += v[n][i] * v[n][i]; }
                 }
@@ -106,36 +174,22 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_fwd(cons
             row_sum(s, none);
             rstd_y = 1.f / sqrtf(s * inv_c + a.eps);
         }
-        const long long gate_row = a.gate ? r / a.per_gate * a.c : 0;
-        float s = 0, none = 0;
+        s = 0;
 #pragma unroll
         for (int n = 0; n < N; n++) {
             const int col = (n * LANES + lane) * V;
-            if (col < a.c) {
-                float h[V], q[V];
-                get<T, V>(a.x, r * a.xs + col, h);
-                if (a.y) {
+            float h[V];
 #pragma unroll
-                    for (int i = 0; i < V; i++) v[n][i] *= rstd_y;
-                    if (a.w1) { get<T, V>(a.w1, col, q);
+            for (int i = 0; i < V; i++) h[i] = (float)xc.e[n].v[i];
+            if (a.y && col < a.c) {
+                float w[V], b[V];
+                if constexpr (!KEEP) factors(col, w, b);
 #pragma unroll
-                        for (int i = 0; i < V; i++) v[n][i] *= q[i]; }
-                    if (a.b1) { get<T, V>(a.b1, col, q);
-#pragma unroll
-                        for (int i = 0; i < V; i++) v[n][i] += q[i]; }
-                    if (a.gate) { get<T, V>(a.gate, gate_row + col, q);
-#pragma unroll
-                        for (int i = 0; i < V; i++) v[n][i] *= q[i]; }
-                    if (a.scale) { get<T, V>(a.scale, col, q);
-#pragma unroll
-                        for (int i = 0; i < V; i++) v[n][i] *= q[i]; }
-#pragma unroll
-                    for (int i = 0; i < V; i++) h[i] += v[n][i];
-                }
-                put<T, V>(a.h, r * a.hs + col, h);
-#pragma unroll
-                for (int i = 0; i < V; i++) { v[n][i] = h[i]; s += h[i]; }
+                for (int i = 0; i < V; i++) h[i] += v[n][i] * rstd_y * (KEEP ? k1[KEEP ? n : 0][i] : w[i]) + (KEEP ? k0[KEEP ? n : 0][i] : b[i]);
             }
+            if (col < a.c) put<T, V>(a.h, r * a.hs + col, h);
+#pragma unroll
+            for (int i = 0; i < V; i++) { v[n][i] = h[i]; s += h[i]; }
         }
         float mean_h = 0, rstd_h = 0;
         if (a.z) {
@@ -143,8 +197,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_fwd(cons
             s = 0;
 #pragma unroll
             for (int n = 0; n < N; n++) {
-                const int col = (n * LANES + lane) * V;
-                if (col < a.c) {
+                if ((n * LANES + lane) * V < a.c) {
 #pragma unroll
                     for (int i = 0; i < V; i++) { v[n][i] -= mean_h; s += v[n][i] * v[n][i]; }
                 }
@@ -155,15 +208,10 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_fwd(cons
             for (int n = 0; n < N; n++) {
                 const int col = (n * LANES + lane) * V;
                 if (col < a.c) {
-                    float q[V];
+                    float w[V], b[V];
+                    if constexpr (!KEEP) factors2(col, w, b);
 #pragma unroll
-                    for (int i = 0; i < V; i++) v[n][i] *= rstd_h;
-                    if (a.w2) { get<T, V>(a.w2, col, q);
-#pragma unroll
-                        for (int i = 0; i < V; i++) v[n][i] *= q[i]; }
-                    if (a.b2) { get<T, V>(a.b2, col, q);
-#pragma unroll
-                        for (int i = 0; i < V; i++) v[n][i] += q[i]; }
+                    for (int i = 0; i < V; i++) v[n][i] = v[n][i] * rstd_h * (KEEP ? k3[KEEP ? n : 0][i] : w[i]) + (KEEP ? k2[KEEP ? n : 0][i] : b[i]);
                     put<T, V>(a.z, r * a.zs + col, v[n]);
                 }
             }
@@ -183,29 +231,13 @@ struct NormBwd {
     int c;
 };
 
-// One row in registers as it lies in memory.
-template <typename T, int V, int N> struct RawRow {
-    struct alignas(V == 1 ? sizeof(T) : 16) E { T v[V]; } e[N];
-    template <int LANES> __device__ inline void load(const void* base, long long at, int lane, int c) {
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            const int col = (n * LANES + lane) * V;
-            if (col < c) e[n] = *(const E*)((const T*)base + at + col);
-            else {
-#pragma unroll
-                for (int i = 0; i < V; i++) e[n].v[i] = (T)0.f;
-            }
-        }
-    }
-};
-
-// A workgroup is a part: ROWS rows at a time, LANES lanes a row.  The next row's loads go out before this one's sums are waited for (rows of few
-// registers; with 4 096 floats a row there is no room).  WHOLE: gates change within the part -- A and B are added up gate by gate; else the
+// A workgroup is a part: ROWS rows at a time, LANES lanes a row.  The vectors stay in registers (KEEP) and the next row's loads go out before this one's
+// sums are waited for (AHEAD) where there are registers for it beside the four sums a column.  WHOLE: gates change within the part -- A and B are added up gate by gate; else the
 // gate is one number a column and P = sum t yhat, T = sum t give A, B and Q at the end.
 template <typename T, int V, int N, int LANES, bool LAYER, bool WHOLE>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_bwd(const NormBwd a) {
     constexpr int THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;
-    constexpr bool AHEAD = !WHOLE && N * V * sizeof(T) <= 32 && LANES <= 512, KEEP = !WHOLE && N * V <= 16 && LANES <= 512;
+    constexpr bool AHEAD = !WHOLE && N * V * sizeof(T) <= 32 && N <= 8 && LANES <= 512, KEEP = !WHOLE && (LANES <= 512 ? N * V <= 16 : N * V * (LAYER ? 12 : 9) <= 80);
     __shared__ float2 lds[2 * (THREADS / 64)];
     __shared__ float sums[LANES < 256 ? THREADS * V * N : 1];
     RowSum<LANES> row_sum{lds};
@@ -436,7 +468,8 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_bwd(cons
     }
 }
 
-// The vectors' gradients from the parts, added in a fixed order by 64 columns x 16 lanes of parts.  Job 0: of post_*, 1: of pre_*, 2 + j: dgate's row j.
+// The vectors' gradients from the parts, added in a fixed order by 32 columns x 32 lanes of parts (64 x 16 where
+// rows are long: whole lines).  Job 0: of post_*, 1: of pre_*, 2 + j: dgate's row j.
 struct NormEnd {
     const float* part;
     const void *scale, *w1, *b1;
@@ -444,12 +477,13 @@ struct NormEnd {
     long long parts, parts_per_gate;
     int c, col_blocks, layer, post, pre;
 };
-template <typename T>
+template <typename T, int COLS>
 __global__ __launch_bounds__(1024) void block_norm_end(const NormEnd a) {
-    __shared__ float lds[2][16][64];
+    constexpr int LANES = 1024 / COLS;
+    __shared__ float lds[2][LANES][COLS];
     const int cb = blockIdx.x % a.col_blocks;
     const long long job = blockIdx.x / a.col_blocks;
-    const int k = threadIdx.x >> 6, lane = threadIdx.x & 63, col = cb * 64 + lane;
+    const int k = threadIdx.x / COLS, lane = threadIdx.x % COLS, col = cb * COLS + lane;
     if ((job == 0 && !a.post) || (job == 1 && !a.pre)) return;
     const long long p0 = job > 1 ? (job - 2) * a.parts_per_gate : 0, p1 = job > 1 ? p0 + a.parts_per_gate : a.parts;
     const int first = job > 1 ? 4 : (int)job * 2;
@@ -458,11 +492,12 @@ __global__ __launch_bounds__(1024) void block_norm_end(const NormEnd a) {
     if (col < a.c) {
         const float* q = a.part + first * (long long)a.c + col;
         const long long step = 5 * (long long)a.c;
-#pragma unroll 8
-        for (long long p = p0 + k; p < p1; p += 16) s0 += q[p * step];
         if (two) {
 #pragma unroll 8
-            for (long long p = p0 + k; p < p1; p += 16) s1 += q[p * step + a.c];
+            for (long long p = p0 + k; p < p1; p += LANES) { s0 += q[p * step]; s1 += q[p * step + a.c]; }
+        } else {
+#pragma unroll 8
+            for (long long p = p0 + k; p < p1; p += LANES) s0 += q[p * step];
         }
     }
     lds[0][k][lane] = s0;
@@ -471,7 +506,7 @@ __global__ __launch_bounds__(1024) void block_norm_end(const NormEnd a) {
     if (k || col >= a.c) return;
     s0 = s1 = 0;
 #pragma unroll
-    for (int i = 0; i < 16; i++) { s0 += lds[0][i][lane]; s1 += lds[1][i][lane]; }
+    for (int i = 0; i < LANES; i++) { s0 += lds[0][i][lane]; s1 += lds[1][i][lane]; }
     const float sc = a.scale ? (float)((const T*)a.scale)[col] : 1.f;
     if (job > 1) {
         ((T*)a.dgate)[(job - 2) * a.c + col] = (T)(s0 * sc);
@@ -488,46 +523,58 @@ __global__ __launch_bounds__(1024) void block_norm_end(const NormEnd a) {
     if (a.db1) ((T*)a.db1)[col] = (T)(sc * s1);
 }
 
+template <typename T> static void (*end_kernel(int cols))(NormEnd) { return cols == 32 ? block_norm_end<T, 32> : block_norm_end<T, 64>; }
+
 static_assert(sizeof(aipt_block_norm_args) == 152 && sizeof(aipt_block_norm_grad_args) == 224, "argument records (api.py packs them by field)");
 
-// ---- which kernel: the fewest lanes that hold a row, 16-byte accesses where every row begins at 16 bytes
+// ---- which kernel: the fewest lanes that hold a row; 16-byte accesses where every row begins at 16 bytes, two 16-bit elements where at 4 (74 400 rows of
+// 902 fp16: 111 us by twos; of 901 one by one: 166).  Up to 8 or 16 columns a lane, so that the vectors stay in registers: 4 lanes for 32 columns of 16
+// bits rather than 16 (65 964 rows: 13 -> 7 us, backward 25 -> 15), 256 for 2 048 rather than 64 with 32 columns each (16 384 rows: 92 -> 55), 512 for
+// 8 192 rather than 256 (8 192 rows: 237 -> 120), 256 for 999 fp16 by ones in the backward pass rather than 64 (20 000 rows: 187 -> 75).
 struct NormShape { int v, n, lanes; };
 template <int S> static NormShape norm_shape(int c, int v, const int (&shapes)[S][2]) {
     for (auto& s : shapes) if (s[0] * s[1] * v >= c) return {v, s[1], s[0]};
     return {0, 0, 0};
 }
-static NormShape fwd_shape(int es, int c, bool wide) {
-    static const int wides[][2] = {{16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}},
-                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}};
-    return wide ? norm_shape(c, 16 / es, wides) : norm_shape(c, 1, ones);
+static NormShape fwd_shape(int es, int c, int v) {
+    static const int w8[][2] = {{4, 1}, {16, 1}, {16, 2}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}},
+                     w4[][2] = {{4, 1}, {16, 1}, {16, 2}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}},
+                     twos[][2] = {{16, 2}, {16, 4}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}},
+                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 4}, {64, 8}, {256, 4}, {256, 8}, {512, 8}, {1024, 6}, {1024, 8}, {1024, 16}};
+    return v == 1 ? norm_shape(c, 1, ones) : v == 8 ? norm_shape(c, 8, w8) : v == 4 ? norm_shape(c, 4, w4) : norm_shape(c, 2, twos);
 }
-static NormShape bwd_shape(int es, int c, bool wide, bool whole) {
-    static const int w2[][2] = {{16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}}, w4[][2] = {{16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}},
-                     ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 8}, {256, 8}, {512, 8}, {1024, 8}, {1024, 16}};
-    static const int g2[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 2}}, g4[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 4}}, gones[][2] = {{16, 4}, {64, 8}, {256, 8}, {1024, 8}, {1024, 16}};
-    if (whole) return !wide ? norm_shape(c, 1, gones) : es == 2 ? norm_shape(c, 8, g2) : norm_shape(c, 4, g4);
-    return !wide ? norm_shape(c, 1, ones) : es == 2 ? norm_shape(c, 8, w2) : norm_shape(c, 4, w4);
+static NormShape bwd_shape(int es, int c, int v, bool whole) {
+    static const int w8[][2] = {{4, 1}, {16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {512, 2}, {1024, 2}}, w4[][2] = {{4, 1}, {16, 1}, {16, 2}, {64, 2}, {256, 1}, {256, 2}, {256, 4}, {512, 4}, {1024, 4}},
+                     twos[][2] = {{16, 2}, {16, 4}, {64, 4}, {256, 2}, {256, 4}, {256, 8}, {512, 8}, {1024, 8}}, ones[][2] = {{16, 2}, {16, 4}, {16, 8}, {64, 8}, {256, 4}, {256, 8}, {512, 8}, {1024, 6}, {512, 16}, {1024, 16}};
+    static const int g8[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 2}}, g4[][2] = {{16, 1}, {64, 2}, {256, 2}, {1024, 4}}, gones[][2] = {{16, 4}, {64, 8}, {256, 8}, {1024, 8}, {1024, 16}};
+    if (whole) return v != 16 / es ? norm_shape(c, 1, gones) : es == 2 ? norm_shape(c, 8, g8) : norm_shape(c, 4, g4);
+    return v == 1 ? norm_shape(c, 1, ones) : v != 16 / es ? norm_shape(c, 2, twos) : es == 2 ? norm_shape(c, 8, w8) : norm_shape(c, 4, w4);
 }
 
 template <typename T> static void (*fwd_kernel(NormShape s))(NormFwd) {
     constexpr int V = 16 / sizeof(T);
 #define AIPT_FWD(VV, NN, LL) if (s.v == VV && s.n == NN && s.lanes == LL) return block_norm_fwd<T, VV, NN, LL>;
-    AIPT_FWD(V, 1, 16) AIPT_FWD(V, 2, 16) AIPT_FWD(V, 1, 64) AIPT_FWD(V, 2, 64) AIPT_FWD(V, 4, 64) AIPT_FWD(V, 2, 256) AIPT_FWD(V, 4, 256) AIPT_FWD(V, 2, 1024)
-    if constexpr (V == 4) { AIPT_FWD(V, 4, 1024) }
-    AIPT_FWD(1, 2, 16) AIPT_FWD(1, 4, 16) AIPT_FWD(1, 8, 16) AIPT_FWD(1, 4, 64) AIPT_FWD(1, 8, 64) AIPT_FWD(1, 4, 256) AIPT_FWD(1, 8, 256) AIPT_FWD(1, 8, 512) AIPT_FWD(1, 8, 1024)
-    return block_norm_fwd<T, 1, 16, 1024>;
+    AIPT_FWD(V, 1, 4) AIPT_FWD(V, 1, 16) AIPT_FWD(V, 2, 16) AIPT_FWD(V, 1, 64) AIPT_FWD(V, 2, 64) AIPT_FWD(V, 2, 256) AIPT_FWD(V, 2, 1024)
+    if constexpr (V == 4) { AIPT_FWD(V, 4, 64) AIPT_FWD(V, 4, 256) AIPT_FWD(V, 4, 1024) }
+    else { AIPT_FWD(V, 1, 256) AIPT_FWD(V, 2, 512) AIPT_FWD(2, 2, 16) AIPT_FWD(2, 4, 16) AIPT_FWD(2, 4, 64) AIPT_FWD(2, 8, 64) AIPT_FWD(2, 4, 256) AIPT_FWD(2, 8, 256) AIPT_FWD(2, 8, 512) AIPT_FWD(2, 8, 1024) }
+    AIPT_FWD(1, 2, 16) AIPT_FWD(1, 4, 16) AIPT_FWD(1, 8, 16) AIPT_FWD(1, 4, 64) AIPT_FWD(1, 8, 64) AIPT_FWD(1, 4, 256) AIPT_FWD(1, 8, 256) AIPT_FWD(1, 8, 512) AIPT_FWD(1, 6, 1024) AIPT_FWD(1, 8, 1024)
+    AIPT_FWD(1, 16, 1024)
+    return nullptr;
 #undef AIPT_FWD
 }
 template <typename T, bool LAYER> static void (*bwd_kernel(NormShape s, bool whole))(NormBwd) {
     constexpr int V = 16 / sizeof(T);
 #define AIPT_BWD(VV, NN, LL, GG) if (s.v == VV && s.n == NN && s.lanes == LL && whole == GG) return block_norm_bwd<T, VV, NN, LL, LAYER, GG>;
-    AIPT_BWD(V, 1, 16, false) AIPT_BWD(V, 2, 16, false) AIPT_BWD(V, 2, 64, false) AIPT_BWD(V, 1, 256, false) AIPT_BWD(V, 2, 256, false)
-    if constexpr (V == 8) { AIPT_BWD(V, 2, 512, false) AIPT_BWD(V, 2, 1024, false) AIPT_BWD(V, 2, 1024, true) }
-    else { AIPT_BWD(V, 4, 256, false) AIPT_BWD(V, 4, 512, false) AIPT_BWD(V, 4, 1024, false) AIPT_BWD(V, 4, 1024, true) }
+    AIPT_BWD(V, 1, 4, false) AIPT_BWD(V, 1, 16, false) AIPT_BWD(V, 2, 16, false) AIPT_BWD(V, 2, 64, false) AIPT_BWD(V, 1, 256, false) AIPT_BWD(V, 2, 256, false)
+    if constexpr (V == 8) {
+        AIPT_BWD(V, 2, 512, false) AIPT_BWD(V, 2, 1024, false) AIPT_BWD(V, 2, 1024, true)
+        AIPT_BWD(2, 2, 16, false) AIPT_BWD(2, 4, 16, false) AIPT_BWD(2, 4, 64, false) AIPT_BWD(2, 2, 256, false) AIPT_BWD(2, 4, 256, false) AIPT_BWD(2, 8, 256, false) AIPT_BWD(2, 8, 512, false) AIPT_BWD(2, 8, 1024, false)
+    } else { AIPT_BWD(V, 4, 256, false) AIPT_BWD(V, 4, 512, false) AIPT_BWD(V, 4, 1024, false) AIPT_BWD(V, 4, 1024, true) }
     AIPT_BWD(V, 1, 16, true) AIPT_BWD(V, 2, 64, true) AIPT_BWD(V, 2, 256, true)
-    AIPT_BWD(1, 2, 16, false) AIPT_BWD(1, 4, 16, false) AIPT_BWD(1, 8, 16, false) AIPT_BWD(1, 8, 64, false) AIPT_BWD(1, 8, 256, false) AIPT_BWD(1, 8, 512, false) AIPT_BWD(1, 8, 1024, false) AIPT_BWD(1, 16, 1024, false)
-    AIPT_BWD(1, 4, 16, true) AIPT_BWD(1, 8, 64, true) AIPT_BWD(1, 8, 256, true) AIPT_BWD(1, 8, 1024, true)
-    return block_norm_bwd<T, 1, 16, 1024, LAYER, true>;
+    AIPT_BWD(1, 2, 16, false) AIPT_BWD(1, 4, 16, false) AIPT_BWD(1, 8, 16, false) AIPT_BWD(1, 8, 64, false) AIPT_BWD(1, 4, 256, false) AIPT_BWD(1, 8, 256, false) AIPT_BWD(1, 8, 512, false) AIPT_BWD(1, 6, 1024, false) AIPT_BWD(1, 16, 512, false)
+    AIPT_BWD(1, 16, 1024, false) AIPT_BWD(1, 4, 16, true) AIPT_BWD(1, 8, 64, true) AIPT_BWD(1, 8, 256, true) AIPT_BWD(1, 8, 1024, true)
+    AIPT_BWD(1, 16, 1024, true)
+    return nullptr;
 #undef AIPT_BWD
 }
 
@@ -557,10 +604,14 @@ static NormParts norm_parts(long long rows, long long groups, int lanes) {
 
 using aipt::fail;
 
-static bool on16(std::initializer_list<const void*> ptrs) {
+// how many elements may move together: 16 bytes' worth, two of 16 bits, or one.  `strides`: 0 for what is not there.
+static int norm_unit(int es, int c, long long rows, std::initializer_list<const void*> ptrs, std::initializer_list<long long> strides) {
     uintptr_t all = 0;
     for (const void* p : ptrs) all |= (uintptr_t)p;
-    return !(all & 15);
+    long long lines = c;
+    if (rows > 1) for (long long s : strides) lines |= s;
+    for (int v : {16 / es, 2}) if (v * es <= 16 && (es == 2 || v == 4) && !(all & (v * es - 1)) && !(lines & (v - 1))) return v;
+    return 1;
 }
 
 extern "C" {
@@ -600,15 +651,16 @@ int aipt_block_norm(aipt_ctx* ctx, const aipt_block_norm_args* a) {
                 return fail(ctx, AIPT_E_INVALID, "%s: an output overlaps an input", me);
         for (int i = 0; i < o; i++) if (aipt::overlap(out[o], out[i])) return fail(ctx, AIPT_E_INVALID, "%s: outputs overlap", me);
     }
-    const int vec = 16 / es;
-    const bool wide = a->c % vec == 0 && on16({a->x, a->y, a->h, a->z, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->pre_bias}) &&
-                      (a->rows == 1 || (!(a->x_stride % vec) && !(a->h_stride % vec) && !(a->y && a->y_stride % vec) && !(a->z && a->z_stride % vec)));
-    const aipt::NormShape s = aipt::fwd_shape(es, a->c, wide);
+    const int v = norm_unit(es, a->c, a->rows, {a->x, a->y, a->h, a->z, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->pre_bias},
+                            {a->x_stride, a->h_stride, a->y ? a->y_stride : 0, a->z ? a->z_stride : 0});
+    const aipt::NormShape s = aipt::fwd_shape(es, a->c, v);
     const aipt::NormFwd f = {a->x, a->y, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->pre_bias, a->h, a->z, a->stats,
                              a->rows, a->rows / (a->gate ? a->groups : 1), a->x_stride, a->y_stride, a->h_stride, a->z_stride, a->c, a->kind == AIPT_NORM_LAYER, a->eps};
     const int threads = std::max(256, s.lanes), per = threads / s.lanes;
     const long long want = (a->rows + per - 1) / per;
-    const size_t blocks = (size_t)std::min(want, 1ll << 20);
+    // 1 024 threads a CU, 512 where a lane holds more than 8 columns (its registers leave no more): 16 384 x 2 048 bf16 78 us with 512, 55 with
+    // 1 024 and 58 with 2 048; 74 400 x 902 fp16 146, 111, 136 us with 256, 512 and 1 024.
+    const size_t blocks = (size_t)std::min(want, (s.n * s.v <= 8 ? 1024ll : 512ll) * 256 / threads);
     auto* k = a->type == AIPT_TYPE_F32 ? aipt::fwd_kernel<float>(s) : a->type == AIPT_TYPE_BF16 ? aipt::fwd_kernel<aipt::bf16>(s) : aipt::fwd_kernel<aipt::f16>(s);
     AIPT_NEED_CTX(ctx);
     aipt::DeviceScope dev(ctx->device);
@@ -639,8 +691,10 @@ int aipt_block_norm_backward_workspace(aipt_ctx* ctx, const aipt_block_norm_grad
     if (rc) return rc;
     const long long groups = norm_gated(a) ? a->groups : 1;
     size_t most = 0;
-    for (bool wide : {false, true}) {
-        const aipt::NormShape s = aipt::bwd_shape(aipt::type_bytes(a->type), a->c, wide, aipt::norm_whole(groups));
+    const int es = aipt::type_bytes(a->type);
+    for (int v : {1, 2, 16 / es}) {
+        if (v == 2 && es == 4) continue;
+        const aipt::NormShape s = aipt::bwd_shape(es, a->c, v, aipt::norm_whole(groups));
         const aipt::NormParts p = aipt::norm_parts(std::max(1ll, a->rows), groups, s.lanes);
         most = std::max(most, (size_t)p.parts * 5 * a->c * sizeof(float));
     }
@@ -691,15 +745,11 @@ int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* a, 
         for (int o = 2; o < 8; o++) AIPT_HIP(ctx, aipt::zero_fill(ctx->stream, out[o].data, (size_t)(out[o].lines * out[o].len)));
         return AIPT_OK;
     }
-    const int vec = 16 / es;
-    bool wide = a->c % vec == 0 && on16({a->dh, a->dz, a->y, a->dz ? a->h : nullptr, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->dx, a->dy, a->dgate});
-    if (a->rows > 1) {
-        for (long long s : strides) wide = wide && !(s % vec);
-        wide = wide && !(a->dx && a->dx_stride % vec) && !(a->dy && a->dy_stride % vec);
-    }
+    const int v = norm_unit(es, a->c, a->rows, {a->dh, a->dz, a->y, a->dz ? a->h : nullptr, a->gate, a->scale, a->post_weight, a->post_bias, a->pre_weight, a->dx, a->dy, a->dgate},
+                            {strides[0], strides[1], strides[2], strides[3], a->dx ? a->dx_stride : 0, a->dy ? a->dy_stride : 0});
     const long long groups = norm_gated(a) ? a->groups : 1;
     const bool whole = aipt::norm_whole(groups);
-    const aipt::NormShape s = aipt::bwd_shape(es, a->c, wide, whole);
+    const aipt::NormShape s = aipt::bwd_shape(es, a->c, v, whole);
     const int threads = std::max(256, s.lanes);
     const aipt::NormParts p = aipt::norm_parts(a->rows, groups, s.lanes);
     const size_t blocks = (size_t)p.parts;
@@ -718,12 +768,12 @@ int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* a, 
     AIPT_HIP(ctx, dev.err);
     AIPT_HIP(ctx, aipt::launch(k, blocks, threads, 0, ctx->stream, b));
     if (part) {
-        const int cb = (a->c + 63) / 64;
+        const int cols = a->c <= 1024 ? 32 : 64, cb = (a->c + cols - 1) / cols;
         const bool gates = a->dgate && p.per_gate_parts;
         const aipt::NormEnd e = {(const float*)d_workspace, a->scale, a->post_weight, a->post_bias, a->dgate, a->dscale, a->dpost_weight, a->dpost_bias, a->dpre_weight, a->dpre_bias,
                                  p.parts, p.per_gate_parts, a->c, cb, layer, a->dscale || a->dpost_weight || a->dpost_bias, a->dpre_weight || a->dpre_bias};
         const size_t jobs = 2 + (gates ? (size_t)a->groups : 0);
-        auto* ke = a->type == AIPT_TYPE_F32 ? aipt::block_norm_end<float> : a->type == AIPT_TYPE_BF16 ? aipt::block_norm_end<aipt::bf16> : aipt::block_norm_end<aipt::f16>;
+        auto* ke = a->type == AIPT_TYPE_F32 ? aipt::end_kernel<float>(cols) : a->type == AIPT_TYPE_BF16 ? aipt::end_kernel<aipt::bf16>(cols) : aipt::end_kernel<aipt::f16>(cols);
         AIPT_HIP(ctx, aipt::launch(ke, jobs * cb, 1024, 0, ctx->stream, e));
     }
     return AIPT_OK;

@@ -70,6 +70,10 @@ inline bool overlap(const Extent& a, const Extent& b) {
 template <int N> __device__ inline float rotate16(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true));
 }
+__device__ inline float sum4(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true));   // the other of a pair
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, true));   // the other pair
+}
 __device__ inline float sum16(float v) {
     v += rotate16<8>(v);
     v += rotate16<4>(v);

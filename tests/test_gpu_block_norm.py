@@ -308,3 +308,22 @@ def test_same_bits_and_captured():
         torch.cuda.synchronize()
         for n in eager:
             assert torch.equal(eager[n], captured[n]), n
+
+
+# A workgroup goes through several rows, their gates change on the way, and each way of reading a row (16 bytes, two elements, one) is taken.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,c,groups", [(150000, 24, 3), (150000, 24, 75000), (40000, 57, 5), (40000, 38, 40000), (9000, 600, 9), (9000, 602, 2), (9000, 601, 9000), (3600, 1500, 3), (3600, 1501, 1), (3600, 1502, 1800),
+                                        (1200, 4500, 400), (1200, 4502, 3), (1200, 4501, 3), (800, 6100, 2), (800, 6801, 4), (600, 9000, 6), (600, 9001, 1), (600, 9002, 300)])
+def test_several_rows_a_workgroup(m, c, groups, dtype):
+    gen = generator(m + c)
+    for kind, in_place in (("layer", False), ("rms", True)):
+        check_forward(matrix(gen, m, c, dtype), matrix(gen, m, c, dtype), vectors(gen, c, dtype, kind, groups), kind, in_place=in_place)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("c", [16, 30, 32, 60, 66, 130, 258, 514, 998, 1000, 1026, 2049, 2050, 4097, 4098, 6146, 6150, 7001])
+def test_backward_more_widths(c, kind, dtype):
+    gen = generator(c + 2)
+    m = 2700 if c < 1000 else 1500
+    check_backward(*(matrix(gen, m, c, dtype) for _ in range(4)), vectors(gen, c, dtype, kind, 3), kind)
