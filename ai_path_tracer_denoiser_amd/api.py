@@ -513,16 +513,18 @@ class Context:
     # Tensors are torch's; the work runs on the context's stream.  Where that is not torch's current stream, the call waits for what is
     # queued there and what is queued there later waits for the call, so that tensors may be used, and freed, like in any torch program.
     def _on_stream(self, entry, *args):
-        import torch
         if self._stream is None:
+            import torch
             p = _P()
             self._ck(lib().aipt_stream(self._h, C.byref(p)))
             self._stream = p.value or 0
             # (ExternalStream takes 0 for "none given" and makes a new stream)
             self._ext = torch.cuda.ExternalStream(self._stream, device=self.device) if self._stream else torch.cuda.default_stream(self.device)
-        if torch._C._cuda_getCurrentRawStream(self.device) == self._stream:
+            self._current = torch._C._cuda_getCurrentRawStream
+        if self._current(self.device) == self._stream:
             rc = entry(self._h, *args)
             return self._ck(rc) if rc else None
+        import torch
         now = torch.cuda.current_stream(self.device)
         if not self._stream and torch.cuda.is_current_stream_capturing():
             raise AiptError("a context on the default stream cannot take part in a capture: make one with stream=<the capturing stream's handle>")
@@ -570,6 +572,12 @@ class Context:
             raise AiptError(f"{name}: stride {t.stride(0)}")
         return t.data_ptr()
 
+    # the same of several at once: a call of little work is bound by what is done here for each tensor
+    def _vectors(self, dtype, n, **of):
+        dev, shape = self.device, (n,)
+        return [0 if t is None else t.data_ptr() if t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.stride() == (1,)
+                else self._vector(name, t, dtype, n) for name, t in of.items()]
+
     def linear(self, x, w, y, bias=None, residual=None, preact=None, act: str = "none", slope: float = 0.1):
         """aipt_linear: y = act(x w^T + bias) + residual.  x [m, k], w [n, k], y [m, n] -- each with unit stride along either axis, so a planar
         feature map [channels, pixels] comes as its .t() -- bias [n], residual [m, n] (may be y); preact [m, n] receives x w^T + bias, which
@@ -606,30 +614,40 @@ class Context:
         hold, ptr, size = self._scratch(lib().aipt_linear_backward_workspace, record)
         self._on_stream(lib().aipt_linear_backward, record, ptr, size)
 
-    def _rows(self, name, t, dtype, rows, c):
-        """(address, row stride) of an optional [rows, c] with contiguous rows"""
-        if t is None:
-            return 0, 0
-        self._want(name, t, dtype, rows, c)
-        if c > 1 and t.stride(1) != 1:
-            raise AiptError(f"{name}: stride {t.stride(1)} between the channels of a row")
-        return t.data_ptr(), t.stride(0)
+    def _rows(self, dtype, rows, c, **of):
+        """the addresses and the row strides of optional [rows, c] with contiguous rows"""
+        dev, shape, at, strides = self.device, (rows, c), [], []
+        for name, t in of.items():
+            if t is None:
+                at.append(0)
+                strides.append(0)
+                continue
+            if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+                self._want(name, t, dtype, rows, c)
+            row, col = t.stride()
+            if col != 1 and c > 1:
+                raise AiptError(f"{name}: stride {col} between the channels of a row")
+            at.append(t.data_ptr())
+            strides.append(row)
+        return at, strides
 
     def _gates(self, name, t, dtype, c, groups):
         if t is None:
             return 0
-        if t.dim() != 2 or not t.is_contiguous():
-            raise AiptError(f"{name}: {tuple(t.shape)} contiguous [groups, channels] is wanted")
-        self._want(name, t, dtype, groups, c)
+        if t.dtype is not dtype or t.get_device() != self.device or t.shape != (groups, c) or t.stride() != (c, 1):
+            if t.dim() != 2 or not t.is_contiguous():
+                raise AiptError(f"{name}: {tuple(t.shape)} contiguous [groups, channels] is wanted")
+            self._want(name, t, dtype, groups, c)
         return t.data_ptr()
 
     def _stats(self, stats, rows):
         if stats is None:
             return 0
-        import torch
-        self._want("stats", stats, torch.float32, rows, 4)
-        if not stats.is_contiguous():
-            raise AiptError("stats is not contiguous")
+        if _TYPES.get(stats.dtype) != TYPE_F32 or stats.get_device() != self.device or stats.shape != (rows, 4) or stats.stride() != (4, 1):
+            import torch
+            self._want("stats", stats, torch.float32, rows, 4)
+            if not stats.is_contiguous():
+                raise AiptError("stats is not contiguous")
         return stats.data_ptr()
 
     def block_norm(self, y, x, h, z=None, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, kind: str = "rms",
@@ -643,10 +661,9 @@ class Context:
             raise AiptError(f"block_norm: x {tuple(x.shape)}")
         rows, c = x.shape
         groups = gate.shape[0] if gate is not None and gate.dim() == 2 else 1
-        (xp, xs), (yp, ys), (hp, hs), (zp, zs) = self._rows("x", x, d, rows, c), self._rows("y", y, d, rows, c), self._rows("h", h, d, rows, c), self._rows("z", z, d, rows, c)
-        record = _NORM.pack(t, _choice("kind", kind, NORMS), eps, c, rows, groups, xp, yp, hp, zp, xs, ys, hs, zs, self._gates("gate", gate, d, c, groups),
-                            self._vector("scale", scale, d, c), self._vector("post_weight", post_weight, d, c), self._vector("post_bias", post_bias, d, c),
-                            self._vector("pre_weight", pre_weight, d, c), self._vector("pre_bias", pre_bias, d, c), self._stats(stats, rows))
+        at, strides = self._rows(d, rows, c, x=x, y=y, h=h, z=z)
+        record = _NORM.pack(t, _choice("kind", kind, NORMS), eps, c, rows, groups, *at, *strides, self._gates("gate", gate, d, c, groups),
+                            *self._vectors(d, c, scale=scale, post_weight=post_weight, post_bias=post_bias, pre_weight=pre_weight, pre_bias=pre_bias), self._stats(stats, rows))
         self._on_stream(lib().aipt_block_norm, record)
         return h, z
 
@@ -661,12 +678,11 @@ class Context:
         rows, c = like.shape
         g = gate if gate is not None else dgate
         groups = g.shape[0] if g is not None and g.dim() == 2 else 1
-        r = [self._rows(n, v, d, rows, c) for n, v in (("dh", dh), ("dz", dz), ("y", y), ("h", h), ("dx", dx), ("dy", dy))]
-        vec = [self._vector(n, v, d, c) for n, v in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight), ("dscale", dscale),
-                                                     ("dpost_weight", dpost_weight), ("dpost_bias", dpost_bias), ("dpre_weight", dpre_weight), ("dpre_bias", dpre_bias))]
-        record = _NORM_GRAD.pack(t, _choice("kind", kind, NORMS), c, 0, rows, groups, r[0][0], r[1][0], r[2][0], r[3][0], self._stats(stats, rows),
-                                 self._gates("gate", gate, d, c, groups), *vec[:4], r[4][0], r[5][0], r[0][1], r[1][1], r[2][1], r[3][1], r[4][1], r[5][1],
-                                 self._gates("dgate", dgate, d, c, groups), *vec[4:])
+        at, strides = self._rows(d, rows, c, dh=dh, dz=dz, y=y, h=h, dx=dx, dy=dy)
+        vec = self._vectors(d, c, scale=scale, post_weight=post_weight, post_bias=post_bias, pre_weight=pre_weight, dscale=dscale, dpost_weight=dpost_weight,
+                            dpost_bias=dpost_bias, dpre_weight=dpre_weight, dpre_bias=dpre_bias)
+        record = _NORM_GRAD.pack(t, _choice("kind", kind, NORMS), c, 0, rows, groups, *at[:4], self._stats(stats, rows), self._gates("gate", gate, d, c, groups),
+                                 *vec[:4], *at[4:], *strides, self._gates("dgate", dgate, d, c, groups), *vec[4:])
         hold, ptr, size = self._scratch(lib().aipt_block_norm_backward_workspace, record)
         self._on_stream(lib().aipt_block_norm_backward, record, ptr, size)
 
