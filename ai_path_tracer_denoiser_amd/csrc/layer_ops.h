@@ -36,9 +36,10 @@ struct DeviceScope {
 };
 
 // hipLaunchKernel answers for this launch alone (hipGetLastError would also hand over an error somebody else left behind)
-template <typename Args>
-inline hipError_t launch(void (*kernel)(Args), size_t blocks, unsigned threads, unsigned lds, hipStream_t st, Args args) {
-    void* p[] = {&args};
+template <typename... Args, typename... Given>
+inline hipError_t launch(void (*kernel)(Args...), size_t blocks, unsigned threads, unsigned lds, hipStream_t st, const Given&... args) {
+    static_assert((std::is_same_v<std::remove_const_t<Args>, Given> && ...), "the kernel's arguments");
+    void* p[] = {(void*)&args...};
     return hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3((unsigned)blocks), dim3(threads), p, lds, st);
 }
 

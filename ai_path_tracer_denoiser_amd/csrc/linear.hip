@@ -345,21 +345,21 @@ template <typename T, int ACT> __device__ inline void epilogue8(const GemmArgs& 
     *(Oct*)((T*)g.c + i * g.cs + j) = q;
 }
 
+template <int TI, int TJ, int WI, int WJ, int S> constexpr int tile_lds() {       // bytes: the ring, or the slabs that results go through
+    const int ring = S % 2 ? S * TI * 128 : S / 2 * (TI + TJ) * 128, slabs = WI * WJ * (TI / WI < 64 ? TI / WI : 64) * (TJ / WJ) * 4;
+    return ring > slabs ? ring : slabs;
+}
 template <typename T, bool AK, bool BK, int TI, int TJ, int WI, int WJ, int S, int W>
-__global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
+__device__ __forceinline__ void tile_of(const GemmArgs& g, const int block, const int total, AIPT_LDS char* lds) {
     constexpr int NT = WI * WJ * 64, WTI = TI / WI, WTJ = TJ / WJ, FI = WTI / 16, FJ = WTJ / 16;
     static_assert(TI == TJ || S % 2 == 0, "an odd ring's slots hold A and B in turn");
     constexpr int SA = TI * 128, SB = TJ * 128;              // bytes of a slot
     constexpr int SLAB = WTI < 64 ? WTI : 64;                // rows of a wave's results that go through LDS at a time
-    constexpr int RING = S % 2 ? S * SA : S / 2 * (SA + SB);
-    constexpr int BYTES = RING > WI * WJ * SLAB * WTJ * 4 ? RING : WI * WJ * SLAB * WTJ * 4;
-    __shared__ __attribute__((aligned(1024))) char lds_[BYTES];
-    AIPT_LDS char* lds = (AIPT_LDS char*)lds_;
     using V = typename Frag<T>::V;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // workgroups go round the eight XCDs: each XCD takes a run of neighbouring tiles, which share operands in its L2 ...
-    const int total = gridDim.x, per = total >> 3, extra = total & 7, x = blockIdx.x & 7;
-    int job = (x < extra ? x * (per + 1) : extra * (per + 1) + (x - extra) * per) + (blockIdx.x >> 3);
+    const int per = total >> 3, extra = total & 7, x = block & 7;
+    int job = (x < extra ? x * (per + 1) : extra * (per + 1) + (x - extra) * per) + (block >> 3);
     const int tiles = g.tiles_i * g.tiles_j, split = job / tiles;
     job -= split * tiles;
     // ... in columns of 8 tiles
@@ -547,16 +547,27 @@ __global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
     }
 }
 
+template <typename T, bool AK, bool BK, int TI, int TJ, int WI, int WJ, int S, int W>
+__global__ __launch_bounds__(WI * WJ * 64, 1) void gemm_tile(const GemmArgs g) {
+    __shared__ __attribute__((aligned(1024))) char lds[tile_lds<TI, TJ, WI, WJ, S>()];
+    tile_of<T, AK, BK, TI, TJ, WI, WJ, S, W>(g, blockIdx.x, gridDim.x, (AIPT_LDS char*)lds);
+}
+// Both gradients of a small layer in one launch, by tiles of 64 x 64: neither fills the chip.  AK, BK: of the first (nx workgroups); AK2, BK2.
+template <typename T, bool AK, bool BK, bool AK2, bool BK2>
+__global__ __launch_bounds__(256, 1) void gemm_both(const GemmArgs dx, const GemmArgs dw, const unsigned nx) {
+    __shared__ __attribute__((aligned(1024))) char lds[tile_lds<64, 64, 2, 2, 6>()];
+    if (blockIdx.x < nx) tile_of<T, AK, BK, 64, 64, 2, 2, 6, 16>(dx, blockIdx.x, nx, (AIPT_LDS char*)lds);
+    else tile_of<T, AK2, BK2, 64, 64, 2, 2, 6, 16>(dw, blockIdx.x - nx, gridDim.x - nx, (AIPT_LDS char*)lds);
+}
+
 // The splits of a long contraction, added in a fixed order, and the epilogue: four neighbours a thread.  SIDE threads share a result's splits
 // (many splits of a small result: one thread for each result ran for 245 us at 368 splits of 64 x 46).
-template <typename T, int SIDE>
-__global__ __launch_bounds__(256) void gemm_join(const GemmArgs g) {
+template <typename T, int SIDE> __device__ inline void join(const GemmArgs& g, long long block, long long blocks, float4 (*lds)[16]) {
     constexpr int QUADS = 256 / SIDE;
-    __shared__ float4 lds[SIDE > 1 ? SIDE : 1][QUADS];
     const int per = (g.J + 3) / 4, x = threadIdx.x % QUADS, side = threadIdx.x / QUADS;
     const long long quads = (long long)g.I * per, n = (long long)g.I * g.J;
     const bool quad16 = !(g.J & 3);
-    for (long long q0 = (long long)blockIdx.x * QUADS; q0 < quads; q0 += (long long)gridDim.x * QUADS) {
+    for (long long q0 = block * QUADS; q0 < quads; q0 += blocks * QUADS) {
         const long long at = q0 + x;
         const int i = (int)(at / per), j = (int)(at - (long long)i * per) * 4;
         float s[4] = {};
@@ -592,6 +603,18 @@ __global__ __launch_bounds__(256) void gemm_join(const GemmArgs g) {
             for (int e = 0; e < 4; e++) if (j + e < g.J) epilogue<T>(g, i, j + e, s[e]);
         }
     }
+}
+
+constexpr int JOIN_SIDE = 16;
+static bool join_by_side(const GemmArgs& g) { return g.splits > 8; }
+static size_t join_blocks(const GemmArgs& g) {
+    const size_t quads = (size_t)g.I * ((g.J + 3) / 4);
+    return join_by_side(g) ? std::min<size_t>((quads + 15) / 16, 8192) : std::min<size_t>((quads + 255) / 256, 4096);
+}
+template <typename T, int SIDE>
+__global__ __launch_bounds__(256) void gemm_join(const GemmArgs g) {
+    __shared__ float4 lds[SIDE > 1 ? SIDE : 1][16];
+    join<T, SIDE>(g, blockIdx.x, gridDim.x, lds);
 }
 
 // ---- a few rows (at most 8): every line of the many is read once, 16 bytes a lane, by the wave that its results belong to: no tile, no split, one
@@ -636,22 +659,26 @@ __global__ __launch_bounds__(256) void gemm_rows(const GemmArgs g) {
 // ---- lines that begin anywhere (of halves: an element is one or two), copied to lines on 16 bytes, padded with zeros: twice the operand's bytes, once, for loads of 16 bytes
 // in every tile that reads it (1375 x 909 by 303 x 909: 58 us by gemm_any)
 struct PackArgs {
-    struct { const unsigned short* p; Chunk<unsigned short>* to; long long stride, chunks; int len, line; } m[2];      // line: chunks of a line
+    struct Lines { const unsigned short* p; Chunk<unsigned short>* to; long long stride, chunks; int len, line; } m[4];      // line: chunks of a line
+    int n;
+    long long chunks() const { return m[0].chunks + m[1].chunks + m[2].chunks + m[3].chunks; }
+    size_t blocks() const { return (size_t)std::min<long long>((chunks() + 255) / 256, 8192); }
 };
-__global__ __launch_bounds__(256) void pack_lines(const PackArgs g) {
-    const long long n = g.m[0].chunks + g.m[1].chunks;
-    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
-        const bool second = at >= g.m[0].chunks;
-        const auto& m = g.m[second];
-        const long long c = second ? at - g.m[0].chunks : at, l = c / m.line;
-        const int k = (int)(c - l * m.line) * 8;
-        const unsigned short* s = m.p + l * m.stride + k;
-        Chunk<unsigned short> q;
+__device__ inline void pack(const PackArgs& g, long long block, long long blocks) {
+    for (int o = 0; o < g.n; o++) {
+        const auto& m = g.m[o];
+        for (long long c = block * 256 + threadIdx.x; c < m.chunks; c += blocks * 256) {
+            const long long l = c / m.line;
+            const int k = (int)(c - l * m.line) * 8;
+            const unsigned short* s = m.p + l * m.stride + k;
+            Chunk<unsigned short> q;
 #pragma unroll
-        for (int e = 0; e < 8; e++) q.v[e] = k + e < m.len ? s[e] : (unsigned short)0;
-        m.to[c] = q;
+            for (int e = 0; e < 8; e++) q.v[e] = k + e < m.len ? s[e] : (unsigned short)0;
+            m.to[c] = q;
+        }
     }
 }
+__global__ __launch_bounds__(256) void pack_lines(const PackArgs g) { pack(g, blockIdx.x, gridDim.x); }
 
 // ---- dz = dy * act'(z), rounded to the element type, and its sums over rows: dy is read once for both.  V elements a lane: 16 bytes where lines
 // lie on 16 bytes, two where they lie on two, else one.  A workgroup takes `high` rows; `across` lanes (a power of two) share a row, so that narrow rows too fill a
@@ -666,11 +693,13 @@ struct DzArgs {
     int line;                        // dz's lines, with their padding (of zeros)
     int high, tiles_n, across, act;
     float slope;
+    unsigned blocks;
 };
 template <typename T, int V, bool TURNED>
-__global__ __launch_bounds__(256) void act_backward(const DzArgs g) {
+__global__ __launch_bounds__(256) void act_backward(const DzArgs g, const PackArgs copies) {
     struct alignas(V * sizeof(T)) E { T v[V]; };
     __shared__ float lds[TURNED ? 1 : 256 * V];
+    if (blockIdx.x >= g.blocks) return pack(copies, blockIdx.x - g.blocks, gridDim.x - g.blocks);      // the products' operands that are copied, in the same launch
     const int tm = (int)(blockIdx.x / g.tiles_n), tn = (int)(blockIdx.x % g.tiles_n);
     // V elements: in [is there an element], out [is there one of dz, padding included]
     auto one = [&](const T* dyp, const T* zp, T* dzp, bool in, bool out, float* d) {
@@ -775,21 +804,31 @@ struct SumArgs {
     void* out;
     int parts, N;
 };
+// What is left when both products are done, in one launch: their splits joined and the bias's partial sums added (16 columns x 16 lanes of parts).
 template <typename T>
-__global__ __launch_bounds__(1024) void sum_parts(const SumArgs g) {
-    __shared__ float lds[16][64];
-    const int x = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + x;
+__global__ __launch_bounds__(256) void grad_end(const GemmArgs dx, const GemmArgs dw, const SumArgs g, const unsigned nx, const unsigned nw) {
+    __shared__ float4 lds[JOIN_SIDE][16];
+    unsigned block = blockIdx.x;
+    if (block < nx + nw) {
+        const GemmArgs& j = block < nx ? dx : dw;
+        const unsigned at = block < nx ? block : block - nx, n = block < nx ? nx : nw;
+        if (j.splits > 8) join<T, JOIN_SIDE>(j, at, n, lds);
+        else join<T, 1>(j, at, n, lds);
+        return;
+    }
+    float (*sums)[16] = (float (*)[16])lds;
+    const int x = threadIdx.x & 15, w = threadIdx.x >> 4, n = (block - nx - nw) * 16 + x;
     float s = 0;
     if (n < g.N) {
 #pragma unroll 8
         for (int p = w; p < g.parts; p += 16) s += g.part[(long long)p * g.N + n];
     }
-    lds[w][x] = s;
+    sums[w][x] = s;
     __syncthreads();
     if (w || n >= g.N) return;
     s = 0;
 #pragma unroll
-    for (int i = 0; i < 16; i++) s += lds[i][x];
+    for (int i = 0; i < 16; i++) s += sums[i][x];
     ((T*)g.out)[n] = (T)s;
 }
 
@@ -988,25 +1027,28 @@ static int row_unit(int es, const GemmArgs& g) {
     return on(16) ? 8 : g.J % 2 == 0 && on(2 * es) ? 2 : 1;
 }
 
+// the product itself, its operands' copies being made: where they lie and the partial sums
+static void place(Plan& p, char* ws) {
+    for (int o = 0; o < 2; o++) {
+        if (!p.pack.m[o].chunks) continue;
+        p.pack.m[o].to = (Chunk<unsigned short>*)(ws + (size_t)p.pack.m[o].to);
+        (o ? p.g.b : p.g.a) = p.pack.m[o].to;
+    }
+    p.g.partial = (float*)(ws + p.pack_bytes);
+}
+template <typename T> static hipError_t launch_gemm(hipStream_t st, Plan& p) {
+    p.g.cv = row_unit(sizeof(T), p.g);
+    return launch(gemm_of<T>(p), p.blocks, 256, 0, st, p.g);
+}
 template <typename T> static hipError_t run_gemm_t(hipStream_t st, Plan& p, void* ws) {
     if (!p.blocks) return hipSuccess;
-    if (p.pack_bytes) {
-        for (int o = 0; o < 2; o++) {
-            if (!p.pack.m[o].chunks) continue;
-            p.pack.m[o].to = (Chunk<unsigned short>*)((char*)ws + (size_t)p.pack.m[o].to);
-            (o ? p.g.b : p.g.a) = p.pack.m[o].to;
-        }
-        const hipError_t e = launch(pack_lines, (size_t)std::min<long long>((p.pack.m[0].chunks + p.pack.m[1].chunks + 255) / 256, 8192), 256, 0, st, p.pack);
-        if (e != hipSuccess) return e;
-    }
-    p.g.partial = (float*)((char*)ws + p.pack_bytes);
-    p.g.cv = row_unit(sizeof(T), p.g);
-    hipError_t e = launch(gemm_of<T>(p), p.blocks, 256, 0, st, p.g);
+    place(p, (char*)ws);
+    hipError_t e = hipSuccess;
+    p.pack.n = 2;
+    if (p.pack_bytes) e = launch(pack_lines, p.pack.blocks(), 256, 0, st, p.pack);
+    if (e == hipSuccess) e = launch_gemm<T>(st, p);
     if (e == hipSuccess && p.g.splits > 1)
-    {
-        const size_t quads = (size_t)p.g.I * ((p.g.J + 3) / 4);
-        e = p.g.splits > 8 ? launch(gemm_join<T, 16>, std::min<size_t>((quads + 15) / 16, 8192), 256, 0, st, p.g) : launch(gemm_join<T, 1>, std::min<size_t>((quads + 255) / 256, 4096), 256, 0, st, p.g);
-    }
+        e = join_by_side(p.g) ? launch(gemm_join<T, JOIN_SIDE>, join_blocks(p.g), 256, 0, st, p.g) : launch(gemm_join<T, 1>, join_blocks(p.g), 256, 0, st, p.g);
     return e;
 }
 static hipError_t run_gemm(int type, hipStream_t st, Plan& p, void* ws) {
@@ -1092,15 +1134,46 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         p.dw = o.second ? plan_gemm(a->type, flip(d), flip(x), a->n, a->k, a->m) : plan_gemm(a->type, flip(x), flip(d), a->k, a->n, a->m);
         p.dw.g.c = a->dw.data; p.dw.g.cs = o.other;
     }
-    p.gemm_bytes = up256(std::max(p.want_dx ? p.dx.bytes() : 0, p.want_dw ? p.dw.bytes() : 0));
+    p.gemm_bytes = up256(p.want_dx ? p.dx.bytes() : 0) + up256(p.want_dw ? p.dw.bytes() : 0);
     return p;
 }
 
-template <typename T> static void (*dz_kernel(const GradPlan& p))(DzArgs) {
+template <typename T> static void (*dz_kernel(const GradPlan& p))(DzArgs, PackArgs) {
     constexpr int V = 16 / sizeof(T);
     if (p.dz_v == V) return p.dz_turned ? act_backward<T, V, true> : act_backward<T, V, false>;
     if (p.dz_v == 2) return p.dz_turned ? act_backward<T, 2, true> : act_backward<T, 2, false>;
     return p.dz_turned ? act_backward<T, 1, true> : act_backward<T, 1, false>;
+}
+
+// The gradients: dz with its sums and the operands' copies, the products, and what is left of both -- three to four launches.
+template <typename T> static hipError_t run_backward(hipStream_t st, GradPlan& p, const aipt_linear_grad_args* a, char* ws) {
+    hipError_t e = hipSuccess;
+    PackArgs copies = {};
+    char* at = ws + p.dz_bytes + p.part_bytes;
+    for (Plan* q : {&p.dx, &p.dw}) {
+        if (!q->blocks) continue;
+        place(*q, at);
+        at += up256(q->bytes());
+        for (auto& m : q->pack.m) if (m.chunks) copies.m[copies.n++] = m;
+    }
+    if (p.dz_blocks) {
+        p.dz.blocks = (unsigned)p.dz_blocks;
+        e = launch(dz_kernel<T>(p), p.dz_blocks + copies.blocks(), 256, 0, st, p.dz, copies);
+    } else if (copies.n) e = launch(pack_lines, copies.blocks(), 256, 0, st, copies);
+    if (e == hipSuccess && p.want_db && !a->m) e = zero_fill(st, a->dbias, (size_t)a->n * sizeof(T));
+    // where both go by the small tile and the matrices lie all one way: rows, or planar
+    const Plan &x = p.dx, &w = p.dw;
+    const bool rows = x.ak && !x.bk && !w.ak && !w.bk, planar = !x.ak && x.bk && !w.ak && w.bk;
+    if (e == hipSuccess && x.blocks && w.blocks && x.tile == 3 && w.tile == 3 && !x.small && !w.small && (rows || planar) && grid_fits(x.blocks + w.blocks, 256)) {
+        p.dx.g.cv = row_unit(sizeof(T), x.g);
+        p.dw.g.cv = row_unit(sizeof(T), w.g);
+        e = launch(rows ? gemm_both<T, true, false, false, false> : gemm_both<T, false, true, false, true>, x.blocks + w.blocks, 256, 0, st, x.g, w.g, (unsigned)x.blocks);
+    } else
+        for (Plan* q : {&p.dx, &p.dw}) if (e == hipSuccess && q->blocks) e = launch_gemm<T>(st, *q);
+    const size_t nx = p.dx.blocks && p.dx.g.splits > 1 ? join_blocks(p.dx.g) : 0, nw = p.dw.blocks && p.dw.g.splits > 1 ? join_blocks(p.dw.g) : 0,
+                 nb = p.want_db && p.parts > 1 ? (size_t)((a->n + 15) / 16) : 0;
+    if (e == hipSuccess && nx + nw + nb) e = launch(grad_end<T>, nx + nw + nb, 256, 0, st, p.dx.g, p.dw.g, SumArgs{p.dz.part, a->dbias, p.parts, (int)a->n}, (unsigned)nx, (unsigned)nw);
+    return e;
 }
 
 static int linear_check(aipt_ctx* ctx, const char* me, int type, int act, float slope, int reserved, long long m, long long n, long long k) {
@@ -1199,7 +1272,7 @@ int aipt_linear_backward(aipt_ctx* ctx, const aipt_linear_grad_args* a, void* d_
     if (rc) return rc;
     const int es = aipt::type_bytes(a->type);
     aipt::GradPlan p = aipt::plan_backward(a, (char*)d_workspace);
-    if ((p.want_dx && !p.dx.fits) || (p.want_dw && !p.dw.fits) || !aipt::grid_fits(p.dz_blocks, 256))
+    if ((p.want_dx && !p.dx.fits) || (p.want_dw && !p.dw.fits) || !aipt::grid_fits(p.dz_blocks + 8192, 256))
         return fail(ctx, AIPT_E_INVALID, "%s: %lld x %lld x %lld has too many tiles", me, a->m, a->n, a->k);
     if (p.bytes() && (!d_workspace || workspace_bytes < p.bytes() || ((uintptr_t)d_workspace & 255)))
         return fail(ctx, AIPT_E_INVALID, "%s: workspace of %zu bytes, %zu are wanted, 256-byte aligned", me, workspace_bytes, p.bytes());
@@ -1217,16 +1290,8 @@ int aipt_linear_backward(aipt_ctx* ctx, const aipt_linear_grad_args* a, void* d_
     AIPT_HIP(ctx, dev.err);
     const hipStream_t st = ctx->stream;
     const int t = a->type;
-    if (p.dz_blocks)
-        AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::dz_kernel<float>(p) : t == AIPT_TYPE_BF16 ? aipt::dz_kernel<aipt::bf16>(p) : aipt::dz_kernel<aipt::f16>(p), p.dz_blocks, 256, 0, st, p.dz));
-    if (p.want_db) {
-        if (p.parts > 1) AIPT_HIP(ctx, aipt::launch(t == AIPT_TYPE_F32 ? aipt::sum_parts<float> : t == AIPT_TYPE_BF16 ? aipt::sum_parts<aipt::bf16> : aipt::sum_parts<aipt::f16>, (size_t)((a->n + 63) / 64), 1024, 0, st,
-                                             aipt::SumArgs{p.dz.part, a->dbias, p.parts, (int)a->n}));
-        else if (!a->m) AIPT_HIP(ctx, aipt::zero_fill(st, a->dbias, (size_t)a->n * es));
-    }
-    char* gemm_ws = (char*)d_workspace + p.dz_bytes + p.part_bytes;
-    if (p.want_dx) AIPT_HIP(ctx, aipt::run_gemm(t, st, p.dx, gemm_ws));
-    if (p.want_dw) AIPT_HIP(ctx, aipt::run_gemm(t, st, p.dw, gemm_ws));
+    char* ws = (char*)d_workspace;
+    AIPT_HIP(ctx, t == AIPT_TYPE_F32 ? aipt::run_backward<float>(st, p, a, ws) : t == AIPT_TYPE_BF16 ? aipt::run_backward<aipt::bf16>(st, p, a, ws) : aipt::run_backward<aipt::f16>(st, p, a, ws));
     return AIPT_OK;
 }
 
