@@ -915,7 +915,7 @@ static const struct Tile { int i, j, fit; double start, pair[2][3]; } TILES[] = 
 constexpr int NTILES = 6, CUS = 256;
 
 // The tile and how often the contraction is split, by the estimate above: rounds of workgroups, and for a split the partial sums' way out and
-// back (a join's launch and some 3.5 TB/s).  small: the lines are on 4 bytes only.
+// back (a join's launch and some 3.5 TB/s).  small: the lines are on 4 bytes only, whose loads cost the steps half again (floats: a quarter).
 static double pick(bool wide, bool small, long long I, long long J, long long pairs, int& tile, long long& splits) {
     double best = 1e30;
     for (int t = 1; t < NTILES; t++) {
@@ -926,7 +926,7 @@ static double pick(bool wide, bool small, long long I, long long J, long long pa
             long long s = fill ? std::min(CUS * fill / std::max(1ll, tiles), pairs / 2) : 1;
             if (s < 1 || (fill && s == 1)) continue;
             const long long n = (pairs + s - 1) / s, blocks = tiles * s, full = blocks / (CUS * c.fit), rest = blocks - full * CUS * c.fit;
-            auto round = [&](int with) { return c.start + n * c.pair[wide][with - 1]; };
+            auto round = [&](int with) { return c.start + n * c.pair[wide][with - 1] * (small ? wide ? 1.25 : 1.45 : 1); };
             double us = full * round(c.fit);
             if (rest) us += round((int)((rest + CUS - 1) / CUS));
             if (s > 1) us += 4 + (double)(s + 1) * I * J * 4 / 3.5e6;
@@ -936,8 +936,8 @@ static double pick(bool wide, bool small, long long I, long long J, long long pa
     return best;
 }
 
-// C[i][j] = sum_k A[i][k] B[j][k]; A (I x K) and B (J x K) by their strides; the result's j axis contiguous
-static Plan plan_gemm(int type, View a, View b, long long I, long long J, long long K) {
+// C[i][j] = sum_k A[i][k] B[j][k]; A (I x K) and B (J x K) by their strides; the result's j axis contiguous.  copy_us: what a launch for copies costs
+static Plan plan_gemm(int type, View a, View b, long long I, long long J, long long K, double copy_us) {
     Plan p;
     const int es = type_bytes(type), E = 16 / es, ks = 8 * E;
     p.ak = a.second; p.bk = b.second;
@@ -950,18 +950,36 @@ static Plan plan_gemm(int type, View a, View b, long long I, long long J, long l
             if (!((uintptr_t)v.p & (w - 1)) && v.other * es % w == 0 && (v.padded || len * es % w == 0)) return w;
         return 0;
     };
+    const long long pairs = (K + ks - 1) / ks;
+    long long splits = 1;
     int w[2];
     for (int o = 0; o < 2; o++) w[o] = unit(o ? b : a, (o ? b : a).second ? K : o ? J : I);
+    // Copied to lines of 16 bytes: 16-bit lines on less than 4; a small operand for whose sake the other would go by 4 too; and whatever lies on 4
+    // where the estimate says so, a copy at 2.2 TB/s included (bf16 8192 x 2050 x 2048: 158 -> 92 us; 4096 x 1030 x 1024 27 by loads of 4, 33 copied).
+    long long lines[2], line[2];
+    bool copy[2];
+    for (int o = 0; o < 2; o++) {
+        const View& v = o ? b : a;
+        const long long rows = o ? J : I;
+        line[o] = ((v.second ? K : rows) + E - 1) / E;
+        lines[o] = v.second ? rows : K;
+        copy[o] = (!w[o] && es == 2) || (w[o] != 16 && w[1 - o] == 16 && lines[o] * line[o] * 16 <= std::max(1ll << 20, (o ? I : J) * K * es / 4));
+    }
+    if (I && J && (w[0] || copy[0]) && (w[1] || copy[1]) && ((w[0] == 4 && !copy[0]) || (w[1] == 4 && !copy[1]))) {
+        double bytes = 0;
+        for (int o = 0; o < 2; o++) if (w[o] == 4 && !copy[o]) bytes += (double)lines[o] * line[o] * 16;
+        int t = 0;
+        if (pick(es == 4, false, I, J, pairs, t, splits) + copy_us + bytes * 2 / 2.2e6 < pick(es == 4, true, I, J, pairs, t, splits))
+            for (int o = 0; o < 2; o++) copy[o] |= w[o] == 4;
+    }
     for (int o = 0; o < 2; o++) {
         View& v = o ? b : a;
-        const long long rows = o ? J : I, len = v.second ? K : rows, lines = v.second ? rows : K, line = (len + E - 1) / E;
-        // copied to lines of 16 bytes: 16-bit lines on less than 4, and a small operand for whose sake the other would go by 4 too
-        const bool small = w[o] != 16 && w[1 - o] == 16 && lines * line * 16 <= std::max(1ll << 20, (o ? I : J) * K * es / 4);
-        if (I && J && K && ((!w[o] && es == 2) || small) && line * 16 * 256 < (1ll << 31)) {
+        const long long len = v.second ? K : o ? J : I;
+        if (I && J && K && copy[o] && line[o] * 16 * 256 < (1ll << 31)) {
             const int h = es / 2;                            // halves of an element
-            p.pack.m[o] = {(const unsigned short*)v.p, (Chunk<unsigned short>*)p.pack_bytes, v.other * h, lines * line, (int)len * h, (int)line};   // (`to`: an offset for now)
-            p.pack_bytes += up256((size_t)(lines * line) * 16);
-            v = {nullptr, v.second ? line * E : 1, v.second ? 1 : line * E, v.second, line * E, true};
+            p.pack.m[o] = {(const unsigned short*)v.p, (Chunk<unsigned short>*)p.pack_bytes, v.other * h, lines[o] * line[o], (int)len * h, (int)line[o]};   // (`to`: an offset for now)
+            p.pack_bytes += up256((size_t)(lines[o] * line[o]) * 16);
+            v = {nullptr, v.second ? line[o] * E : 1, v.second ? 1 : line[o] * E, v.second, line[o] * E, true};
             w[o] = 16;
         }
     }
@@ -969,8 +987,7 @@ static Plan plan_gemm(int type, View a, View b, long long I, long long J, long l
     p.g.as = a.other; p.g.bs = b.other;
     p.g.avec = !((uintptr_t)a.p & 15) && (a.other % E == 0);
     p.g.bvec = !((uintptr_t)b.p & 15) && (b.other % E == 0);
-    const long long pairs = (K + ks - 1) / ks;
-    long long splits = 1;
+    splits = 1;
     p.small = std::min(w[0], w[1]) == 4;
     if (w[0] && w[1] && I && J) {
         const double us = pick(es == 4, p.small, I, J, pairs, p.tile, splits);
@@ -1059,7 +1076,7 @@ static hipError_t run_gemm(int type, hipStream_t st, Plan& p, void* ws) {
 static Plan plan_forward(const aipt_linear_args* a) {
     const View x = view_of(a->x, a->m, a->k), w = view_of(a->w, a->n, a->k), y = view_of(a->y, a->m, a->n);
     const bool turn = !y.second;
-    Plan p = turn ? plan_gemm(a->type, w, x, a->n, a->m, a->k) : plan_gemm(a->type, x, w, a->m, a->n, a->k);
+    Plan p = turn ? plan_gemm(a->type, w, x, a->n, a->m, a->k, 4) : plan_gemm(a->type, x, w, a->m, a->n, a->k, 4);
     GemmArgs& g = p.g;
     g.c = a->y.data; g.cs = y.other;
     g.bias = a->bias; g.bias_i = turn; g.act = a->act; g.slope = a->slope;
@@ -1126,12 +1143,12 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
     auto flip = [](View v) { std::swap(v.ri, v.rj); v.second = !v.second; return v; };
     if (p.want_dx) {                 // dx[m][k] = sum_n dz[m][n] w[n][k]
         const View w = view_of(a->w, a->n, a->k), o = view_of(a->dx, a->m, a->k);
-        p.dx = o.second ? plan_gemm(a->type, d, flip(w), a->m, a->k, a->n) : plan_gemm(a->type, flip(w), d, a->k, a->m, a->n);
+        p.dx = o.second ? plan_gemm(a->type, d, flip(w), a->m, a->k, a->n, 0) : plan_gemm(a->type, flip(w), d, a->k, a->m, a->n, 0);
         p.dx.g.c = a->dx.data; p.dx.g.cs = o.other;
     }
     if (p.want_dw) {                 // dw[n][k] = sum_m dz[m][n] x[m][k]
         const View x = view_of(a->x, a->m, a->k), o = view_of(a->dw, a->n, a->k);
-        p.dw = o.second ? plan_gemm(a->type, flip(d), flip(x), a->n, a->k, a->m) : plan_gemm(a->type, flip(x), flip(d), a->k, a->n, a->m);
+        p.dw = o.second ? plan_gemm(a->type, flip(d), flip(x), a->n, a->k, a->m, 0) : plan_gemm(a->type, flip(x), flip(d), a->k, a->n, a->m, 0);
         p.dw.g.c = a->dw.data; p.dw.g.cs = o.other;
     }
     p.gemm_bytes = up256(p.want_dx ? p.dx.bytes() : 0) + up256(p.want_dw ? p.dw.bytes() : 0);
