@@ -773,8 +773,11 @@ class AdamW:
             records.append(_ADAMW_TENSOR.pack(p.data_ptr(), g.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), d, 0))
         s, h = self._state, _P()
         ptr = {k: s[k].data_ptr() if k in s else None for k in ("m", "v", "m_scale", "v_scale", "step")}
-        ctx._ck(lib().aipt_adamw_create(ctx._h, b"".join(records), len(records), _types()[kinds.pop()], _types()[copies.pop()], self.state_bits, ptr["m"], ptr["v"],
-                                        ptr["m_scale"], ptr["v_scale"], ptr["step"], self.norm.data_ptr(), self._scratch.data_ptr(), self._scratch.numel(), C.byref(h)))
+        if torch.cuda.is_current_stream_capturing():
+            raise AiptError("adamw: a plan is made, and bound, before a capture")
+        # (in the streams' order: the workspace's zeros, or an earlier plan's last step, come before the table that is written there)
+        ctx._on_stream(lib().aipt_adamw_create, b"".join(records), len(records), _types()[kinds.pop()], _types()[copies.pop()], self.state_bits, ptr["m"], ptr["v"],
+                       ptr["m_scale"], ptr["v_scale"], ptr["step"], self.norm.data_ptr(), self._scratch.data_ptr(), self._scratch.numel(), C.byref(h))
         self.close()
         self._h, self._grads = h, grads
         self._held = [t for t in (*self._params, *grads, *self._copies, *s.values()) if t is not None]

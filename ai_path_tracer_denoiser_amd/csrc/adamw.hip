@@ -244,9 +244,11 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
             }
             q = nq;
         }
-    // The last workgroup advances the step number: every workgroup has read it (and waited for what it read) before it counts itself.  Nothing is
+    // The last workgroup advances the step number: every wave of a workgroup has read it (and waited for what it read) before the barrier behind which
+    // the workgroup counts itself.  Nothing is
     // handed from one to another, so there is no fence: a release writes the L2s back, workgroup by workgroup (50 us here).  One counter
     // for all would take 15 ns a workgroup, one after the other: each counts at one of 32, and the last of those at the last.
+    __syncthreads();
     if (threadIdx.x == 0) {
         auto count = [&](int at) { return __hip_atomic_fetch_add(a.ticket + at * 32, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
         const unsigned c = blockIdx.x % COUNTERS, mine = (gridDim.x - c + COUNTERS - 1) / COUNTERS, used = min((unsigned)COUNTERS, gridDim.x);

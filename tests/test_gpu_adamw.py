@@ -281,3 +281,40 @@ def test_refusals():
     plan.close()
     with pytest.raises(api.AiptError, match="closed"):
         plan.update(LR)
+
+
+def test_plan_made_while_the_streams_are_busy():
+    """The table is written behind the workspace's zeros, and behind the steps of the plan before, whatever the streams are."""
+    sizes = [70000, 3, 1025]
+    ctx, gen = api.Context(0), generator(31)
+    start, grads = tensors(gen, sizes, 0.1), [tensors(gen, sizes, 1e-2), tensors(gen, sizes, 1e-2)]
+
+    def run(c, wait):
+        p = [t.clone() for t in start]
+        torch.cuda.synchronize()
+        if wait:
+            big = torch.zeros(1 << 28, device="cuda")
+            for _ in range(20):
+                big.add_(1.0)
+        plan = c.adamw(p, grads[0], weight_decay=0.01)
+        for k in range(4):
+            if k == 2:
+                plan.bind(grads[1])
+            plan.update(LR)
+        torch.cuda.synchronize()
+        return p, int(plan.state()["step"])
+
+    (a, s), (b, t) = run(ctx, True), run(context(), False)
+    assert s == t == 4 and all(torch.equal(x, y) for x, y in zip(a, b))
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    captured = api.Context(0, stream=side.cuda_stream)
+    p = [t.clone() for t in start]
+    plan = captured.adamw(p, grads[0])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        plan.update(LR)
+        with pytest.raises(api.AiptError, match="before a capture"):
+            plan.bind(grads[1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(plan.state()["step"]) == 1
