@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256) void gemm_any(const GemmArgs g) {
     int job = blockIdx.x;
     const int split = job % g.splits; job /= g.splits;
     const int i0 = job / g.tiles_j * GT, j0 = job % g.tiles_j * GT;
-    const int k0 = split * g.k_split, k1 = min(g.K, k0 + g.k_split);
+    const int k0 = split * g.k_split, k1 = (int)min((long long)g.K, (long long)k0 + g.k_split);
     f32x4 acc[2][2] = {};
     const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
     for (int k = k0; k < k1; k += KS) {
@@ -365,7 +365,7 @@ __device__ __forceinline__ void tile_of(const GemmArgs& g, const int block, cons
     // ... in columns of 8 tiles
     const int band = 8 * g.tiles_j, b0 = job / band * 8, bh = min(8, g.tiles_i - b0);
     const int i0 = (b0 + (job % band) % bh) * TI, j0 = (job % band) / bh * TJ;
-    const int k0 = split * g.k_split, k1 = min(g.K, k0 + g.k_split), KP = 128 / (int)sizeof(T), n = (k1 - k0 + KP - 1) / KP;
+    const int k0 = split * g.k_split, k1 = (int)min((long long)g.K, (long long)k0 + g.k_split), KP = 128 / (int)sizeof(T), n = (k1 - k0 + KP - 1) / KP;
 
     TileLoad<sizeof(T), AK, TI, NT, W> la;
     TileLoad<sizeof(T), BK, TJ, NT, W> lb;
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g, const PackAr
         }
     };
     if constexpr (TURNED) {
-        const int lane = threadIdx.x & 63, l1 = min(g.N, tn * 64 + 64), c0 = tm * g.high, c1 = min(max(g.M, g.line), c0 + g.high);
+        const int lane = threadIdx.x & 63, l1 = min(g.N, tn * 64 + 64), c0 = tm * g.high, c1 = (int)min((long long)max(g.M, g.line), (long long)c0 + g.high);
         for (int l = tn * 64 + (threadIdx.x >> 6); l < l1; l += 4) {
             const T* dyp = (const T*)g.dy + l * g.dys;
             const T* zp = (const T*)g.z + l * g.zj;
@@ -744,7 +744,7 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g, const PackAr
         }
     } else {
         const int x = threadIdx.x % g.across, y = threadIdx.x / g.across, down = 256 / g.across;
-        const int c = (tn * g.across + x) * V, l0 = tm * g.high + y, l1 = min(g.M, (tm + 1) * g.high);
+        const int c = (tn * g.across + x) * V, l0 = tm * g.high + y, l1 = (int)min((long long)g.M, (tm + 1ll) * g.high);
         float sum[V] = {};
         if (c < max(g.N, g.line)) {
             const T* dyp = (const T*)g.dy + l0 * g.dys + c;
@@ -1127,9 +1127,9 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         g.tiles_n = (int)(turned ? (a->n + 63) / 64 : (wide + g.across * v - 1) / (g.across * v));
         // some 2 048 workgroups, each with 4 rows a thread at least, and no more than 1 024 partial sums a column
         const long long unit = turned ? 64 * v : 256 / g.across, fair = (a->m * g.tiles_n + 2047) / 2048;
-        const long long high = (std::max({4 * unit, fair, (a->m + 1023) / 1024}) + unit - 1) / unit * unit;
+        const long long high = std::min((std::max({4 * unit, fair, (a->m + 1023) / 1024}) + unit - 1) / unit * unit, 0x40000000ll);
         const long long tm = (a->m + high - 1) / high;
-        g.high = (int)std::min(high, 0x40000000ll);
+        g.high = (int)high;
         p.parts = (int)tm;
         if (p.want_db && tm > 1) p.part_bytes = up256((size_t)tm * a->n * sizeof(float));
         g.dy = a->dy.data; g.z = a->preact.data; g.dz = p.make_dz ? d.p : nullptr;

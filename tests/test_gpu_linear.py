@@ -311,3 +311,19 @@ def test_captured_and_replayed():
     with pytest.raises(api.AiptError, match="default stream"):
         with torch.cuda.graph(default):
             step(context(), eager)
+
+
+# Rows whose numbers come close to 2^31: the last of what is added lies there.  Integers up to 256, which bf16 holds: exact.
+@pytest.mark.parametrize("layout", ["rows", "planar"])
+def test_backward_of_two_thousand_million_rows(layout):
+    m, n = 2 ** 31 - 5000, 2
+    shape = (m, n) if layout == "rows" else (n, m)
+    turn = (lambda v: v) if layout == "rows" else (lambda v: v.t())
+    dy, z, x = turn(torch.zeros(shape, device="cuda", dtype=torch.bfloat16)), turn(torch.full(shape, -1.0, device="cuda", dtype=torch.bfloat16)), torch.zeros(m, 1, device="cuda", dtype=torch.bfloat16)
+    at = torch.tensor([0, 1, 4097, 2 ** 20 + 3, 2 ** 30 - 1, 2 ** 30, 3 * 2 ** 29 + 77, m - 2 ** 21, m - 70000, m - 300, m - 65, m - 64, m - 9, m - 2, m - 1], device="cuda")
+    dy[at, 0], dy[at, 1] = 2.0, 4.0
+    x[at, 0] = (torch.arange(len(at), device="cuda") % 5 + 1).to(torch.bfloat16)
+    dw, db = torch.full((n, 1), 9.0, device="cuda", dtype=torch.bfloat16), torch.full((n,), 9.0, device="cuda", dtype=torch.bfloat16)
+    context().linear_backward(dy, x, None, preact=z, act="leaky", slope=0.5, dw=dw, dbias=db)
+    total = float(x[at, 0].sum())
+    assert dw.flatten().tolist() == [total, 2 * total] and db.tolist() == [float(len(at)), 2.0 * len(at)]
