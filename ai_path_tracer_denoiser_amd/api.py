@@ -575,7 +575,7 @@ class Context:
     # the same of several at once: a call of little work is bound by what is done here for each tensor
     def _vectors(self, dtype, n, **of):
         dev, shape = self.device, (n,)
-        return [0 if t is None else t.data_ptr() if t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.stride() == (1,)
+        return [0 if t is None else t.data_ptr() if t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.is_contiguous()
                 else self._vector(name, t, dtype, n) for name, t in of.items()]
 
     def linear(self, x, w, y, bias=None, residual=None, preact=None, act: str = "none", slope: float = 0.1):
@@ -634,7 +634,7 @@ class Context:
     def _gates(self, name, t, dtype, c, groups):
         if t is None:
             return 0
-        if t.dtype is not dtype or t.get_device() != self.device or t.shape != (groups, c) or t.stride() != (c, 1):
+        if t.dtype is not dtype or t.get_device() != self.device or t.shape != (groups, c) or not t.is_contiguous():
             if t.dim() != 2 or not t.is_contiguous():
                 raise AiptError(f"{name}: {tuple(t.shape)} contiguous [groups, channels] is wanted")
             self._want(name, t, dtype, groups, c)
@@ -643,7 +643,7 @@ class Context:
     def _stats(self, stats, rows):
         if stats is None:
             return 0
-        if _TYPES.get(stats.dtype) != TYPE_F32 or stats.get_device() != self.device or stats.shape != (rows, 4) or stats.stride() != (4, 1):
+        if _TYPES.get(stats.dtype) != TYPE_F32 or stats.get_device() != self.device or stats.shape != (rows, 4) or not stats.is_contiguous():
             import torch
             self._want("stats", stats, torch.float32, rows, 4)
             if not stats.is_contiguous():
@@ -781,7 +781,8 @@ class AdamW:
         self.close()
         self._h, self._grads = h, grads
         self._held = [t for t in (*self._params, *grads, *self._copies, *s.values()) if t is not None]
-        self._at = [t.data_ptr() for t in self._held]
+        self._address = torch.Tensor.data_ptr
+        self._at = list(map(self._address, self._held))
 
     def state(self) -> dict:
         """The state tensors themselves, to be saved, or to go on from in another plan."""
@@ -792,7 +793,7 @@ class AdamW:
         the chances by which 8-bit state is rounded.  A captured step replays its lr; the step number goes on with every replay."""
         if not self._h:
             raise AiptError("adamw: the plan is closed")
-        if [t.data_ptr() for t in self._held] != self._at:
+        if list(map(self._address, self._held)) != self._at:
             raise AiptError("adamw: a tensor's storage has moved: bind() the plan anew")
         if max_norm is not None and not max_norm > 0:
             raise AiptError(f"adamw: max_norm {max_norm}")

@@ -740,7 +740,7 @@ int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* a, 
     }
     if (!a->rows) {                                          // nothing to add up
         AIPT_NEED_CTX(ctx);
-    aipt::DeviceScope dev(ctx->device);
+        aipt::DeviceScope dev(ctx->device);
         AIPT_HIP(ctx, dev.err);
         for (int o = 2; o < 8; o++) AIPT_HIP(ctx, aipt::zero_fill(ctx->stream, out[o].data, (size_t)(out[o].lines * out[o].len)));
         return AIPT_OK;
