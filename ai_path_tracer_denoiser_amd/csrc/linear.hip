@@ -744,7 +744,8 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g, const PackAr
         }
     } else {
         const int x = threadIdx.x % g.across, y = threadIdx.x / g.across, down = 256 / g.across;
-        const int c = (tn * g.across + x) * V, l0 = tm * g.high + y, l1 = (int)min((long long)g.M, (tm + 1ll) * g.high);
+        int l0 = tm * g.high + y;
+        const int c = (tn * g.across + x) * V, l1 = (int)min((long long)g.M, (tm + 1ll) * g.high);
         float sum[V] = {};
         if (c < max(g.N, g.line)) {
             const T* dyp = (const T*)g.dy + l0 * g.dys + c;
@@ -752,38 +753,37 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g, const PackAr
             T* dzp = (T*)g.dz + l0 * g.dzs + c;
             const long long dyd = down * g.dys, zd = down * g.zi, dzd = down * g.dzs;
             const bool in = c < g.N, out = g.dz && c < g.line;
-            // U rows' loads before the first one's result (which might, for all the compiler knows, be what the next row reads)
+            // U rows' loads before the first one's result (which might, for all the compiler knows, be what the next row reads); the last rows one by one
             constexpr int U = V * sizeof(T) == 16 ? 2 : 4;
-            for (int l = l0; l < l1; l += U * down) {
-                E dy[U], z[U];
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (in && l + u * down < l1) {
-                        dy[u] = *(const E*)(dyp + u * dyd);
-                        if (g.act != AIPT_ACT_NONE) z[u] = *(const E*)(zp + u * zd);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (l + u * down >= l1) break;
-                    float d[V] = {};
+            auto rows = [&](auto uv, int end) {
+                constexpr int UU = decltype(uv)::value;
+                for (; l0 + (UU - 1) * down < end; l0 += UU * down) {
+                    E dy[UU] = {}, z[UU] = {};
                     if (in) {
 #pragma unroll
-                        for (int i = 0; i < V; i++) {
-                            d[i] = (float)dy[u].v[i];
-                            if (g.act != AIPT_ACT_NONE) d[i] *= act_slope_of((float)z[u].v[i], g.act, g.slope);
-                            sum[i] += d[i];
+                        for (int u = 0; u < UU; u++) dy[u] = *(const E*)(dyp + u * dyd);
+                        if (g.act != AIPT_ACT_NONE) {
+#pragma unroll
+                            for (int u = 0; u < UU; u++) z[u] = *(const E*)(zp + u * zd);
                         }
                     }
-                    if (out) {
+#pragma unroll
+                    for (int u = 0; u < UU; u++) {
                         E o;
 #pragma unroll
-                        for (int i = 0; i < V; i++) o.v[i] = (T)d[i];
-                        *(E*)(dzp + u * dzd) = o;
+                        for (int i = 0; i < V; i++) {
+                            float d = (float)dy[u].v[i];
+                            if (g.act != AIPT_ACT_NONE) d *= act_slope_of((float)z[u].v[i], g.act, g.slope);
+                            sum[i] += d;
+                            o.v[i] = (T)d;
+                        }
+                        if (out) *(E*)(dzp + u * dzd) = o;
                     }
+                    dyp += UU * dyd; zp += UU * zd; dzp += UU * dzd;
                 }
-                dyp += U * dyd; zp += U * zd; dzp += U * dzd;
-            }
+            };
+            rows(std::integral_constant<int, U>{}, l1);
+            rows(std::integral_constant<int, 1>{}, l1);
         }
         if (!g.part && !g.sum) return;
 #pragma unroll
@@ -1124,6 +1124,9 @@ static GradPlan plan_backward(const aipt_linear_grad_args* a, char* ws) {
         const long long wide = std::max<long long>(a->n, turned ? 0 : g.line), v = p.dz_v;
         g.across = 4;
         while (g.across < 256 && g.across * v < wide) g.across *= 2;
+        // fewer lanes a row, and more workgroups side by side, where that leaves fewer idle (3431 x 2304 fp16, 288 lanes' worth: 20 us by 256, 15 by 32)
+        auto lanes = [&](int across) { return (wide + across * v - 1) / (across * v) * across; };
+        for (int across = g.across / 2; across >= 32; across /= 2) if (lanes(across) * 11 < lanes(g.across) * 10) g.across = across;
         g.tiles_n = (int)(turned ? (a->n + 63) / 64 : (wide + g.across * v - 1) / (g.across * v));
         // some 2 048 workgroups, each with 4 rows a thread at least, and no more than 1 024 partial sums a column
         const long long unit = turned ? 64 * v : 256 / g.across, fair = (a->m * g.tiles_n + 2047) / 2048;
