@@ -672,8 +672,13 @@ __device__ inline void pack(const PackArgs& g, long long block, long long blocks
             const int k = (int)(c - l * m.line) * 8;
             const unsigned short* s = m.p + l * m.stride + k;
             Chunk<unsigned short> q;
+            if (k + 8 <= m.len) {                            // 16 bytes from anywhere: the chip loads them so
+                struct __attribute__((packed, aligned(2))) Any { unsigned v[4]; };
+                q = __builtin_bit_cast(Chunk<unsigned short>, *(const Any*)s);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) q.v[e] = k + e < m.len ? s[e] : (unsigned short)0;
+                for (int e = 0; e < 8; e++) q.v[e] = k + e < m.len ? s[e] : (unsigned short)0;
+            }
             m.to[c] = q;
         }
     }
