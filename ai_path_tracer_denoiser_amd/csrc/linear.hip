@@ -31,7 +31,7 @@ struct GemmArgs {
     void* pre;
     long long pi, pj;
     int turned;                      // gemm_rows: A and B are the result's j and i
-    int cv;                          // elements that move together: 8 (rows of c, res and pre on 16 bytes, j contiguous), 2 (on two elements) or 1
+    int cv;                          // elements that move together: 8 (rows of c, res and pre on 16 bytes, j contiguous), 9: 8 from anywhere on, or 1
 };
 
 // 1 / (1 + e^-z) by the chip's exponential and reciprocal (an ulp each): z is within 2^-24 |z| of what it should be in the exponent
@@ -315,7 +315,7 @@ template <typename T, bool KC, int R, int N> struct TileRead {
 };
 
 // eight neighbours of a row: bias, activation, residual, 16-byte stores
-template <typename T, int ACT> __device__ inline void epilogue8(const GemmArgs& g, int i, int j, float* z, const float* bias_j) {
+template <typename T, int ACT, bool ANY> __device__ inline void epilogue8(const GemmArgs& g, int i, int j, float* z, const float* bias_j) {
     float b[8];
     if (g.bias_i) {
         const float v = g.bias ? (float)((const T*)g.bias)[i] : 0.f;
@@ -326,23 +326,31 @@ template <typename T, int ACT> __device__ inline void epilogue8(const GemmArgs& 
         for (int e = 0; e < 8; e++) b[e] = bias_j[e];
     }
     struct alignas(16) Oct { T v[8]; } q;
+    struct __attribute__((packed, aligned(sizeof(T)))) Loose { unsigned w[2 * sizeof(T)]; };
+    auto store = [&](T* p) {
+        if constexpr (ANY) *(Loose*)p = __builtin_bit_cast(Loose, q);
+        else *(Oct*)p = q;
+    };
 #pragma unroll
     for (int e = 0; e < 8; e++) z[e] += b[e];
     if (g.pre) {
 #pragma unroll
         for (int e = 0; e < 8; e++) q.v[e] = (T)z[e];
-        *(Oct*)((T*)g.pre + i * g.pi + j) = q;
+        store((T*)g.pre + i * g.pi + j);
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) z[e] = act_of(z[e], ACT, g.slope);
     if (g.res) {
-        const Oct r = *(const Oct*)((const T*)g.res + i * g.ri + j);
+        const T* p = (const T*)g.res + i * g.ri + j;
+        Oct r;
+        if constexpr (ANY) r = __builtin_bit_cast(Oct, *(const Loose*)p);
+        else r = *(const Oct*)p;
 #pragma unroll
         for (int e = 0; e < 8; e++) z[e] += (float)r.v[e];
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) q.v[e] = (T)z[e];
-    *(Oct*)((T*)g.c + i * g.cs + j) = q;
+    store((T*)g.c + i * g.cs + j);
 }
 
 template <int TI, int TJ, int WI, int WJ, int S> constexpr int tile_lds() {       // bytes: the ring, or the slabs that results go through
@@ -466,42 +474,26 @@ __device__ __forceinline__ void tile_of(const GemmArgs& g, const int block, cons
     float bias_j[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) bias_j[e] = g.bias && !g.bias_i && g.splits == 1 && j + e < g.J ? (float)((const T*)g.bias)[j + e] : 0.f;
-    // rows that begin anywhere: neighbouring lanes, EV neighbouring elements each
-    auto narrow = [&](auto ev, int s) {
-        constexpr int EV = decltype(ev)::value, LN = WTJ / EV < 64 ? WTJ / EV : 64, RS = 64 / LN;
-        struct alignas(EV * sizeof(T)) E { T v[EV]; };
+    // one by one, neighbouring lanes neighbouring elements
+    auto narrow = [&](int s) {
+        constexpr int LN = WTJ < 64 ? WTJ : 64, RS = 64 / LN;
 #pragma unroll
-        for (int h = 0; h < WTJ / (EV * LN); h++) {
-            const int c = (h * LN + lane % LN) * EV, jj = j0 + wj + c;
-            if (jj >= g.J) continue;                         // (EV = 2: J is even)
-            float bias[EV];
-#pragma unroll
-            for (int e = 0; e < EV; e++) bias[e] = g.bias && !g.bias_i ? (float)((const T*)g.bias)[jj + e] : 0.f;
+        for (int h = 0; h < WTJ / LN; h++) {
+            const int c = h * LN + lane % LN, jj = j0 + wj + c;
+            if (jj >= g.J) continue;
+            const float bias = g.bias && !g.bias_i ? (float)((const T*)g.bias)[jj] : 0.f;
             const int r0 = lane / LN, ii = i0 + wi + s * SLAB + r0, end = min(SLAB, g.I - (i0 + wi + s * SLAB));
             T* o = (T*)g.c + (long long)ii * g.cs + jj;
             T* pre = g.pre ? (T*)g.pre + ii * g.pi + jj * g.pj : nullptr;
             const T* res = g.res ? (const T*)g.res + ii * g.ri + jj * g.rj : nullptr;
 #pragma unroll 4
             for (int r = r0; r < end; r += RS, o += RS * g.cs) {
-                float z[EV];
-#pragma unroll
-                for (int e = 0; e < EV; e++) z[e] = *(AIPT_LDS float*)(slab + r * (WTJ * 4) + (((c >> 2) ^ (r & XM)) * 16) + (c & 3) * 4 + e * 4);
-                E q;
-                const float bi = g.bias && g.bias_i ? (float)((const T*)g.bias)[ii - r0 + r] : 0.f;
-#pragma unroll
-                for (int e = 0; e < EV; e++) { z[e] += g.bias_i ? bi : bias[e]; q.v[e] = (T)z[e]; }
-                if (pre) { *(E*)pre = q; pre += RS * g.pi; }
-#pragma unroll
-                for (int e = 0; e < EV; e++) z[e] = act_of(z[e], g.act, g.slope);
-                if (res) {
-                    const E v = *(const E*)res;
-#pragma unroll
-                    for (int e = 0; e < EV; e++) z[e] += (float)v.v[e];
-                    res += RS * g.ri;
-                }
-#pragma unroll
-                for (int e = 0; e < EV; e++) q.v[e] = (T)z[e];
-                *(E*)o = q;
+                float z = *(AIPT_LDS float*)(slab + r * (WTJ * 4) + (((c >> 2) ^ (r & XM)) * 16) + (c & 3) * 4);
+                z += g.bias && g.bias_i ? (float)((const T*)g.bias)[ii - r0 + r] : bias;
+                if (pre) { *pre = (T)z; pre += RS * g.pi; }
+                z = act_of(z, g.act, g.slope);
+                if (res) { z += (float)*res; res += RS * g.ri; }
+                *o = (T)z;
             }
         }
     };
@@ -514,7 +506,7 @@ __device__ __forceinline__ void tile_of(const GemmArgs& g, const int block, cons
                 const int r = p * 16 + (lane & 15), c = q * 4 + (lane >> 4);
                 *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & XM)) * 16)) = acc[s * (SLAB / 16) + p][q];
             }
-        auto rows = [&](auto done) {
+        auto rows_by = [&](auto anywhere, int je, auto done) {
             for (int r = lane / LR; r < SLAB; r += RPI) {
                 const int i = i0 + wi + s * SLAB + r;
                 if (i >= g.I || j >= g.J) continue;
@@ -522,9 +514,19 @@ __device__ __forceinline__ void tile_of(const GemmArgs& g, const int block, cons
                 const int c = lane % LR * 2;
                 *(f32x4*)z = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + ((c ^ (r & XM)) * 16));
                 *(f32x4*)(z + 4) = *(AIPT_LDS f32x4*)(slab + r * (WTJ * 4) + (((c + 1) ^ (r & XM)) * 16));
+                if constexpr (decltype(anywhere)::value) {
+                    if (je != j) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int k = je - (j0 + wj) + e;
+                            z[e] = *(AIPT_LDS float*)(slab + r * (WTJ * 4) + (((k >> 2) ^ (r & XM)) * 16) + (k & 3) * 4);
+                        }
+                    }
+                }
                 done(i, z);
             }
         };
+        auto rows = [&](auto done) { rows_by(integral_constant<bool, false>{}, j, done); };
         if (g.splits > 1) rows([&](int i, float* z) {
             float* o = g.partial + ((long long)split * g.I + i) * g.J + j;
             if (j + 8 <= g.J && !(g.J & 3)) { *(f32x4*)o = *(f32x4*)z; *(f32x4*)(o + 4) = *(f32x4*)(z + 4); }
@@ -533,17 +535,26 @@ __device__ __forceinline__ void tile_of(const GemmArgs& g, const int block, cons
                 for (int e = 0; e < 8; e++) if (j + e < g.J) o[e] = z[e];
             }
         });
-        else if (g.cv == 2) narrow(integral_constant<int, 2>{}, s);
-        else if (g.cv == 1) {
-            narrow(integral_constant<int, 1>{}, s);
-        } else if (!whole) rows([&](int i, float* z) {
+        else if (g.cv == 1 || (g.cv == 9 && g.J - (j0 + wj) < 8)) narrow(s);
+        else if (g.cv == 8 && !whole) rows([&](int i, float* z) {
 #pragma unroll
             for (int e = 0; e < 8; e++) if (j + e < g.J) epilogue<T>(g, i, j + e, z[e]);
         });
-        else if (g.act == AIPT_ACT_NONE) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_NONE>(g, i, j, z, bias_j); });
-        else if (g.act == AIPT_ACT_LEAKY) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_LEAKY>(g, i, j, z, bias_j); });
-        else if (g.act == AIPT_ACT_SILU) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_SILU>(g, i, j, z, bias_j); });
-        else rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_GELU>(g, i, j, z, bias_j); });
+        else if (g.cv == 8) {
+            if (g.act == AIPT_ACT_NONE) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_NONE, false>(g, i, j, z, bias_j); });
+            else if (g.act == AIPT_ACT_LEAKY) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_LEAKY, false>(g, i, j, z, bias_j); });
+            else if (g.act == AIPT_ACT_SILU) rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_SILU, false>(g, i, j, z, bias_j); });
+            else rows([&](int i, float* z) { epilogue8<T, AIPT_ACT_GELU, false>(g, i, j, z, bias_j); });
+        } else {                     // rows that begin anywhere: a row's last eight end with it, and some of them are the neighbouring lane's as well (the same bits)
+            const int je = whole ? j : g.J - 8;
+#pragma unroll
+            for (int e = 0; e < 8; e++) bias_j[e] = g.bias && !g.bias_i ? (float)((const T*)g.bias)[je + e] : 0.f;
+            auto rows_any = [&](auto done) { rows_by(integral_constant<bool, true>{}, je, done); };
+            if (g.act == AIPT_ACT_NONE) rows_any([&](int i, float* z) { epilogue8<T, AIPT_ACT_NONE, true>(g, i, je, z, bias_j); });
+            else if (g.act == AIPT_ACT_LEAKY) rows_any([&](int i, float* z) { epilogue8<T, AIPT_ACT_LEAKY, true>(g, i, je, z, bias_j); });
+            else if (g.act == AIPT_ACT_SILU) rows_any([&](int i, float* z) { epilogue8<T, AIPT_ACT_SILU, true>(g, i, je, z, bias_j); });
+            else rows_any([&](int i, float* z) { epilogue8<T, AIPT_ACT_GELU, true>(g, i, je, z, bias_j); });
+        }
     }
 }
 
@@ -1040,13 +1051,13 @@ template <typename T> static void (*gemm_of(const Plan& p))(GemmArgs) {
     }
     return p.ak ? (p.bk ? gemm_any<T, true, true> : gemm_any<T, true, false>) : (p.bk ? gemm_any<T, false, true> : gemm_any<T, false, false>);
 }
-// how many elements the epilogue may move together
+// How many elements the epilogue may move together.  A row's last eight may be two lanes', so that a residual in place is not read by eights
+// from anywhere.  942080 x 143 fp16: 322 us one by one, 178 by eights; 235520 x 58 bf16 37 by twos, 31; 1375 x 303 fp16 11.1, 9.1.
 static int row_unit(int es, const GemmArgs& g) {
-    auto on = [&](int bytes) {
-        const long long e = bytes / es;
-        return !(((uintptr_t)g.c | (uintptr_t)g.res | (uintptr_t)g.pre) & (bytes - 1)) && g.cs % e == 0 && (!g.res || (g.rj == 1 && g.ri % e == 0)) && (!g.pre || (g.pj == 1 && g.pi % e == 0));
-    };
-    return on(16) ? 8 : g.J % 2 == 0 && on(2 * es) ? 2 : 1;
+    const long long e = 16 / es;
+    if ((g.res && g.rj != 1) || (g.pre && g.pj != 1)) return 1;
+    if (!(((uintptr_t)g.c | (uintptr_t)g.res | (uintptr_t)g.pre) & 15) && g.cs % e == 0 && (!g.res || g.ri % e == 0) && (!g.pre || g.pi % e == 0)) return 8;
+    return g.res == g.c ? 1 : 9;
 }
 
 // the product itself, its operands' copies being made: where they lie and the partial sums

@@ -327,3 +327,19 @@ def test_backward_of_two_thousand_million_rows(layout):
     context().linear_backward(dy, x, None, preact=z, act="leaky", slope=0.5, dw=dw, dbias=db)
     total = float(x[at, 0].sum())
     assert dw.flatten().tolist() == [total, 2 * total] and db.tolist() == [float(len(at)), 2.0 * len(at)]
+
+
+# Rows that begin at any element, their last ones short of a tile, a wave or eight elements: what lies between and behind them stays as it was.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [70, 20000])
+@pytest.mark.parametrize("n", [7, 8, 9, 31, 33, 39, 41, 57, 63, 65, 71, 73, 127, 129, 143, 303])
+def test_rows_that_begin_anywhere(n, m, dtype):
+    gen = generator(n * 7 + m)
+    k = 64
+    x, w, b, r = matrix(gen, m, k, dtype), matrix(gen, n, k, dtype, scale=k ** -0.5), matrix(gen, 1, n, dtype)[0], matrix(gen, m, n, dtype, pad=1, offset=1)
+    check_forward(x, w, b, r, ACTS[n % 4], pad=n % 3, offset=1)
+    y = r.clone()
+    context().linear(x, w, y, bias=b, residual=y, act="gelu")
+    yr, yb, _, _ = forward_reference(x, w, b, r, "gelu")
+    within(y, yr, yb)
+    check_backward(*(matrix(gen, m, c, dtype) for c in (k, n)), matrix(gen, k, n, dtype, scale=n ** -0.5), matrix(gen, m, k, dtype), "silu", pad=n % 2, offset=1)
