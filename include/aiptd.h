@@ -237,7 +237,8 @@ int aipt_trace_first_hit_materials(aipt_ctx* ctx, int* h_mat, int n);
  * itself.  A host that runs such third-party kernels on the same GPU at the same time (torch ops on other streams, another
  * process) either orders them against aipt_* work (aipt_sync, events on the context's stream), keeps them on disjoint CUs
  * (hipExtStreamCreateWithCUMask), or opts out of the trigger with aipt_denoise_set_impl(ctx, AIPT_DN_IMPL_MFMA): fp32-input
- * MFMAs never cause it (at about half the denoiser throughput). */
+ * MFMAs never cause it (at about half the denoiser throughput).  The 16-bit matrix instructions of aipt_linear and
+ * aipt_linear_backward are to be treated alike: order such kernels against them, or keep them on other CUs. */
 /* blob: flat weight file, format in ai_path_tracer_denoiser_amd/arch.py (header + 28 x {W,b,gamma,beta,mean,var}).
  * Loading weights resets the recurrent hidden state (the next AIPT_DN_HIDDEN_CARRY frame starts from zeros). */
 int aipt_denoise_load_weights(aipt_ctx* ctx, const void* blob, size_t bytes);
