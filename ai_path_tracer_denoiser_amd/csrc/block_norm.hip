@@ -12,7 +12,7 @@
 //     A = sum g t yhat,  B = sum g t,  Q = sum_(rows of a gate) t (w1 yhat + b1),  W = sum dz hhat,  V = sum dz
 // they are  dw1 = s A,  db1 = s B,  ds = w1 A + b1 B,  dgate = s Q,  dw2 = W,  db2 = V: four (five) sums a column, which each
 // workgroup keeps in registers over the rows it handles and writes once; a second, small launch adds those in a fixed order.
-// Measured, 16 384 x 4 096 bf16: forward 101 - 112 us (106 at a large copy's 5.05 TB/s), backward 172 us and 8 for the sums (160).
+// Measured, 16 384 x 4 096 bf16: forward 101 - 112 us (106 at a large copy's 5.05 TB/s), backward 167 us and 6 for the sums (160).
 #include "layer_ops.h"
 
 namespace aipt {
@@ -579,12 +579,13 @@ template <typename T, bool LAYER> static void (*bwd_kernel(NormShape s, bool who
 #undef AIPT_BWD
 }
 
-// Parts of the backward pass (a workgroup each): 1 024 of 256 threads, 256 of 1 024, none shorter than 4 rows for each row handled at a time.  Gates
-// fewer than that are split into parts; more, and a part takes whole gates.
+// Parts of the backward pass (a workgroup each): two a CU, one where a lane's columns fill its registers or the workgroup is larger (100 000 x 512 bf16
+// layer 142 us with 512 parts, 171 with 768, 158 with 1 024; 16 384 x 4 096 bf16 rms 173 with 256, 182 with 512), none shorter than 4 rows for each
+// row handled at a time.  Gates fewer than that are split into parts; more, and a part takes whole gates.
 struct NormParts { long long parts, span, per_gate_parts; };
 static bool norm_whole(long long groups) { return groups >= 512; }
-static NormParts norm_parts(long long rows, long long groups, int lanes) {
-    const long long want = lanes <= 64 ? 1024 : lanes == 256 ? 512 : 256, at_once = lanes < 256 ? 256 / lanes : 1;
+static NormParts norm_parts(long long rows, long long groups, NormShape s) {
+    const long long want = s.lanes < 256 || (s.lanes == 256 && s.n * s.v <= 8) ? 512 : 256, at_once = s.lanes < 256 ? 256 / s.lanes : 1;
     const long long per = std::max(1ll, rows / groups);
     NormParts p;
     if (norm_whole(groups)) {
@@ -696,7 +697,7 @@ int aipt_block_norm_backward_workspace(aipt_ctx* ctx, const aipt_block_norm_grad
     for (int v : {1, 2, 16 / es}) {
         if (v == 2 && es == 4) continue;
         const aipt::NormShape s = aipt::bwd_shape(es, a->c, v, aipt::norm_whole(groups));
-        const aipt::NormParts p = aipt::norm_parts(std::max(1ll, a->rows), groups, s.lanes);
+        const aipt::NormParts p = aipt::norm_parts(std::max(1ll, a->rows), groups, s);
         most = std::max(most, (size_t)p.parts * 5 * a->c * sizeof(float));
     }
     *bytes = most;
@@ -752,7 +753,7 @@ int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* a, 
     const bool whole = aipt::norm_whole(groups);
     const aipt::NormShape s = aipt::bwd_shape(es, a->c, v, whole);
     const int threads = std::max(256, s.lanes);
-    const aipt::NormParts p = aipt::norm_parts(a->rows, groups, s.lanes);
+    const aipt::NormParts p = aipt::norm_parts(a->rows, groups, s);
     const size_t blocks = (size_t)p.parts;
     const bool part = sums || (a->dgate && p.per_gate_parts);
     const size_t need = part ? blocks * 5 * a->c * sizeof(float) : 0;
