@@ -526,12 +526,20 @@ class Context:
             return self._ck(rc) if rc else None
         import torch
         now = torch.cuda.current_stream(self.device)
-        if not self._stream and torch.cuda.is_current_stream_capturing():
+        if not self._stream and self._capturing():
             raise AiptError("a context on the default stream cannot take part in a capture: make one with stream=<the capturing stream's handle>")
         self._ext.wait_stream(now)
         rc = entry(self._h, *args)
         now.wait_stream(self._ext)
         self._ck(rc)
+
+    def _capturing(self) -> bool:
+        """Is torch's current stream of this device being captured?"""
+        import torch
+        if torch._C._cuda_getDevice() == self.device:
+            return torch._C._cuda_isCurrentStreamCapturing()
+        with torch.cuda.device(self.device):
+            return torch._C._cuda_isCurrentStreamCapturing()
 
     def _scratch(self, entry, record):
         """(memory or None, its address, bytes) of an operator's workspace: torch's, so that a captured graph keeps its own"""
@@ -717,7 +725,8 @@ class AdamW:
     state: None (zeros, step 0) or the dict that state() of an earlier plan of the same sizes returned, which goes on being updated in place:
     step int32 [1]; m and v float32 (state_bits 32), or m, v float8_e4m3fn with m_scale, v_scale float32 for each 256 elements (state_bits
     8; v holds the second moment's root); tensor i begins at element 256 * (number of 256-blocks of the tensors before it).
-    norm: float32 [1], the gradients' norm at the last update that clipped."""
+    norm: float32 [1], the gradients' norm at the last update that clipped.
+    A graph that captured update() steps the tensors that were bound then, whatever is bound later, as long as this object lives."""
 
     def __init__(self, ctx, params, grads, copies=None, weight_decay=0.01, state_bits=32, state=None):
         import torch
@@ -750,11 +759,11 @@ class AdamW:
                 raise AiptError(f"adamw: state {k} is not contiguous")
         self._state = dict(state)
         self.norm = torch.zeros(1, device=dev)
-        self._scratch = torch.zeros(need, device=dev, dtype=torch.uint8)
+        self._need, self._captured, self._kept = need, None, []
         self.bind(grads)
 
     def bind(self, grads):
-        """Bind the plan to these gradients, and to where the parameters and copies lie now."""
+        """Bind the plan to these gradients, and to where the parameters and copies lie now.  Waits for the stream; not in a capture."""
         import torch
         grads, ctx = list(grads), self.ctx
         if len(grads) != len(self._params):
@@ -773,13 +782,20 @@ class AdamW:
             records.append(_ADAMW_TENSOR.pack(p.data_ptr(), g.data_ptr(), 0 if c is None else c.data_ptr(), p.numel(), d, 0))
         s, h = self._state, _P()
         ptr = {k: s[k].data_ptr() if k in s else None for k in ("m", "v", "m_scale", "v_scale", "step")}
-        if torch.cuda.is_current_stream_capturing():
+        if ctx._capturing():
             raise AiptError("adamw: a plan is made, and bound, before a capture")
-        # (in the streams' order: the workspace's zeros, or an earlier plan's last step, come before the table that is written there)
+        # Each binding has a table of its own: a graph that captured a step reads that binding's, and steps of it may still run.
+        # (in the streams' order: the table is written behind the zeros)
+        scratch = torch.zeros(self._need, device=s["step"].device, dtype=torch.uint8)
         ctx._on_stream(lib().aipt_adamw_create, b"".join(records), len(records), _types()[kinds.pop()], _types()[copies.pop()], self.state_bits, ptr["m"], ptr["v"],
-                       ptr["m_scale"], ptr["v_scale"], ptr["step"], self.norm.data_ptr(), self._scratch.data_ptr(), self._scratch.numel(), C.byref(h))
+                       ptr["m_scale"], ptr["v_scale"], ptr["step"], self.norm.data_ptr(), scratch.data_ptr(), scratch.numel(), C.byref(h))
+        if self._captured:
+            self._kept.append(self._captured)
         self.close()
-        self._h, self._grads = h, grads
+        self._h, self._grads, self._scratch, self._captured = h, grads, scratch, None
+        for t in (scratch, self.norm):                   # every step runs on the context's stream, under whatever current stream it is called
+            if ctx._ext is not None:
+                t.record_stream(ctx._ext)
         self._held = [t for t in (*self._params, *grads, *self._copies, *s.values()) if t is not None]
         self._address = torch.Tensor.data_ptr
         self._at = list(map(self._address, self._held))
@@ -797,6 +813,8 @@ class AdamW:
             raise AiptError("adamw: a tensor's storage has moved: bind() the plan anew")
         if max_norm is not None and not max_norm > 0:
             raise AiptError(f"adamw: max_norm {max_norm}")
+        if not self._captured and self.ctx._capturing():
+            self._captured = [self._scratch, *(t.detach() for t in self._held)]      # the graph's: kept, wherever these tensors' storage moves
         self.ctx._on_stream(lib().aipt_adamw_step, self._h, lr, beta1, beta2, eps, 0.0 if max_norm is None else max_norm, seed & 0xffffffff)
 
     def close(self):

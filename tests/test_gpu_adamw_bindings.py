@@ -1,0 +1,74 @@
+"""AdamW plans whose tensors change: graphs, bindings and streams."""
+import pytest
+import torch
+
+from ai_path_tracer_denoiser_amd import api
+from tests.layer_util import context, generator
+from tests.test_gpu_adamw import LR, tensors
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [5000, 3, 257]
+
+
+def same(plan, other, p, q):
+    assert all(torch.equal(a, b) for a, b in zip(p, q))
+    assert all(torch.equal(a.view(torch.uint8), other.state()[k].view(torch.uint8)) for k, a in plan.state().items())
+
+
+@pytest.mark.parametrize("clip", [None, 0.05])
+@pytest.mark.parametrize("gtype", [torch.float32, torch.bfloat16])
+def test_a_captured_step_keeps_the_gradients_it_was_captured_with(gtype, clip):
+    gen, side = generator(40), torch.cuda.Stream()
+    ctx = api.Context(0, stream=side.cuda_stream)
+    p, g, new = tensors(gen, SIZES, 0.1), tensors(gen, SIZES, 0.01), tensors(gen, SIZES, 0.01, gtype)
+    q = [t.clone() for t in p]
+    want = context().adamw(q, [t.clone() for t in g])
+    plan, graph = ctx.adamw(p, g), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        plan.update(LR, max_norm=clip)
+    graph.replay()
+    torch.cuda.synchronize()
+    want.update(LR, max_norm=clip)
+    same(plan, want, p, q)
+    plan.bind(new)
+    for t in g:                                          # (the graph's gradients are kept by the plan, under whatever name)
+        assert any(t.data_ptr() == k.data_ptr() for k in plan._kept[0])
+    del g, t
+    filler = [torch.full((n,), 1e30, device="cuda") for n in SIZES for _ in range(8)]
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want.update(LR, max_norm=clip)
+        same(plan, want, p, q)
+    assert len(filler) == 24
+    plan.update(LR, max_norm=clip)                       # and the plan itself goes on with what is bound now
+    last = context().adamw(q, [t.clone() for t in new], state=want.state())
+    last.update(LR, max_norm=clip)
+    torch.cuda.synchronize()
+    same(plan, last, p, q)
+
+
+def test_a_plan_freed_while_its_steps_run():
+    """Steps are queued from another current stream than the plan was made on; its memory is not given to others before they are done."""
+    gen = generator(41)
+    start, g = tensors(gen, SIZES, 0.1), tensors(gen, SIZES, 0.01)
+    q = [t.clone() for t in start]
+    want = context().adamw(q, g)
+    for _ in range(3):
+        want.update(LR, max_norm=1.0)
+    ctx, side = api.Context(0), torch.cuda.Stream()
+    p = [t.clone() for t in start]
+    torch.cuda.synchronize()
+    plan = ctx.adamw(p, g)
+    with torch.cuda.stream(side):
+        big = torch.zeros(1 << 27, device="cuda")
+        for _ in range(20):
+            big.add_(1.0)
+        for _ in range(3):
+            plan.update(LR, max_norm=1.0)
+    del plan
+    junk = [torch.full((k * 512,), 0xff, device="cuda", dtype=torch.uint8) for k in range(1, 60)]
+    torch.cuda.synchronize()
+    assert len(junk) == 59 and all(torch.equal(a, b) for a, b in zip(p, q))

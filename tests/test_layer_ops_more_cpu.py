@@ -1,0 +1,55 @@
+"""The layer operators' host side: what the binding hands to the library, without a GPU."""
+import ctypes as C
+
+import torch
+
+from ai_path_tracer_denoiser_amd import api
+
+
+class Recorder(api.Context):
+    """A context of the CPU's tensors (device -1) that notes the calls instead of making them."""
+
+    def __init__(self):
+        self._h, self.device, self._ext, self.capturing, self.calls = None, -1, None, False, []
+
+    def _capturing(self):
+        return self.capturing
+
+    def _on_stream(self, entry, *args):
+        self.calls.append((entry, args))
+        if entry is api.lib().aipt_adamw_create:
+            args[-1]._obj.value = 1
+
+
+def adamw_plan(params, grads, bits=32):
+    """An AdamW of CPU tensors, as its constructor leaves it."""
+    counts = (C.c_longlong * len(params))(*[p.numel() for p in params])
+    total, plan = api.lib().aipt_adamw_state_elements(counts, len(params)), api.AdamW.__new__(api.AdamW)
+    plan.ctx, plan._h, plan._params, plan._copies, plan._decay, plan.state_bits = Recorder(), None, params, [None] * len(params), [0.0] * len(params), bits
+    plan._state = {"m": torch.zeros(total), "v": torch.zeros(total), "step": torch.zeros(1, dtype=torch.int32)}
+    plan.norm, plan._need, plan._captured, plan._kept = torch.zeros(1), api.lib().aipt_adamw_workspace(counts, len(params)), None, []
+    plan.close = lambda: None                            # (its handle is none)
+    plan.bind(grads)
+    return plan
+
+
+def workspaces(plan):
+    return [(args[-3], args[-2]) for entry, args in plan.ctx.calls if entry is api.lib().aipt_adamw_create]
+
+
+def test_each_binding_has_a_workspace_of_its_own():
+    """A graph reads the table of the binding that it captured a step of: a later one is written elsewhere, and the captured one's memory stays."""
+    p = [torch.zeros(300), torch.zeros(5)]
+    g = [[torch.zeros(300), torch.zeros(5)] for _ in range(4)]
+    plan = adamw_plan(p, g[0])
+    plan.ctx.capturing = True
+    plan.update(1e-3)
+    plan.ctx.capturing = False
+    held = plan._scratch
+    plan.bind(g[1])
+    plan.update(1e-3)                                    # not captured: this binding's memory may go
+    plan.bind([t.to(torch.bfloat16) for t in g[2]])
+    (a, size), (b, _), (c, _) = workspaces(plan)
+    assert size == plan._need and abs(a - b) >= size and abs(a - c) >= size
+    assert [k[0] is held for k in plan._kept] == [True] and held.data_ptr() == a
+    assert {t.data_ptr() for t in plan._kept[0]} >= {t.data_ptr() for t in p + g[0]}      # what the graph reads is not freed either
