@@ -225,9 +225,13 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
                 *(float4*)((float*)a.m + place) = make_float4(q.m[0], q.m[1], q.m[2], q.m[3]);
                 *(float4*)((float*)a.v + place) = make_float4(q.v[0], q.v[1], q.v[2], q.v[3]);
             } else {
-                const float mt = wave_max(fmaxf(fmaxf(fabsf(q.m[0]), fabsf(q.m[1])), fmaxf(fabsf(q.m[2]), fabsf(q.m[3]))));
-                const float vt = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
-                const bool ml = mt >= LIVE, vl = vt >= LIVE;
+                // (a NaN is the largest, and so the scale: the block's state is spoilt, not plausible; fabsf of the root for the sign of a NaN)
+                float mt = 0, vt = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) { mt = max_magnitude(mt, fabsf(q.m[i])); vt = max_magnitude(vt, fabsf(r[i])); }
+                mt = wave_max_magnitude(mt);
+                vt = wave_max_magnitude(vt);
+                const bool ml = !(mt < LIVE), vl = !(vt < LIVE);
                 const float mi = ml ? 1.f / mt * TOP : 0.f, vi = vl ? 1.f / vt * TOP : 0.f;
                 unsigned vq = 0;
 #pragma unroll

@@ -88,13 +88,18 @@ __device__ inline float wave_sum(float v) {
     v += __shfl_xor(v, 32);
     return v;
 }
-__device__ inline float wave_max(float v) {
-    v = fmaxf(v, rotate16<8>(v));
-    v = fmaxf(v, rotate16<4>(v));
-    v = fmaxf(v, rotate16<2>(v));
-    v = fmaxf(v, rotate16<1>(v));
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+// The largest of 64 magnitudes, each at least +0: as whole numbers they are in the same order, and a NaN is above infinity (the chip's maximum of
+// floats would pass over it).
+__device__ inline float wave_max_magnitude(float v) {
+    unsigned m = __float_as_uint(v);
+    auto rotate = [&](auto n) { m = max(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x120 + decltype(n)::value, 0xf, 0xf, true)); };
+    rotate(std::integral_constant<int, 8>{});
+    rotate(std::integral_constant<int, 4>{});
+    rotate(std::integral_constant<int, 2>{});
+    rotate(std::integral_constant<int, 1>{});
+    m = max(m, (unsigned)__shfl_xor((int)m, 16));
+    return __uint_as_float(max(m, (unsigned)__shfl_xor((int)m, 32)));
 }
+__device__ inline float max_magnitude(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
 
 }  // namespace aipt

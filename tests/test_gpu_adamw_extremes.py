@@ -1,0 +1,37 @@
+"""AdamW where the numbers are extreme: gradients and states at the ends of fp32, and what is none."""
+import pytest
+import torch
+
+from tests.layer_util import F, context, generator, within
+from tests.test_gpu_adamw import LR, make_state, segments, tensors, values
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [600, 7]                                         # blocks of 256, 256, 88 and 7 elements
+
+
+@pytest.mark.parametrize("bad", [float("nan"), -float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("gtype", [torch.float32, torch.bfloat16])
+def test_a_gradient_that_is_no_number_spoils_its_blocks_state_and_no_other(gtype, bad):
+    """8-bit state, no clipping: all of the block's m and v, none of another's; its element alone with 32 bits."""
+    for bits in (8, 32):
+        plans = []
+        for spoil in (False, True):
+            gen = generator(50)
+            p, g, st = tensors(gen, SIZES, 0.1), tensors(gen, SIZES, 0.01, gtype), make_state(gen, SIZES, bits, 5)
+            if spoil:
+                g[0][300] = bad
+            plan = context().adamw(p, g, state_bits=bits, state=st)
+            plan.update(LR, seed=3)
+            plans.append((p, st))
+        (p, good), (q, odd) = plans
+        spoilt = torch.zeros(1024, dtype=torch.bool, device="cuda")
+        spoilt[256:512] = True
+        if bits == 32:
+            spoilt[:] = False
+            spoilt[300] = True
+        for a, b in zip(values(good, bits), values(odd, bits)):
+            assert not torch.isfinite(b[spoilt]).any() and torch.equal(a[~spoilt], b[~spoilt])
+        assert torch.equal(p[1], q[1]) and not torch.isfinite(q[0][300])
+        plan.update(LR, seed=4)                          # a step later it is still seen
+        assert not any(torch.isfinite(v[spoilt][:1]).any() for v in values(odd, bits)) and torch.isfinite(q[1]).all()
