@@ -201,8 +201,10 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
                 const float gi = q.g[i] * factor;
                 q.m[i] = q.m[i] * a.beta1 + gi * a.omb1;
                 q.v[i] = q.v[i] * a.beta2 + gi * gi * a.omb2;
-                // the chip's root and reciprocal, an ulp each: the step is within 6 ulp of itself, far below the parameter's own (a root that is stored is exact)
-                r[i] = BITS == 8 ? sqrtf(q.v[i]) : __builtin_amdgcn_sqrtf(q.v[i]);
+                // the chip's root and reciprocal, an ulp each: the step is within 6 ulp of itself, far below the parameter's own (a root that is stored is exact).
+                // That root takes no subnormal numbers, which an eps of 0 would be felt by: they are scaled, by powers of two
+                const bool tiny = q.v[i] < 0x1p-96f;
+                r[i] = BITS == 8 ? sqrtf(q.v[i]) : __builtin_amdgcn_sqrtf(tiny ? q.v[i] * 0x1p64f : q.v[i]) * (tiny ? 0x1p-32f : 1.f);
                 q.p[i] = q.p[i] * keep - rate * q.m[i] * __builtin_amdgcn_rcpf(r[i] * root2 + a.eps);
             }
             if (q.wide) {

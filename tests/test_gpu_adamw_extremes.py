@@ -35,3 +35,21 @@ def test_a_gradient_that_is_no_number_spoils_its_blocks_state_and_no_other(gtype
         assert torch.equal(p[1], q[1]) and not torch.isfinite(q[0][300])
         plan.update(LR, seed=4)                          # a step later it is still seen
         assert not any(torch.isfinite(v[spoilt][:1]).any() for v in values(odd, bits)) and torch.isfinite(q[1]).all()
+
+
+def test_an_eps_of_nothing_and_subnormal_second_moments():
+    """32-bit state: the step lr m / sqrt(v) of a v below 2^-126 is what the formula says."""
+    n = 512
+    v0 = torch.logspace(-44, -30, n, dtype=torch.float64, device="cuda").float()
+    m0 = torch.full((n,), 1e-22, device="cuda")
+    p, g = [torch.zeros(n, device="cuda")], [torch.zeros(n, device="cuda")]
+    st = {"m": m0.clone(), "v": v0.clone(), "step": torch.full((1,), 1000, device="cuda", dtype=torch.int32)}
+    plan = context().adamw(p, g, weight_decay=0.0, state=st)
+    plan.update(LR, eps=0.0)
+    m, v = 0.9 * m0.double(), 0.999 * v0.double()
+    want = -LR / (1 - 0.9 ** 1001) * m / (v / (1 - 0.999 ** 1001)).sqrt()
+    # v = beta2 v0: beta2 is an fp32 number, within F of 0.999, and the product is rounded, by F or by half of 2^-149: together (1 + F)(1 + F) - 1, 2 F of it
+    # to first order, and 2^-150.  Its root feels half of that; beside it 8 roundings and the ulp each of root and reciprocal
+    ev = (2.0 ** -150 + 2 * F * v) / v
+    within(st["v"], v, ev * v, "v")
+    within(p[0], want, want.abs() * (ev / 2 / (1 - ev) + 12 * F), "p")
