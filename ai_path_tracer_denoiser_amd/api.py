@@ -513,6 +513,8 @@ class Context:
     # Tensors are torch's; the work runs on the context's stream.  Where that is not torch's current stream, the call waits for what is
     # queued there and what is queued there later waits for the call, so that tensors may be used, and freed, like in any torch program.
     def _on_stream(self, entry, *args):
+        if not self._h:
+            raise AiptError("the context is closed")
         if self._stream is None:
             import torch
             p = _P()
@@ -533,9 +535,12 @@ class Context:
         now.wait_stream(self._ext)
         self._ck(rc)
 
-    def _capturing(self) -> bool:
-        """Is torch's current stream of this device being captured?"""
+    def _capturing(self, stream=None) -> bool:
+        """Is this stream, or torch's current one of this device, being captured?"""
         import torch
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return torch._C._cuda_isCurrentStreamCapturing()
         if torch._C._cuda_getDevice() == self.device:
             return torch._C._cuda_isCurrentStreamCapturing()
         with torch.cuda.device(self.device):
@@ -759,7 +764,7 @@ class AdamW:
                 raise AiptError(f"adamw: state {k} is not contiguous")
         self._state = dict(state)
         self.norm = torch.zeros(1, device=dev)
-        self._need, self._captured, self._kept = need, None, []
+        self._need, self._captured, self._kept, self._homes = need, None, [], [None]
         self.bind(grads)
 
     def bind(self, grads):
@@ -793,9 +798,9 @@ class AdamW:
             self._kept.append(self._captured)
         self.close()
         self._h, self._grads, self._scratch, self._captured = h, grads, scratch, None
-        for t in (scratch, self.norm):                   # every step runs on the context's stream, under whatever current stream it is called
-            if ctx._ext is not None:
-                t.record_stream(ctx._ext)
+        home = None if ctx._ext is None else torch.cuda.current_stream(ctx.device)
+        if home not in self._homes:
+            self._homes.append(home)
         self._held = [t for t in (*self._params, *grads, *self._copies, *s.values()) if t is not None]
         self._address = torch.Tensor.data_ptr
         self._at = list(map(self._address, self._held))
@@ -817,8 +822,22 @@ class AdamW:
             self._captured = [self._scratch, *(t.detach() for t in self._held)]      # the graph's: kept, wherever these tensors' storage moves
         self.ctx._on_stream(lib().aipt_adamw_step, self._h, lr, beta1, beta2, eps, 0.0 if max_norm is None else max_norm, seed & 0xffffffff)
 
+    def _release(self):
+        """Memory of the plan may be freed next.  Every step runs on the context's stream, whatever stream it was queued from: the streams that the
+        memory was taken on wait for it, so that who gets it there does not write under a step.  (A closed context's stream is done.)"""
+        ctx = self.ctx
+        if not ctx._h or ctx._ext is None:
+            return
+        homes = [s for s in self._homes if s is not None and s != ctx._ext]
+        if homes and any(map(ctx._capturing, (ctx._ext, *homes))):
+            ctx._keep.append((self._scratch, self.norm, self._state))         # no waiting into a capture or out of one
+            return
+        for s in homes:
+            s.wait_stream(ctx._ext)
+
     def close(self):
         if getattr(self, "_h", None):
+            self._release()
             lib().aipt_adamw_destroy(self._h)
             self._h = None
 

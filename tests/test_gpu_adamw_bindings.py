@@ -71,4 +71,34 @@ def test_a_plan_freed_while_its_steps_run():
     del plan
     junk = [torch.full((k * 512,), 0xff, device="cuda", dtype=torch.uint8) for k in range(1, 60)]
     torch.cuda.synchronize()
-    assert len(junk) == 59 and all(torch.equal(a, b) for a, b in zip(p, q))
+    assert len(junk) == 59
+    for a, b in zip(p, q):
+        assert torch.equal(a, b)
+
+
+def test_a_plan_that_outlives_its_context_or_goes_in_a_capture():
+    gen = generator(42)
+    p, g = tensors(gen, SIZES, 0.1), tensors(gen, SIZES, 0.01)
+    ctx = api.Context(0)
+    plan = ctx.adamw(p, g)
+    plan.update(LR)
+    ctx.close()                                          # its stream is gone
+    with pytest.raises(api.AiptError, match="closed"):
+        plan.update(LR)
+    state = plan.state()
+    del plan
+    assert int(state["step"]) == 1
+    del state
+    side, x = torch.cuda.Stream(), torch.ones(1000, device="cuda")
+    captured = api.Context(0, stream=side.cuda_stream)
+    one, two = captured.adamw([t.clone() for t in p], g), captured.adamw([t.clone() for t in p], g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        one.update(LR)
+        two.close()
+        x.add_(1)
+    for k in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(one.state()["step"]) == k + 1 and float(x[0]) == k + 2

@@ -1,6 +1,7 @@
 """The layer operators' host side: what the binding hands to the library, without a GPU."""
 import ctypes as C
 
+import pytest
 import torch
 
 from ai_path_tracer_denoiser_amd import api
@@ -12,7 +13,7 @@ class Recorder(api.Context):
     def __init__(self):
         self._h, self.device, self._ext, self.capturing, self.calls = None, -1, None, False, []
 
-    def _capturing(self):
+    def _capturing(self, stream=None):
         return self.capturing
 
     def _on_stream(self, entry, *args):
@@ -27,7 +28,7 @@ def adamw_plan(params, grads, bits=32):
     total, plan = api.lib().aipt_adamw_state_elements(counts, len(params)), api.AdamW.__new__(api.AdamW)
     plan.ctx, plan._h, plan._params, plan._copies, plan._decay, plan.state_bits = Recorder(), None, params, [None] * len(params), [0.0] * len(params), bits
     plan._state = {"m": torch.zeros(total), "v": torch.zeros(total), "step": torch.zeros(1, dtype=torch.int32)}
-    plan.norm, plan._need, plan._captured, plan._kept = torch.zeros(1), api.lib().aipt_adamw_workspace(counts, len(params)), None, []
+    plan.norm, plan._need, plan._captured, plan._kept, plan._homes = torch.zeros(1), api.lib().aipt_adamw_workspace(counts, len(params)), None, [], [None]
     plan.close = lambda: None                            # (its handle is none)
     plan.bind(grads)
     return plan
@@ -53,3 +54,12 @@ def test_each_binding_has_a_workspace_of_its_own():
     assert size == plan._need and abs(a - b) >= size and abs(a - c) >= size
     assert [k[0] is held for k in plan._kept] == [True] and held.data_ptr() == a
     assert {t.data_ptr() for t in plan._kept[0]} >= {t.data_ptr() for t in p + g[0]}      # what the graph reads is not freed either
+
+
+def test_a_closed_context_takes_no_calls():
+    ctx = api.Context.__new__(api.Context)
+    ctx._h, ctx.device = None, -1
+    x = torch.zeros(4, 4)
+    for call in (lambda: ctx.linear(x, x, torch.zeros(4, 4)), lambda: ctx.block_norm(None, x, torch.zeros(4, 4)), lambda: ctx.linear_backward(x, x, x)):
+        with pytest.raises(api.AiptError, match="context is closed"):
+            call()
