@@ -40,7 +40,7 @@ struct AdamArgs {
     void *m, *v;
     float *ms, *vs;
     int* step;
-    const float* partial;            // sums of the gradients' squares to clip by, or NULL
+    const double* partial;           // sums of the gradients' squares to clip by, or NULL
     float* norm;                     // receives their root
     int npartial;
     float max_norm;
@@ -172,12 +172,12 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
     bool skip = false;
     if (a.partial) {                 // every workgroup adds the partial sums, in the same order: cheaper than a launch of its own
         double s = 0;
-        for (int i = threadIdx.x; i < a.npartial; i += 256) s += (double)a.partial[i];
+        for (int i = threadIdx.x; i < a.npartial; i += 256) s += a.partial[i];
 #pragma unroll
         for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
         if (lane == 0) norms[threadIdx.x >> 6] = s;
         __syncthreads();
-        const float norm = sqrtf((float)((norms[0] + norms[1]) + (norms[2] + norms[3])));
+        const float norm = (float)sqrt((norms[0] + norms[1]) + (norms[2] + norms[3]));
         factor = fminf(1.f, a.max_norm / (norm + 1e-6f));
         skip = !(norm <= 3.4028235e38f);                                   // inf and NaN
         if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
@@ -271,12 +271,13 @@ __global__ __launch_bounds__(256) void adamw_step(const AdamArgs a) {
 }
 
 // ---- the norm of all gradients: partial sums of squares in fixed places, which the step adds.  It reads the gradients once more than the
-// step itself would, and there is no way round it: no parameter may change before the last gradient has been seen.
+// step itself would, and there is no way round it: no parameter may change before the last gradient has been seen.  In fp64, which holds the square of
+// every gradient: in fp32 one of 1.9e19 made the norm infinite, and the step was skipped.
 struct NormArgs {
     const AdamTensor* tab;
     int n;
     unsigned blocks;
-    float* partial;                  // one for each workgroup
+    double* partial;                 // one for each workgroup
 };
 template <typename G>
 __global__ __launch_bounds__(256) void grad_square(const NormArgs a) {
@@ -284,7 +285,7 @@ __global__ __launch_bounds__(256) void grad_square(const NormArgs a) {
     const int lane = threadIdx.x & 63;
     const unsigned waves = gridDim.x * 4;
     int ti = 0;
-    float s = 0;
+    double s = 0;
     for (unsigned b = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)); b < a.blocks; b += waves) {
         long long at;
         const int left = locate(tab, a.n, b, lane, ti, at);
@@ -297,13 +298,14 @@ __global__ __launch_bounds__(256) void grad_square(const NormArgs a) {
             for (int i = 0; i < 4; i++) if (i < left) g[i] = (float)gp[i];
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) s += g[i] * g[i];
+        for (int i = 0; i < 4; i++) s = fma((double)g[i], (double)g[i], s);
     }
-    __shared__ float part[4];
-    s = wave_sum(s);
+    __shared__ double part[4];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
     if (lane == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) a.partial[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 }  // namespace aipt
@@ -315,7 +317,7 @@ struct aipt_adamw {
     int grad_type = 0, copy_type = 0, bits = 0;
     aipt::AdamArgs args = {};
     unsigned grid = 0;
-    float* partial = nullptr;        // in the caller's workspace
+    double* partial = nullptr;       // in the caller's workspace
 };
 
 namespace aipt {
@@ -345,7 +347,7 @@ long long aipt_adamw_state_elements(const long long* counts, int n) {
 
 long long aipt_adamw_workspace(const long long* counts, int n) {
     if (aipt_adamw_state_elements(counts, n) < 0) return AIPT_E_INVALID;
-    return (long long)(aipt::SCRATCH + aipt::GRID * sizeof(float) + (size_t)n * sizeof(aipt::AdamTensor));
+    return (long long)(aipt::SCRATCH + aipt::GRID * sizeof(double) + (size_t)n * sizeof(aipt::AdamTensor));
 }
 
 int aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, int grad_type, int copy_type, int state_bits,
@@ -404,7 +406,7 @@ int aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, in
         }
     }
     if (blocks > 0xffffff00ll) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: %lld blocks of 256 elements are too many", blocks);
-    const size_t need = aipt::SCRATCH + aipt::GRID * sizeof(float) + (size_t)n * sizeof(aipt::AdamTensor);
+    const size_t need = aipt::SCRATCH + aipt::GRID * sizeof(double) + (size_t)n * sizeof(aipt::AdamTensor);
     if (workspace_bytes < need) return fail(ctx, AIPT_E_INVALID, "aipt_adamw_create: workspace of %zu bytes, %zu are wanted", workspace_bytes, need);
     AIPT_NEED_CTX(ctx);
     std::vector<aipt::AdamTensor> tab;
@@ -422,7 +424,7 @@ int aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, in
         return fail(ctx, AIPT_E_NOMEM, "aipt_adamw_create: out of host memory");
     }
     a->ctx = ctx; a->grad_type = grad_type; a->copy_type = copy_type; a->bits = state_bits;
-    a->partial = (float*)((char*)d_workspace + aipt::SCRATCH);
+    a->partial = (double*)((char*)d_workspace + aipt::SCRATCH);
     aipt::AdamTensor* d_tab = (aipt::AdamTensor*)(a->partial + aipt::GRID);
     a->args.tab = d_tab; a->args.n = (int)tab.size(); a->args.blocks = (unsigned)blocks;
     a->args.m = m; a->args.v = v; a->args.ms = m_scale; a->args.vs = v_scale; a->args.step = step; a->args.ticket = (unsigned*)d_workspace; a->args.norm = norm;

@@ -53,3 +53,24 @@ def test_an_eps_of_nothing_and_subnormal_second_moments():
     ev = (2.0 ** -150 + 2 * F * v) / v
     within(st["v"], v, ev * v, "v")
     within(p[0], want, want.abs() * (ev / 2 / (1 - ev) + 12 * F), "p")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("gtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e20, 1e-30])
+def test_the_norm_of_gradients_whose_squares_are_no_floats(size, gtype, bits):
+    """1e20, whose square is beyond fp32's largest: clipped like any other; 1e-30, whose square is below its least: the norm is not zero."""
+    gen = generator(51)
+    p, g = tensors(gen, SIZES, 0.0), tensors(gen, SIZES, size, gtype)
+    plan = context().adamw(p, g, weight_decay=0.0, state_bits=bits)
+    plan.update(LR, max_norm=0.5)
+    norm = torch.cat([t.double() for t in g]).square().sum().sqrt()
+    # fp64 sums and root (errors of 2^-44 at these sizes), one rounding to fp32
+    assert abs(float(plan.norm) - float(norm)) <= 1.01 * F * float(norm)
+    assert int(plan.state()["step"]) == 1
+    clipped = [t.double() * min(1.0, 0.5 / (float(norm) + 1e-6)) for t in g]
+    # the first step of a plan is lr g / (|g| + eps), eps and |g| taken by a root each: 24 F of its terms, a factor's 4 F among them.
+    # Below 1e-18 the square is no normal number and the step g / eps: within v's root of nothing, which is |g| at most (and eps is 1e12 of them)
+    for a, c in zip(p, clipped):
+        want = -LR * c / (c.abs() + 1e-8)
+        within(a, want, want.abs() * 24 * F + (LR * c.abs() / 1e-8 if size < 1 else 0) + 1e-44, "p")
