@@ -726,7 +726,8 @@ class AdamW:
 
     params: contiguous float32 tensors; grads: as many, of the same sizes, all float32, bfloat16 or float16; copies: None, or bfloat16 or
     float16 tensors that receive the rounded parameters (an entry may be None); weight_decay: a number, or one for each tensor.  The plan is
-    bound to these tensors' memory: a gradient that is replaced by another tensor, or storage that moves, is bound anew with bind().
+    bound to these tensors' memory: a gradient that is replaced by another tensor, or storage that moves, is bound anew with bind(); where a gradient is its
+    parameter's .grad, update() refuses to step with one that is so no longer.
     state: None (zeros, step 0) or the dict that state() of an earlier plan of the same sizes returned, which goes on being updated in place:
     step int32 [1]; m and v float32 (state_bits 32), or m, v float8_e4m3fn with m_scale, v_scale float32 for each 256 elements (state_bits
     8; v holds the second moment's root); tensor i begins at element 256 * (number of 256-blocks of the tensors before it).
@@ -802,6 +803,7 @@ class AdamW:
         if home not in self._homes:
             self._homes.append(home)
         self._held = [t for t in (*self._params, *grads, *self._copies, *s.values()) if t is not None]
+        self._own_grads = [(p, g) for p, g in zip(self._params, grads) if p.is_leaf and p.grad is g]
         self._address = torch.Tensor.data_ptr
         self._at = list(map(self._address, self._held))
 
@@ -816,6 +818,9 @@ class AdamW:
             raise AiptError("adamw: the plan is closed")
         if list(map(self._address, self._held)) != self._at:
             raise AiptError("adamw: a tensor's storage has moved: bind() the plan anew")
+        for p, g in self._own_grads:
+            if p.grad is not g:
+                raise AiptError("adamw: a parameter's .grad is none or another tensor than the plan was bound to: bind() the plan anew, or keep gradients (zero_grad(set_to_none=False))")
         if max_norm is not None and not max_norm > 0:
             raise AiptError(f"adamw: max_norm {max_norm}")
         if not self._captured and self.ctx._capturing():

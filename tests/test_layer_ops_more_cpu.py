@@ -63,3 +63,30 @@ def test_a_closed_context_takes_no_calls():
     for call in (lambda: ctx.linear(x, x, torch.zeros(4, 4)), lambda: ctx.block_norm(None, x, torch.zeros(4, 4)), lambda: ctx.linear_backward(x, x, x)):
         with pytest.raises(api.AiptError, match="context is closed"):
             call()
+
+
+def test_a_gradient_that_was_replaced_is_not_stepped_with():
+    """zero_grad() and a backward pass make new gradients: the old ones, which the plan keeps alive, are refused."""
+    p = [torch.zeros(300, requires_grad=True), torch.zeros(5, requires_grad=True)]
+    (p[0].sum() * 2 + p[1].sum()).backward()
+    plan = adamw_plan(p, [t.grad for t in p])
+    steps = len(plan.ctx.calls)
+    plan.update(1e-3)
+    assert len(plan.ctx.calls) == steps + 1
+    for t in p:
+        t.grad.zero_()                                   # in place: the same gradients
+    (p[0].sum() * 3 + p[1].sum()).backward()
+    plan.update(1e-3)
+    opt = torch.optim.SGD(p)
+    opt.zero_grad()
+    with pytest.raises(api.AiptError, match="bind"):
+        plan.update(1e-3)
+    (p[0].sum() * 4 + p[1].sum()).backward()
+    with pytest.raises(api.AiptError, match="bind"):
+        plan.update(1e-3)
+    plan.bind([t.grad for t in p])
+    plan.update(1e-3)
+    assert len(plan.ctx.calls) == steps + 4              # three steps, and a binding
+    other = adamw_plan(p, [torch.zeros(300), torch.zeros(5)])      # gradients that are none of .grad are the caller's own
+    opt.zero_grad()
+    other.update(1e-3)
