@@ -511,7 +511,9 @@ class Context:
 
     # ------------------------------------------------------------------ layer operators
     # Tensors are torch's; the work runs on the context's stream.  Where that is not torch's current stream, the call waits for what is
-    # queued there and what is queued there later waits for the call, so that tensors may be used, and freed, like in any torch program.
+    # queued there and what is queued there later waits for the call, so that tensors may be used, and freed, like in any torch program.  Autograd
+    # records none of these calls (gradients are the _backward methods'), but it is told what they write: a tensor that it saved for a backward pass
+    # of its own and that is written since is refused there.
     def _on_stream(self, entry, *args):
         if not self._h:
             raise AiptError("the context is closed")
@@ -604,6 +606,7 @@ class Context:
                               *self._matrix("preact", preact, d, m, n), self._vector("bias", bias, d, n))
         hold, ptr, size = self._scratch(lib().aipt_linear_workspace, record)
         self._on_stream(lib().aipt_linear, record, ptr, size)
+        _written(y, preact)
         return y
 
     def linear_backward(self, dy, x, w, preact=None, act: str = "none", slope: float = 0.1, dx=None, dw=None, dbias=None):
@@ -626,6 +629,7 @@ class Context:
                                    *self._matrix("dw", dw, d, n, k), self._vector("dbias", dbias, d, n))
         hold, ptr, size = self._scratch(lib().aipt_linear_backward_workspace, record)
         self._on_stream(lib().aipt_linear_backward, record, ptr, size)
+        _written(dx, dw, dbias)
 
     def _rows(self, dtype, rows, c, **of):
         """the addresses and the row strides of optional [rows, c] with contiguous rows"""
@@ -678,6 +682,7 @@ class Context:
         record = _NORM.pack(t, _choice("kind", kind, NORMS), eps, c, rows, groups, *at, *strides, self._gates("gate", gate, d, c, groups),
                             *self._vectors(d, c, scale=scale, post_weight=post_weight, post_bias=post_bias, pre_weight=pre_weight, pre_bias=pre_bias), self._stats(stats, rows))
         self._on_stream(lib().aipt_block_norm, record)
+        _written(h, z, stats)
         return h, z
 
     def block_norm_backward(self, dh, dz, y, h, stats, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None, kind: str = "rms",
@@ -698,6 +703,7 @@ class Context:
                                  *vec[:4], *at[4:], *strides, self._gates("dgate", dgate, d, c, groups), *vec[4:])
         hold, ptr, size = self._scratch(lib().aipt_block_norm_backward_workspace, record)
         self._on_stream(lib().aipt_block_norm_backward, record, ptr, size)
+        _written(dx, dy, dgate, dscale, dpost_weight, dpost_bias, dpre_weight, dpre_bias)
 
     def adamw(self, params, grads, copies=None, weight_decay=0.01, state_bits: int = 32, state=None) -> "AdamW":
         """A plan for AdamW steps over these tensors (class AdamW)."""
@@ -713,6 +719,12 @@ def _types():
 
 
 _TYPES = None
+
+
+def _written(*tensors):
+    """These were written through their addresses, which torch does not see: their versions go on, as after an operation in place."""
+    import torch
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
 
 
 def _choice(name, value, choices):
@@ -803,6 +815,8 @@ class AdamW:
         if home not in self._homes:
             self._homes.append(home)
         self._held = [t for t in (*self._params, *grads, *self._copies, *s.values()) if t is not None]
+        bases = [t if t._base is None else t._base for t in (*self._params, *self._copies) if t is not None]      # views of one tensor count as it does
+        self._steps_on = list({id(t): t for t in bases}.values())
         self._own_grads = [(p, g) for p, g in zip(self._params, grads) if p.is_leaf and p.grad is g]
         self._address = torch.Tensor.data_ptr
         self._at = list(map(self._address, self._held))
@@ -826,6 +840,7 @@ class AdamW:
         if not self._captured and self.ctx._capturing():
             self._captured = [self._scratch, *(t.detach() for t in self._held)]      # the graph's: kept, wherever these tensors' storage moves
         self.ctx._on_stream(lib().aipt_adamw_step, self._h, lr, beta1, beta2, eps, 0.0 if max_norm is None else max_norm, seed & 0xffffffff)
+        _written(*self._steps_on)
 
     def _release(self):
         """Memory of the plan may be freed next.  Every step runs on the context's stream, whatever stream it was queued from: the streams that the

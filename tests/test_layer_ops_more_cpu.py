@@ -16,17 +16,20 @@ class Recorder(api.Context):
     def _capturing(self, stream=None):
         return self.capturing
 
+    def _scratch(self, entry, record):
+        return None, None, 0
+
     def _on_stream(self, entry, *args):
         self.calls.append((entry, args))
         if entry is api.lib().aipt_adamw_create:
             args[-1]._obj.value = 1
 
 
-def adamw_plan(params, grads, bits=32):
+def adamw_plan(params, grads, bits=32, copies=None):
     """An AdamW of CPU tensors, as its constructor leaves it."""
     counts = (C.c_longlong * len(params))(*[p.numel() for p in params])
     total, plan = api.lib().aipt_adamw_state_elements(counts, len(params)), api.AdamW.__new__(api.AdamW)
-    plan.ctx, plan._h, plan._params, plan._copies, plan._decay, plan.state_bits = Recorder(), None, params, [None] * len(params), [0.0] * len(params), bits
+    plan.ctx, plan._h, plan._params, plan._copies, plan._decay, plan.state_bits = Recorder(), None, params, copies or [None] * len(params), [0.0] * len(params), bits
     plan._state = {"m": torch.zeros(total), "v": torch.zeros(total), "step": torch.zeros(1, dtype=torch.int32)}
     plan.norm, plan._need, plan._captured, plan._kept, plan._homes = torch.zeros(1), api.lib().aipt_adamw_workspace(counts, len(params)), None, [], [None]
     plan.close = lambda: None                            # (its handle is none)
@@ -90,3 +93,26 @@ def test_a_gradient_that_was_replaced_is_not_stepped_with():
     other = adamw_plan(p, [torch.zeros(300), torch.zeros(5)])      # gradients that are none of .grad are the caller's own
     opt.zero_grad()
     other.update(1e-3)
+
+
+def test_autograd_is_told_what_is_written():
+    """A tensor that torch saved for its backward pass and that a call wrote since is refused there, not used with its new values."""
+    ctx, x, st = Recorder(), torch.randn(4, 4), torch.zeros(4, 4)
+    grads = {k: torch.zeros(4) for k in ("dscale", "dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias")}
+    y, z, dx, dw, db, dgate = (torch.zeros(4, 4) for _ in range(6))
+    calls = [(lambda: ctx.linear(x, x.clone(), y, preact=z, act="silu"), [y, z]), (lambda: ctx.linear_backward(x, x.clone(), x.clone(), dx=dx, dw=dw, dbias=db[0]), [dx, dw, db]),
+             (lambda: ctx.block_norm(x, x.clone(), y, z, stats=st, kind="layer"), [y, z, st]),
+             (lambda: ctx.block_norm_backward(x, x.clone(), x.clone(), x.clone(), st, kind="layer", dx=dx, dy=dw, dgate=dgate, **grads), [dx, dw, dgate, *grads.values()])]
+    p, copies = [torch.zeros(300), torch.zeros(600).view(2, 300)[1]], [torch.zeros(300, dtype=torch.bfloat16), None]
+    plan = adamw_plan(p, [torch.zeros(300), torch.zeros(300)], copies=copies)
+    calls.append((lambda: plan.update(1e-3), [*p, copies[0]]))
+    for call, written in calls:
+        before, inputs = [t._version for t in written], x._version
+        call()
+        assert all(t._version > v for t, v in zip(written, before)) and x._version == inputs
+    w = torch.ones(4, 4, requires_grad=True)
+    for call, t in ((calls[0][0], y), (calls[4][0], p[1])):
+        loss = (w.sum() * t).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
