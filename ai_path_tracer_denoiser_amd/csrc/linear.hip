@@ -36,25 +36,49 @@ struct GemmArgs {
 
 // 1 / (1 + e^-z) by the chip's exponential and reciprocal (an ulp each): z is within 2^-24 |z| of what it should be in the exponent
 __device__ inline float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f)); }
-// The normal distribution below z, by Abramowitz and Stegun 7.1.26 (erfc(x) = e^(-x^2) times a polynomial in 1 / (1 + p x), off by at most
-// 1.5e-7, and in the tail by as little of it): some 16 instructions where erff is 40, which a tile's 256 results a lane felt (wide bf16).
-// Beyond 16 the tail is 0.  e: e^(-z^2 / 2), which the slope wants too.
-__device__ inline float below(float z, float& e) {
-    const float a = fminf(fabsf(z), 16.f), t = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * 0.70710678f, 1.f));
-    e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);
-    const float q = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f), 0.5f * -0.284496736f), 0.5f * 0.254829592f) * t * e;
+// The normal distribution below z, and e = e^(-z^2 / 2), which the slope wants too.  With a = |z| and t = 1 / (1 + p a), the tail e erfcx(a / sqrt 2) / 2 is
+// e t P(t): P is a polynomial fitted (weighted least squares, the weights iterated until the largest error is least) for 0 <= a <= 16 by its RELATIVE
+// error, so that what is small is right in its digits too, down to the end of fp32's range.  16-bit results: seven coefficients, 1.2e-6, and an
+// exponent rounded in fp32 (a^2 2^-24): a fiftieth of fp16's half step at most, in some 20 instructions, which a tile's 256 results a lane feel.  Floats:
+// ten, 8.3e-9, and the exponent with what its rounding lost: within 9 x 2^-24 of the result altogether (0.5 (1 + erff), the usual form, is off by 1e-5 of
+// it at -3 and has no digits left at -5.5).
+template <bool FLOAT> __device__ inline float below(float z, float& e) {
+    constexpr float C = -0.72134752f, C_LO = -(float)(0.72134752044448170368 - 0.72134752f);      // -log2(e) / 2
+    const float a = fminf(fabsf(z), 16.f), s = a * a, w = s * C;
+    float q;
+    e = __builtin_amdgcn_exp2f(w);
+    if constexpr (FLOAT) {
+        const float lost = fmaf(fmaf(a, a, -s), C, fmaf(s, C_LO, fmaf(s, C, -w)));
+        e = fmaf(e, lost * 0.69314718f, e);
+        const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.38890873f, 1.f));
+        constexpr float P[] = {
+            0.155146554f, 0.15531975f, 0.129527479f, 0.100390859f, -0.0454047062f,
+            0.177593619f, -0.420847416f, 0.385778248f, -0.166079387f, 0.0285749864f};
+        q = P[9];
+#pragma unroll
+        for (int i = 8; i >= 0; i--) q = fmaf(q, t, P[i]);
+        q = q * t * e;
+    } else {
+        const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.36769553f, 1.f));
+        constexpr float P[] = {
+            0.146736786f, 0.145598784f, 0.136796817f, 0.0406556167f, 0.155492425f, -0.173597828f, 0.0483179614f};
+        q = P[6];
+#pragma unroll
+        for (int i = 5; i >= 0; i--) q = fmaf(q, t, P[i]);
+        q = q * t * e;
+    }
     return z > 0.f ? 1.f - q : q;
 }
-__device__ inline float act_of(float z, int act, float slope) {
+template <typename T> __device__ inline float act_of(float z, int act, float slope) {
     float e;
     switch (act) {
         case AIPT_ACT_LEAKY: return z > 0.f ? z : z * slope;
         case AIPT_ACT_SILU: return z * sigmoid(z);
-        case AIPT_ACT_GELU: return z * below(z, e);
+        case AIPT_ACT_GELU: return z * below<sizeof(T) == 4>(z, e);
     }
     return z;
 }
-__device__ inline float act_slope_of(float z, int act, float slope) {
+template <typename T> __device__ inline float act_slope_of(float z, int act, float slope) {
     switch (act) {
         case AIPT_ACT_LEAKY: return z > 0.f ? 1.f : slope;
         case AIPT_ACT_SILU: {
@@ -63,7 +87,7 @@ __device__ inline float act_slope_of(float z, int act, float slope) {
         }
         case AIPT_ACT_GELU: {
             float e;
-            const float p = below(z, e);
+            const float p = below<sizeof(T) == 4>(z, e);
             return fmaf(z, e * 0.39894228f, p);
         }
     }
@@ -73,7 +97,7 @@ __device__ inline float act_slope_of(float z, int act, float slope) {
 template <typename T> __device__ inline void epilogue(const GemmArgs& g, int i, int j, float z) {
     if (g.bias) z += (float)((const T*)g.bias)[g.bias_i ? i : j];
     if (g.pre) ((T*)g.pre)[i * g.pi + j * g.pj] = (T)z;
-    float y = act_of(z, g.act, g.slope);
+    float y = act_of<T>(z, g.act, g.slope);
     if (g.res) y += (float)((const T*)g.res)[i * g.ri + j * g.rj];
     ((T*)g.c)[i * g.cs + j] = (T)y;
 }
@@ -340,7 +364,7 @@ template <typename T, int ACT, bool ANY> __device__ inline void epilogue8(const 
         store((T*)g.pre + i * g.pi + j);
     }
 #pragma unroll
-    for (int e = 0; e < 8; e++) z[e] = act_of(z[e], ACT, g.slope);
+    for (int e = 0; e < 8; e++) z[e] = act_of<T>(z[e], ACT, g.slope);
     if (g.res) {
         const T* p = (const T*)g.res + i * g.ri + j;
         Oct r;
@@ -492,7 +516,7 @@ __device__ __forceinline__ void tile_of(const GemmArgs& g, const int block, cons
                 float z = *(AIPT_LDS float*)(slab + r * (WTJ * 4) + (((c >> 2) ^ (r & XM)) * 16) + (c & 3) * 4);
                 z += g.bias && g.bias_i ? (float)((const T*)g.bias)[ii - r0 + r] : bias;
                 if (pre) { *pre = (T)z; pre += RS * g.pi; }
-                z = act_of(z, g.act, g.slope);
+                z = act_of<T>(z, g.act, g.slope);
                 if (res) { z += (float)*res; res += RS * g.ri; }
                 *o = (T)z;
             }
@@ -727,7 +751,7 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g, const PackAr
             if (g.act != AIPT_ACT_NONE) {
                 const E z = *(const E*)zp;
 #pragma unroll
-                for (int i = 0; i < V; i++) d[i] *= act_slope_of((float)z.v[i], g.act, g.slope);
+                for (int i = 0; i < V; i++) d[i] *= act_slope_of<T>((float)z.v[i], g.act, g.slope);
             }
         }
         if (out) {
@@ -790,7 +814,7 @@ __global__ __launch_bounds__(256) void act_backward(const DzArgs g, const PackAr
 #pragma unroll
                         for (int i = 0; i < V; i++) {
                             float d = (float)dy[u].v[i];
-                            if (g.act != AIPT_ACT_NONE) d *= act_slope_of((float)z[u].v[i], g.act, g.slope);
+                            if (g.act != AIPT_ACT_NONE) d *= act_slope_of<T>((float)z[u].v[i], g.act, g.slope);
                             sum[i] += d;
                             o.v[i] = (T)d;
                         }
