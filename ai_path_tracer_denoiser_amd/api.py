@@ -66,6 +66,12 @@ class AABB(C.Structure):
 
 assert (C.sizeof(Geom), C.sizeof(Face), C.sizeof(Material), C.sizeof(Camera), C.sizeof(AABB)) == (248, 76, 44, 84, 24)
 
+
+class LinearPlan(C.Structure):
+    """aipt_linear_plan: which kernel a product is computed by"""
+    _fields_ = [(n, C.c_int) for n in ("tile_rows", "tile_columns", "load", "lines", "copied", "splits")]
+
+
 # every symbol include/aiptd.h declares: (name, restype, argtypes)
 _P = C.c_void_p
 ABI = [
@@ -125,8 +131,10 @@ ABI = [
     ("aipt_frame_prefetch", C.c_int, [_P, _P, C.c_int, C.c_int, C.c_uint32]),
     ("aipt_linear_workspace", C.c_int, [_P, C.c_char_p, C.POINTER(C.c_size_t)]),
     ("aipt_linear", C.c_int, [_P, C.c_char_p, _P, C.c_size_t]),
+    ("aipt_linear_planned", C.c_int, [_P, C.c_char_p, C.POINTER(LinearPlan)]),
     ("aipt_linear_backward_workspace", C.c_int, [_P, C.c_char_p, C.POINTER(C.c_size_t)]),
     ("aipt_linear_backward", C.c_int, [_P, C.c_char_p, _P, C.c_size_t]),
+    ("aipt_linear_backward_planned", C.c_int, [_P, C.c_char_p, C.POINTER(LinearPlan), C.POINTER(LinearPlan)]),
     ("aipt_block_norm", C.c_int, [_P, C.c_char_p]),
     ("aipt_block_norm_backward_workspace", C.c_int, [_P, C.c_char_p, C.POINTER(C.c_size_t)]),
     ("aipt_block_norm_backward", C.c_int, [_P, C.c_char_p, _P, C.c_size_t]),

@@ -1280,6 +1280,13 @@ static int backward_check(aipt_ctx* ctx, const char* me, const aipt_linear_grad_
     return rc;
 }
 
+static aipt_linear_plan planned(const Plan& p) {
+    if (!p.blocks) return {};
+    const int copied = (p.pack.m[0].chunks ? 1 : 0) | (p.pack.m[1].chunks ? 2 : 0), lines = (p.ak ? 1 : 0) | (p.bk ? 2 : 0);
+    if (p.tile < 0) return {0, p.rows, 16, lines, copied, p.g.splits};
+    return {p.tile ? TILES[p.tile].i : GT, p.tile ? TILES[p.tile].j : GT, !p.tile ? 0 : p.small ? 4 : 16, lines, copied, p.g.splits};
+}
+
 }  // namespace aipt
 
 using aipt::fail;
@@ -1291,6 +1298,14 @@ int aipt_linear_workspace(aipt_ctx* ctx, const aipt_linear_args* a, size_t* byte
     const int rc = aipt::forward_check(ctx, "aipt_linear_workspace", a, false);
     if (rc) return rc;
     *bytes = aipt::plan_forward(a).bytes();
+    return AIPT_OK;
+}
+
+int aipt_linear_planned(aipt_ctx* ctx, const aipt_linear_args* a, aipt_linear_plan* plan) {
+    if (!plan) return fail(ctx, AIPT_E_INVALID, "aipt_linear_planned: plan is NULL");
+    const int rc = aipt::forward_check(ctx, "aipt_linear_planned", a, false);
+    if (rc) return rc;
+    *plan = aipt::planned(aipt::plan_forward(a));
     return AIPT_OK;
 }
 
@@ -1324,6 +1339,16 @@ int aipt_linear_backward_workspace(aipt_ctx* ctx, const aipt_linear_grad_args* a
     const int rc = aipt::backward_check(ctx, "aipt_linear_backward_workspace", a, false);
     if (rc) return rc;
     *bytes = aipt::plan_backward(a, nullptr).bytes();
+    return AIPT_OK;
+}
+
+int aipt_linear_backward_planned(aipt_ctx* ctx, const aipt_linear_grad_args* a, aipt_linear_plan* dx, aipt_linear_plan* dw) {
+    if (!dx || !dw) return fail(ctx, AIPT_E_INVALID, "aipt_linear_backward_planned: dx or dw is NULL");
+    const int rc = aipt::backward_check(ctx, "aipt_linear_backward_planned", a, false);
+    if (rc) return rc;
+    const aipt::GradPlan p = aipt::plan_backward(a, nullptr);
+    *dx = aipt::planned(p.dx);
+    *dw = aipt::planned(p.dw);
     return AIPT_OK;
 }
 

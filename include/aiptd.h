@@ -366,6 +366,15 @@ typedef struct aipt_linear_args {
 int aipt_linear_workspace(aipt_ctx* ctx, const aipt_linear_args* args, size_t* bytes);      /* of a call with these very arguments: the pointers' alignment counts */
 int aipt_linear(aipt_ctx* ctx, const aipt_linear_args* args, void* d_workspace, size_t workspace_bytes);
 
+/* Which kernel such a call launches, for tests and timing.  tile_rows x tile_columns: a workgroup's part of the product (of its transpose where
+ * the result is planar); 0 x r: whole lines a wave, of up to r rows.  load: bytes that a lane loads at a time, 0 where each is checked for
+ * itself.  lines: 1 where the contraction is the contiguous axis of the first operand, 2 of the second, 3 of both.  copied: 1, 2 or 3
+ * likewise, operands copied to aligned lines first.  splits: parts of the contraction, 0 where nothing is to be computed. */
+typedef struct aipt_linear_plan {
+    int tile_rows, tile_columns, load, lines, copied, splits;
+} aipt_linear_plan;
+int aipt_linear_planned(aipt_ctx* ctx, const aipt_linear_args* args, aipt_linear_plan* plan);
+
 /* Gradients: dz = dy * act'(z);  dx = dz w  [m][k];  dw = dz^T x  [n][k];  dbias = sum over rows of dz  [n].  Outputs whose data is
  * NULL are not computed (the gradient of the residual is dy).  preact: the z that aipt_linear kept (not looked at with AIPT_ACT_NONE).  dz
  * is rounded to the element type before the two products (bf16 / fp16: an error of half a step of each factor, as of an input). */
@@ -379,6 +388,7 @@ typedef struct aipt_linear_grad_args {
 } aipt_linear_grad_args;
 int aipt_linear_backward_workspace(aipt_ctx* ctx, const aipt_linear_grad_args* args, size_t* bytes);
 int aipt_linear_backward(aipt_ctx* ctx, const aipt_linear_grad_args* args, void* d_workspace, size_t workspace_bytes);
+int aipt_linear_backward_planned(aipt_ctx* ctx, const aipt_linear_grad_args* args, aipt_linear_plan* dx, aipt_linear_plan* dw);
 
 /* The norms around a residual block, with its gate and residual scale.  For every row of c channels:
  *     u = norm(y) * post_weight + post_bias        the norm behind the block (y NULL: no block, h = x)

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from ai_path_tracer_denoiser_amd import api
+from tests import linear_cases as cases
 
 
 class Recorder(api.Context):
@@ -116,3 +117,45 @@ def test_autograd_is_told_what_is_written():
         call()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             loss.backward()
+
+
+@pytest.mark.parametrize("case", cases.FORWARD)
+def test_sizes_reach_the_kernels_they_are_for(case):
+    for layout in cases.LAYOUTS:
+        m, n, k = cases.sizes(case, layout)
+        for type in ((api.TYPE_F32,) if case[0] == 4 else (api.TYPE_BF16, api.TYPE_F16)):
+            p = cases.forward_plan(type, m, n, k, *layout)
+            assert (case[0], p.tile_rows, p.tile_columns, p.load, p.splits > 1) == case and not p.copied
+            assert p.lines == (layout[0] == "rows") + 2 * (layout[1] == "rows")
+            assert k * case[0] % 128 and -(-k * case[0] // 128) // p.splits >= 7 and m % p.tile_rows and n % p.tile_columns
+
+
+def test_every_kernel_of_the_table_has_its_sizes():
+    """All tiles by 16 bytes and the two that also load by 4, whole and split; floats by 256 x 256 are always split (128 x 128 is cheaper unsplit)."""
+    tiles = [(64, 64, 16), (64, 64, 4), (128, 128, 16), (256, 64, 16), (256, 32, 16), (256, 32, 4), (256, 256, 16)]
+    assert set(cases.FORWARD) == {(e, *t, s) for e in (2, 4) for t in tiles for s in (False, True)} - {(4, 256, 256, 16, False)}
+
+
+@pytest.mark.parametrize("case", cases.BACKWARD)
+def test_gradients_reach_the_kernels_they_are_for(case):
+    for type in ((api.TYPE_F32,) if case[0] == 4 else (api.TYPE_BF16, api.TYPE_F16)):
+        assert tuple((p.tile_rows, p.tile_columns, p.splits > 1) for p in cases.backward_plan(type, 2, *case[1:])) == cases.BACKWARD[case]
+
+
+@pytest.mark.parametrize("es,m,n,k,xpad,wpad", cases.ANY)
+def test_lines_far_apart(es, m, n, k, xpad, wpad):
+    for xl, wl in cases.any_layouts(m, k, xpad):
+        for type in ((api.TYPE_F32,) if es == 4 else (api.TYPE_BF16, api.TYPE_F16)):
+            assert cases.forward_plan(type, m, n, k, xl, wl, xpad=xpad, wpad=wpad).load == 0
+
+
+def test_plans_of_other_kinds():
+    for m, rows in ((1, 1), (2, 2), (3, 4), (8, 8)):
+        assert [getattr(cases.forward_plan(1, m, 2048, 2048, "rows", "rows"), f) for f in ("tile_rows", "tile_columns", "lines", "splits")] == [0, rows, 3, 1]
+    p = cases.forward_plan(2, 1375, 303, 909, "rows", "rows")
+    assert p.copied == 3 and p.load == 16
+    assert cases.forward_plan(0, 0, 40, 8, "rows", "rows").splits == 0
+    L, q = api.lib(), api.LinearPlan()
+    assert L.aipt_linear_planned(None, None, C.byref(q)) == -1 and "args is NULL" in L.aipt_last_error(None).decode()
+    assert L.aipt_linear_planned(None, api._LINEAR.pack(*[0] * 23), None) == -1 and "plan is NULL" in L.aipt_last_error(None).decode()
+    assert L.aipt_linear_backward_planned(None, None, C.byref(q), None) == -1 and "dw is NULL" in L.aipt_last_error(None).decode()
