@@ -912,7 +912,7 @@ static bool strides_ok(const aipt_matrix& m, long long n0, long long n1, bool ou
         const long long s = a ? m.col_stride : m.row_stride, n = a ? n1 : n0;
         if (n > 1 && (s < 0 || s > hi)) return false;
     }
-    if (out) {
+    if (out && n0 && n1) {           // (elements that are none do not coincide)
         if (n0 > 1 && n1 > 1) return (m.col_stride == 1 && m.row_stride >= n1) || (m.row_stride == 1 && m.col_stride >= n0);
         if (n0 > 1) return m.row_stride >= 1;
         if (n1 > 1) return m.col_stride >= 1;

@@ -159,3 +159,16 @@ def test_plans_of_other_kinds():
     assert L.aipt_linear_planned(None, None, C.byref(q)) == -1 and "args is NULL" in L.aipt_last_error(None).decode()
     assert L.aipt_linear_planned(None, api._LINEAR.pack(*[0] * 23), None) == -1 and "plan is NULL" in L.aipt_last_error(None).decode()
     assert L.aipt_linear_backward_planned(None, None, C.byref(q), None) == -1 and "dw is NULL" in L.aipt_last_error(None).decode()
+
+
+def test_outputs_of_no_elements_have_any_stride():
+    """A host's rows of n = 0 elements begin 0 apart: nothing is refused, and nothing but the missing context said."""
+    L, p = api.lib(), 1 << 40
+    for m, n, k in [(40, 0, 8), (0, 40, 8), (40, 30, 0), (0, 0, 0)]:
+        assert cases.forward_plan(0, m, n, k, "rows", "rows").splits == (1 if m and n else 0)
+        dx, dw = cases.backward_plan(0, 2, m, n, k)
+        assert (dx.splits, dw.splits) == (int(bool(m and k)), int(bool(n and k)))
+        record = api._LINEAR.pack(0, 0, 0.1, 0, m, n, k, p, k, 1, 2 * p, k, 1, 3 * p, n, 1, 0, 0, 0, 4 * p, n, 1, 0)
+        assert L.aipt_linear(None, record, None, 0) == -1 and "ctx is NULL" in L.aipt_last_error(None).decode()
+    record = api._LINEAR.pack(0, 0, 0.1, 0, 40, 2, 8, p, 8, 1, 2 * p, 8, 1, 3 * p, 0, 1, 0, 0, 0, 0, 0, 0, 0)
+    assert L.aipt_linear(None, record, None, 0) == -1 and "y: strides" in L.aipt_last_error(None).decode()
