@@ -107,7 +107,9 @@ typedef struct aipt_aabb {            /* MeshBoundingBox, sceneStructs.h:84-87, 
 
 /* ---- context ---------------------------------------------------------------------------------------------- */
 /* stream: an existing hipStream_t to enqueue on (e.g. the caller's torch stream), AIPT_STREAM_DEFAULT for HIP's default stream (the one
- * torch uses unless told otherwise), or NULL to create one. */
+ * torch uses unless told otherwise), or NULL to create one.  HIP lets nothing on a stream that it did not create as non-blocking run beside the default
+ * stream's work, and CU-masked streams cannot be created so: on AIPT_STREAM_DEFAULT the trace of aipt_frame_prefetch waits for what is queued there, and gives
+ * the same frames without the overlap.  Hosts that prefetch take a stream of their own. */
 #define AIPT_STREAM_DEFAULT ((void*)(intptr_t)-1)
 int  aipt_create(int device, void* stream, aipt_ctx** out);
 void aipt_destroy(aipt_ctx* ctx);
