@@ -102,3 +102,32 @@ def test_a_plan_that_outlives_its_context_or_goes_in_a_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert int(one.state()["step"]) == k + 1 and float(x[0]) == k + 2
+
+
+@pytest.mark.parametrize("clip", [None, 0.5])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_of_a_full_grid(bits, clip):
+    """More than 8192 blocks of 256: every workgroup there is, several rounds each, counts itself done, replay by replay, with a step that is skipped among them."""
+    gen, side = generator(43), torch.cuda.Stream()
+    sizes = [3_000_001, 33, 700]
+    ctx = api.Context(0, stream=side.cuda_stream)
+    p, g = tensors(gen, sizes, 0.1), tensors(gen, sizes, 0.01)
+    q, h = [t.clone() for t in p], [t.clone() for t in g]
+    plan, eager = ctx.adamw(p, g, state_bits=bits), context().adamw(q, h, state_bits=bits)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        plan.update(LR, max_norm=clip, seed=5)
+    steps = 0
+    for k in range(5):
+        for a, b in zip(g, h):
+            a.copy_(torch.randn(a.shape, generator=gen, device="cuda") * 0.01)
+            if k == 2 and clip:
+                a[-1] = float("nan")
+            b.copy_(a)
+        graph.replay()
+        eager.update(LR, max_norm=clip, seed=5)
+        torch.cuda.synchronize()
+        steps += not (k == 2 and clip)
+        assert int(plan.state()["step"]) == int(eager.state()["step"]) == steps
+        same(plan, eager, p, q)
