@@ -333,10 +333,11 @@ int aipt_frame_last_times(aipt_ctx* ctx, float* trace_ms, float* denoise_ms);
  * context's stream, asynchronous, no allocation, no synchronisation, no state kept between calls (but for the aipt_adamw plan): a
  * call may be captured into a hipGraph and replayed.  Scratch memory is the caller's: where an operator wants some, its _workspace
  * entry says how much, and two calls that may run at the same time (two streams, two graphs) are given different memory.  Every
- * sum is in fp32 and in an order that depends on the sizes alone: the same inputs give the same bits.  Outputs may not overlap inputs
+ * sum is in fp32 (of the gradients' norm in fp64) and in an order that sizes, strides and alignment alone decide: the same call gives the same bits
+ * whenever it runs; the same numbers laid out otherwise may differ by the sum's rounding.  Outputs may not overlap inputs
  * (AIPT_E_INVALID) but where an entry says so.  All tensors of a call have one element type; sums, statistics and the activation are
  * fp32, and a result is rounded once, to nearest even.  Arguments are checked before the context is looked at: with ctx NULL, which no call
- * accepts but the _workspace entries, aipt_last_error(NULL) says what else is wrong. */
+ * accepts but the _workspace and _planned entries, aipt_last_error(NULL) says what else is wrong. */
 #define AIPT_TYPE_F32  0
 #define AIPT_TYPE_BF16 1
 #define AIPT_TYPE_F16  2
@@ -379,7 +380,9 @@ int aipt_linear_planned(aipt_ctx* ctx, const aipt_linear_args* args, aipt_linear
 
 /* Gradients: dz = dy * act'(z);  dx = dz w  [m][k];  dw = dz^T x  [n][k];  dbias = sum over rows of dz  [n].  Outputs whose data is
  * NULL are not computed (the gradient of the residual is dy).  preact: the z that aipt_linear kept (not looked at with AIPT_ACT_NONE).  dz
- * is rounded to the element type before the two products (bf16 / fp16: an error of half a step of each factor, as of an input). */
+ * is rounded to the element type before the two products, whose matrix instructions take it so, like an input's (bf16 / fp16: half a step of each factor:
+ * a large bf16 gradient is 2.4e-3 off in the root mean square, of which rounding the result alone is 1.7e-3).  dbias adds it unrounded.  fp16: a dz beyond
+ * 65504 -- of a dy that close to it, or a slope above 1 -- is infinite, and one below 2^-14 has fewer digits: scale the loss. */
 typedef struct aipt_linear_grad_args {
     int type, act;
     float slope;
@@ -438,13 +441,15 @@ int aipt_block_norm_backward(aipt_ctx* ctx, const aipt_block_norm_grad_args* arg
  *     t = step + 1;  g = gradient * clip;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *     p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps);   copy = p rounded;   step = t
  * clip = min(1, max_norm / (norm + 1e-6)), norm the 2-norm of all gradients together; with max_norm <= 0 there is no clipping and the
- * norm is not computed.  If the norm is not finite the step changes nothing, not the step number either.
+ * norm is not computed.  If the norm is not finite the step changes nothing, not the step number either.  (It is added in fp64: the squares of finite
+ * gradients do not make it infinite.)  With eps 0 an element whose v is 0 becomes 0 / 0.
  * State: elements of tensor i begin at 256 * (number of 256-blocks of the tensors before it), each tensor's last block padded with
  * zeros; aipt_adamw_state_elements(counts, n) elements in all.  state_bits 32: m and v are float.  state_bits 8: m and sqrt(v) as OCP
  * e4m3 multiples of one float scale for each 256-block (its largest magnitude / 448): m rounded to nearest, the root up or down by
  * chance -- a change of 0.1 % of v must not be lost to rounding for ever -- with 24 bits of a hash of (seed, t, place), a positive
- * root never to zero.  A block whose largest magnitude is below 2^-100 is kept as zeros.  An infinite or NaN gradient spoils its
- * element's state (8 bits: its block's): clip, and such steps are skipped. */
+ * root never to zero.  A block whose largest magnitude is below 2^-100 is kept as zeros.  An infinite or NaN gradient, or one
+ * whose square is infinite in fp32, spoils its element's state (8 bits: its block's, infinite or NaN from then on): clip, and such steps are
+ * skipped, or steps are taken with what clipping left. */
 typedef struct aipt_adamw aipt_adamw;
 typedef struct aipt_adamw_tensor {
     float* param;
@@ -458,7 +463,9 @@ long long aipt_adamw_state_elements(const long long* counts, int n);
 long long aipt_adamw_workspace(const long long* counts, int n);      /* bytes; both: AIPT_E_INVALID for counts that are none */
 /* m, v: float (32 bits) or e4m3 bytes; m_scale, v_scale: float per 256-block (8 bits) or NULL; step: int, device, steps taken so far; norm: float,
  * device, receives the norm of a step that clips.  d_workspace: aipt_adamw_workspace bytes, ZEROED by the caller, the plan's own as long as
- * it (or a graph that captured a step of it) lives.  What a step writes must be apart from everything else the plan names. */
+ * it (or a graph that captured a step of it) lives.  What a step writes must be apart from everything else the plan names.  Making a plan writes a
+ * table of its tensors into the workspace and waits for the stream; it cannot be captured.  A step reads that table, destroyed plan or not: other
+ * tensors, or another plan, take another workspace where a graph holds a step. */
 int  aipt_adamw_create(aipt_ctx* ctx, const aipt_adamw_tensor* tensors, int n, int grad_type, int copy_type, int state_bits,
                        void* m, void* v, float* m_scale, float* v_scale, int* step, float* norm, void* d_workspace,
                        size_t workspace_bytes, aipt_adamw** out);
