@@ -233,12 +233,13 @@ struct NormBwd {
 };
 
 // A workgroup is a part: ROWS rows at a time, LANES lanes a row.  The vectors stay in registers (KEEP) and the next row's loads go out before this one's
-// sums are waited for (AHEAD) where there are registers for it beside the four sums a column.  WHOLE: gates change within the part -- A and B are added up gate by gate; else the
+// sums are waited for (AHEAD) where there are registers for it beside the four sums a column (a workgroup of 1 024 has half: 8 000 x 5 999 fp16 156 us with its
+// six columns a lane kept, 224 read again; layer 164 and 250).  WHOLE: gates change within the part -- A and B are added up gate by gate; else the
 // gate is one number a column and P = sum t yhat, T = sum t give A, B and Q at the end.
 template <typename T, int V, int N, int LANES, bool LAYER, bool WHOLE>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_bwd(const NormBwd a) {
     constexpr int THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;
-    constexpr bool AHEAD = !WHOLE && N * V * sizeof(T) <= 32 && N <= 8 && LANES <= 512, KEEP = !WHOLE && (LANES <= 512 ? N * V <= 16 : N * V * (LAYER ? 12 : 9) <= 80);
+    constexpr bool AHEAD = !WHOLE && N * V * sizeof(T) <= 32 && N <= 8 && LANES <= 512, KEEP = !WHOLE && N * V <= (LANES <= 512 ? 16 : 6);
     __shared__ float2 lds[2 * (THREADS / 64)];
     __shared__ float sums[LANES < 256 ? THREADS * V * N : 1];
     RowSum<LANES> row_sum{lds};
@@ -531,7 +532,11 @@ static_assert(sizeof(aipt_block_norm_args) == 152 && sizeof(aipt_block_norm_grad
 // ---- which kernel: the fewest lanes that hold a row; 16-byte accesses where every row begins at 16 bytes, two 16-bit elements where at 4 (74 400 rows of
 // 902 fp16: 111 us by twos; of 901 one by one: 166).  Up to 8 or 16 columns a lane, so that the vectors stay in registers: 4 lanes for 32 columns of 16
 // bits rather than 16 (65 964 rows: 13 -> 7 us, backward 25 -> 15), 256 for 2 048 rather than 64 with 32 columns each (16 384 rows: 92 -> 55), 512 for
-// 8 192 rather than 256 (8 192 rows: 237 -> 120), 256 for 999 fp16 by ones in the backward pass rather than 64 (20 000 rows: 187 -> 75).
+// 8 192 rather than 256 (8 192 rows: 237 -> 120), 256 for 999 fp16 by ones in the backward pass rather than 64 (20 000 rows: 187 -> 75).  One by one, six
+// columns a lane up to 6 144 (8 000 x 5 999 fp16: 125 us and backward 156, where eight and sixteen take 159 and 174; layer 151 and 164, 191 and 249), and in the
+// backward pass 512 lanes of sixteen up to 8 192, which 1 024 lanes have no registers for (6 000 x 7 999 fp16: 163 us, 882).
+// Whole gates (g*): a lane holds two sums a column more, and so few kernels serve them: half the shapes.  All of the others' would take 16 384 x 2 048 bf16 of 2 048
+// gates from 297 to 167 us and 8 192 x 8 192 from 829 to 302, but 200 000 x 101 from 262 to 382 and 200 000 x 32 from 194 to 226.
 struct NormShape { int v, n, lanes; };
 template <int S> static NormShape norm_shape(int c, int v, const int (&shapes)[S][2]) {
     for (auto& s : shapes) if (s[0] * s[1] * v >= c) return {v, s[1], s[0]};
