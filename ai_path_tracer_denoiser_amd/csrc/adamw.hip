@@ -5,8 +5,8 @@
 // launch over all tensors, a wave per 256-element block (16-byte accesses, and the block's scale is a wave's own maximum), and the step
 // number on the device, advanced by the last workgroup, so that neither the host nor a second launch has a part in it.  The table of tensors
 // lies in device memory, read by scalar loads: the kernel arguments of a launch hold a hundred at most.
-// Measured: 252 M parameters, 8-bit state, bf16 gradients and copies 886 us (4.6 TB/s; a large copy reaches 5.05); the denoiser's 1.5 M, 32-bit state,
-// 9 us and 4 for the norm.
+// Measured: 252 M parameters, 8-bit state, bf16 gradients and copies 890 us (4.5 TB/s; a large copy reaches 5.05); the denoiser's 1.5 M, 32-bit state,
+// 10 us and 4 for the norm.
 #include "layer_ops.h"
 
 #include <cmath>

@@ -12,7 +12,7 @@
 //     A = sum g t yhat,  B = sum g t,  Q = sum_(rows of a gate) t (w1 yhat + b1),  W = sum dz hhat,  V = sum dz
 // they are  dw1 = s A,  db1 = s B,  ds = w1 A + b1 B,  dgate = s Q,  dw2 = W,  db2 = V: four (five) sums a column, which each
 // workgroup keeps in registers over the rows it handles and writes once; a second, small launch adds those in a fixed order.
-// Measured, 16 384 x 4 096 bf16: forward 101 - 112 us (106 at a large copy's 5.05 TB/s), backward 167 us and 6 for the sums (160).
+// Measured, 16 384 x 4 096 bf16: forward 112 us (106 at a large copy's 5.05 TB/s), backward 166 us and 6 for the sums (160).
 #include "layer_ops.h"
 
 namespace aipt {
@@ -84,8 +84,8 @@ template <int LANES> struct RowSum {
 
 // A workgroup goes through rows, ROWS at a time, LANES lanes a row.  With up to 16 columns a lane (8 in a workgroup of 1 024, which has half the
 // registers), what multiplies and adds to a column (scale * gate * w1, scale * gate * b1, w2, b2) stays in registers until the gate changes, and
-// the next row's loads go out before this one's sums are waited for: 74 400 x 902 fp16 457 -> 111 us (106 at the rate of a copy), where the six
-// vectors were read again for each row in accesses as narrow as the rows'; 16 384 x 4 096 bf16 114 -> 101 us.
+// the next row's loads go out before this one's sums are waited for: 74 400 x 902 fp16 457 -> 119 us (106 at the rate of a copy), where the six
+// vectors were read again for each row in accesses as narrow as the rows'.
 template <typename T, int V, int N, int LANES>
 __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void block_norm_fwd(const NormFwd a) {
     constexpr int THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;

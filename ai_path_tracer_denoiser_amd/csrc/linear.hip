@@ -213,8 +213,10 @@ __global__ __launch_bounds__(256) void gemm_any(const GemmArgs g) {
 // at a time ran at 1.15 PFLOP/s).  LDS is a ring of S slots, each one operand's part of a pair, loaded there directly (buffer loads to LDS, 16
 // bytes a lane) in the order A(0) B(0) A(1) B(1) ...; the fragments of a step are read into registers while the matrix instructions of
 // the step before run.  One barrier a pair, before its second step: behind it every wave has read all of pair P, whose slots are
-// free for the loads S ahead of them, and pair P + 1 is visible.  The matrix instructions bound it: 4096^3 bf16 120 us (1.14 PFLOP/s; a large library
-// product 1.32), 8192 x 4096 by 16384 with gelu and two results 918.
+// free for the loads S ahead of them, and pair P + 1 is visible.  4096^3 bf16 112 us (1.23 PFLOP/s) with both operands' k contiguous, 118 - 122
+// otherwise (the library's product 95, 114 - 131); 8192 x 4096 by 16384 with gelu and two results 910.  The matrix pipes are busy 57 % of the cycles of that one
+// (the library's product alone 89 %; under such a load the chip's power limit takes the clock down, to 1.7 - 2.0 GHz here and 1.4 - 1.8 there): what is left between
+// the matrix instructions and the epilogue bound it.
 //   k contiguous:    rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 % 8): the 16 rows a read takes together lie on all banks
 //   rows contiguous: 64 lines (k) of the tile's rows, 32-byte group c of line k at c ^ (k % 4 + k / 8 % 2 * 4), read by the transposing
 //                    LDS load (16 lanes x 4 elements: lines 4q .. 4q + 3, 16 rows -> each lane its row's four); floats: 32 lines, 64-byte
@@ -226,7 +228,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 #define AIPT_LDS __attribute__((address_space(3)))
 
 // The accumulators are pinned to accumulation registers in place: with the builtin the compiler keeps a part of 64 of them in vector
-// registers and moves it to and fro each step (0.84 of 1.3 PFLOP/s).  settle() stands between these instructions and everything else that
+// registers and moves it to and fro each step (0.84 PFLOP/s of 1.2).  settle() stands between these instructions and everything else that
 // touches an accumulator: the compiler does not know that they are matrix instructions, whose results and sources want wait states.
 // float: 16 bytes are four k, one for each of four instructions (any order is a sum).
 template <typename T> struct Frag;
@@ -943,9 +945,9 @@ struct Plan {                        // a product as it will be launched, and th
 
 // The sizes of gemm_tile, and what they cost: `start` microseconds for a workgroup's first loads and its results, pair[c] for a pair of its steps
 // while c + 1 workgroups share the CU, of 16-bit types and of floats (whose matrix instructions bind).  Measured, bf16, where each wins:
-// 4096^3: 256 x 256 101 us, 128 x 128 121; 2048^3: 128 x 128 23, 64 x 64 29, 256 x 256 41; 1024^3: 64 x 64 8.4, 128 x 128 12; 942080 x 32 x 64:
-// 256 x 32 37, 64 x 64 60, 128 x 128 80; 942080 x 64 x 128: 256 x 64 86, 64 x 64 95, 128 x 128 101.  Floats, 2048^3: 256 x 32 137, 64 x 64 140,
-// 128 x 128 142; 942080 x 32 x 64: 256 x 32 93, 256 x 64 and 64 x 64 125.
+// 4096^3: 256 x 256 112 us, 128 x 128 120; 2048^3: 128 x 128 24, 64 x 64 30, 256 x 256 42; 1024^3: 64 x 64 8.0, 128 x 128 12; 942080 x 32 x 64:
+// 256 x 32 38, 64 x 64 59, 128 x 128 82; 942080 x 64 x 128: 256 x 64 86, 64 x 64 95, 128 x 128 99.  Floats, 2048^3: 256 x 32 137, 64 x 64 139,
+// 128 x 128 137; 942080 x 32 x 64: 256 x 32 89, 256 x 64 116, 64 x 64 121.
 static const struct Tile { int i, j, fit; double start, pair[2][3]; } TILES[] = {
     {},
     {256, 256, 1, 12, {{1.4, 0, 0}, {8.0, 0, 0}}},
