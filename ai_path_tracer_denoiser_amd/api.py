@@ -727,12 +727,16 @@ def _types():
 
 
 _TYPES = None
+_INCREMENT = None
 
 
 def _written(*tensors):
     """These were written through their addresses, which torch does not see: their versions go on, as after an operation in place."""
-    import torch
-    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+    global _INCREMENT
+    if _INCREMENT is None:
+        import torch
+        _INCREMENT = torch.autograd.graph.increment_version
+    _INCREMENT([t for t in tensors if t is not None])
 
 
 def _choice(name, value, choices):
